@@ -14,3 +14,5 @@ from dot_amd import __all__, __version__  # noqa: F401
 _sys.modules[__name__ + "._ops"] = _impl._ops
 _sys.modules[__name__ + ".sinkhorn"] = _impl.sinkhorn
 _sys.modules[__name__ + ".bidirectional_softmax"] = _impl.bidirectional_softmax
+_sys.modules[__name__ + ".routing"] = _impl.routing
+_sys.modules[__name__ + ".preference"] = _impl.preference

@@ -8,6 +8,14 @@ bidirectional-softmax operators with the reference's Python API:
     result.cost             # (B,)
     P = dot_amd.bidirectional_softmax(sim, tau=1.0)
 
+and the operators that language models put around a transport plan: routing of
+tokens to experts with its balance loss, log-probabilities of sequences and the
+preference loss over pairs or over a plan:
+
+    r = dot_amd.topk_routing(scores, k=2)        # weights, experts, counts, balance_loss
+    ratio = dot_amd.sequence_logp(logits, tokens, ref_logp=ref)
+    loss = dot_amd.preference_loss(ratio, plan=plan)
+
 The operators are registered as ``torch.ops.dot.*`` (the reference's schemas)
 and run hand-written HIP kernels behind the C ABI in ``include/dot_amd.h``.
 ``import dot`` gives the same API under the reference's package name.
@@ -29,6 +37,20 @@ from .bidirectional_softmax import (
     bidirectional_softmax_with_lengths,
     BidirectionalSoftmax,
 )
+from .routing import (
+    topk_routing,
+    balance_loss,
+    RoutingResult,
+    BalanceResult,
+    TopKRouting,
+    BalanceLoss,
+)
+from .preference import (
+    sequence_logp,
+    preference_loss,
+    SequenceLogp,
+    PreferenceLoss,
+)
 
 __version__ = "0.1.0"
 
@@ -42,4 +64,14 @@ __all__ = [
     "bidirectional_softmax",
     "bidirectional_softmax_with_lengths",
     "BidirectionalSoftmax",
+    "topk_routing",
+    "balance_loss",
+    "RoutingResult",
+    "BalanceResult",
+    "TopKRouting",
+    "BalanceLoss",
+    "sequence_logp",
+    "preference_loss",
+    "SequenceLogp",
+    "PreferenceLoss",
 ]

@@ -30,7 +30,10 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = os.environ.get("DOT_AMD_ARCH", "gfx950")
 
-HIP_SOURCES = ["sinkhorn.hip", "tiled.hip", "bidi.hip", "preflight.hip", "methods.hip", "capi.hip", "noalloc.hip"]
+HIP_SOURCES = ["sinkhorn.hip", "tiled.hip", "bidi.hip", "preflight.hip", "methods.hip", "capi.hip", "noalloc.hip",
+               "routing.hip", "seqlogp.hip", "preference.hip"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_training.cpp"]  # HIP tensors, through the C ABI
+CPU_SOURCES = ["cpu_ops.cpp", "cpu_training.cpp"]
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-mcode-object-version=5",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -86,19 +89,20 @@ def build_torch_ops():
     libdirs = ce.library_paths(device_type="cuda")
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    obj = os.path.join(OBJ, "torch_ops.o")
     cxx = os.environ.get("CXX", "g++")
-    _run([cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-Wno-deprecated-declarations",
-          *[f"-I{p}" for p in incs], f"-I{sysconfig.get_paths()['include']}",
-          "-c", os.path.join(CSRC, "torch_ops.cpp"), "-o", obj])
-    objs = [obj]
-    if os.path.exists(os.path.join(CSRC, "cpu_ops.cpp")):
-        cobj = os.path.join(OBJ, "cpu_ops.o")
-        _run([cxx, "-O3", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-              "-Wno-deprecated-declarations", *[f"-I{p}" for p in incs],
-              "-c", os.path.join(CSRC, "cpu_ops.cpp"), "-o", cobj])
-        objs.append(cobj)
+    incs_py = [*[f"-I{p}" for p in incs], f"-I{sysconfig.get_paths()['include']}"]
+
+    def compile_one(src):
+        obj = os.path.join(OBJ, os.path.splitext(src)[0] + ".o")
+        cpu = src in CPU_SOURCES
+        _run([cxx, "-O3" if cpu else "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+              *([] if cpu else ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]), "-Wno-deprecated-declarations",
+              *incs_py, "-c", os.path.join(CSRC, src), "-o", obj])
+        return obj
+
+    sources = TORCH_SOURCES + CPU_SOURCES
+    with ThreadPoolExecutor(max_workers=min(len(sources), os.cpu_count() or 1)) as ex:
+        objs = list(ex.map(compile_one, sources))
     out = os.path.join(PKG, "_C.so")
     _run([cxx, "-shared", "-o", out, *objs, f"-L{PKG}", "-ldot_amd",
           *[f"-L{p}" for p in libdirs], "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",

@@ -1,0 +1,287 @@
+// Log-probabilities of tokens from rows of logits, summed over sequences, and
+// the gradient of the logits.
+//
+// The forward reads each row once with a running maximum m and sum
+// s = sum_v 2^((x_v - m) k), k = log2(e) / tau; a row may be split over several
+// workgroups, whose (m, s) the second kernel joins.  That kernel also forms
+// the position's value and the sequence's sum in 64 bits: the log ratio of two
+// models is a small difference of large sums.  x - m is formed before the
+// scale, so rows at the type's lowest value give finite statistics.  The
+// backward reads the row again and writes dx_v = c (delta_va - p_v) with
+// p_v = 2^((x_v - m) k) / s.  Rows that are left out are not read.
+#pragma once
+
+#include "elem.cuh"
+#include "row.cuh"
+#include "wave.cuh"
+
+namespace dot_amd {
+namespace seqlogp {
+
+constexpr int kUnroll = 4;       // packs of a thread in flight
+constexpr int kJoinBlock = 1024; // threads of the per-sequence kernel
+
+struct Rows {
+    const void* logits;
+    int64_t sb, ss;
+    int B, S, V;
+    const void* tokens;
+    int tokens64;
+    const uint8_t* mask;
+    float k;     // log2(e) / tau
+    int splits;  // workgroups per row
+};
+
+// The token of a position, or -1 where it is left out.
+__device__ __forceinline__ int token_of(const Rows& r, int64_t at) {
+    if (r.mask && !r.mask[at]) return -1;
+    const int64_t t = int_at(r.tokens, r.tokens64, at);
+    return t >= 0 && t < r.V ? int(t) : -1;
+}
+
+template <class T>
+__device__ __forceinline__ const T* row_of(const Rows& r, int64_t at) {
+    const int64_t b = at / r.S, s = at - b * r.S;
+    return static_cast<const T*>(r.logits) + b * r.sb + s * r.ss;
+}
+
+// Split `part` of `parts` of a row of V elements: whole packs [p0, p1) after
+// `head` unaligned elements; the first split takes the head, the last the tail
+// from `tail` on.
+struct Span {
+    int head, tail;
+    int p0, p1;
+};
+template <class T>
+__device__ __forceinline__ Span span_of(const T* row, int V, int part, int parts) {
+    constexpr int PN = Pack<T>::N;
+    Span s;
+    const int off = int((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+    s.head = min((PN - off) % PN, V);
+    const int packs = (V - s.head) / PN;
+    s.tail = s.head + packs * PN;
+    const int per = (packs + parts - 1) / parts;
+    s.p0 = min(part * per, packs);
+    s.p1 = min(s.p0 + per, packs);
+    return s;
+}
+
+// Largest value and sum of 2^((x - m) k) so far; m = -inf: nothing but -inf.
+struct MaxSum {
+    float m = -__builtin_inff();
+    float s = 0.0f;
+    __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.0f : m; }
+    __device__ __forceinline__ void raise(float to, float k) {
+        const float old = m;
+        m = fmaxf(m, to);
+        s *= __builtin_amdgcn_exp2f((old - base()) * k);
+    }
+    __device__ __forceinline__ void add(float x, float k) { s += __builtin_amdgcn_exp2f((x - base()) * k); }
+    __device__ __forceinline__ void join(float om, float os, float k) {
+        raise(om, k);
+        s += os * __builtin_amdgcn_exp2f((om - base()) * k);
+    }
+};
+
+// Partial statistics of every row: parts[row * splits + split] = (m, s).
+template <class T>
+__global__ __launch_bounds__(kBlock) void row_stats(Rows r, float2* parts) {
+    __shared__ float sm[kWavesPerBlock], ss[kWavesPerBlock];
+    const int64_t at = blockIdx.x / unsigned(r.splits);
+    const int part = int(blockIdx.x % unsigned(r.splits));
+    if (token_of(r, at) < 0) return;
+    const T* row = row_of<T>(r, at);
+    const Span sp = span_of(row, r.V, part, r.splits);
+    const T* body = row + sp.head;
+    constexpr int PN = Pack<T>::N;
+    MaxSum a;
+    int p = sp.p0 + int(threadIdx.x);
+    for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
+        Pack<T> x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) x[u] = load_pack(body + int64_t(p + u * kBlock) * PN);
+        float most = to_float(x[0].v[0]);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < PN; ++i) most = fmaxf(most, to_float(x[u].v[i]));
+        a.raise(most, r.k);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < PN; ++i) a.add(to_float(x[u].v[i]), r.k);
+    }
+    for (; p < sp.p1; p += kBlock) {
+        const Pack<T> x = load_pack(body + int64_t(p) * PN);
+        float most = to_float(x.v[0]);
+#pragma unroll
+        for (int i = 1; i < PN; ++i) most = fmaxf(most, to_float(x.v[i]));
+        a.raise(most, r.k);
+#pragma unroll
+        for (int i = 0; i < PN; ++i) a.add(to_float(x.v[i]), r.k);
+    }
+    if (part == 0 && int(threadIdx.x) < sp.head) {
+        const float x = to_float(row[threadIdx.x]);
+        a.raise(x, r.k);
+        a.add(x, r.k);
+    }
+    if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) {
+        const float x = to_float(row[sp.tail + threadIdx.x]);
+        a.raise(x, r.k);
+        a.add(x, r.k);
+    }
+    const float m = wave_max(a.m);
+    a.raise(m, r.k);
+    const float s = wave_sum(a.s);
+    if (threadIdx.x % kWave == 0) {
+        sm[threadIdx.x / kWave] = m;
+        ss[threadIdx.x / kWave] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        MaxSum t;
+        for (int w = 0; w < kWavesPerBlock; ++w) t.join(sm[w], ss[w], r.k);
+        parts[blockIdx.x] = make_float2(t.m, t.s);
+    }
+}
+
+struct JoinArgs {
+    const void* ref;
+    int ref64, ref_per_token;
+    int reduction;
+    float* out;
+    float2* stats;
+    float* weight;
+};
+
+__device__ __forceinline__ double float_at(const void* p, int is64, int64_t i) {
+    return is64 ? static_cast<const double*>(p)[i] : double(static_cast<const float*>(p)[i]);
+}
+
+// One workgroup per sequence: joins the parts of its rows, forms the values of
+// its positions and their sum.
+template <class T>
+__global__ __launch_bounds__(kJoinBlock) void join(Rows r, const float2* parts, JoinArgs j) {
+    __shared__ double wsum[kJoinBlock / kWave];
+    __shared__ int wcount[kJoinBlock / kWave];
+    const int b = batch_of_block();
+    if (b >= r.B) return;
+    double sum = 0.0;
+    int count = 0;
+    for (int s = threadIdx.x; s < r.S; s += kJoinBlock) {
+        const int64_t at = int64_t(b) * r.S + s;
+        const int tok = token_of(r, at);
+        double v = 0.0;
+        if (tok >= 0) {
+            MaxSum t;
+            for (int i = 0; i < r.splits; ++i) {
+                const float2 p = parts[at * r.splits + i];
+                t.join(p.x, p.y, r.k);
+            }
+            const float x = to_float(row_of<T>(r, at)[tok]);
+            if (j.stats) j.stats[at] = make_float2(t.base(), 1.0f / t.s);
+            v = (double(x) - double(t.base())) * (double(r.k) * 0.693147180559945309417) - log(double(t.s));
+            if (j.ref && j.ref_per_token) v -= float_at(j.ref, j.ref64, at);
+            sum += v;
+            ++count;
+        }
+        if (j.reduction == DOT_REDUCE_NONE) j.out[at] = float(v);
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        sum += __shfl_xor(sum, d);
+        count += __shfl_xor(count, d);
+    }
+    if (threadIdx.x % kWave == 0) {
+        wsum[threadIdx.x / kWave] = sum;
+        wcount[threadIdx.x / kWave] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        int n = 0;
+        for (int w = 0; w < kJoinBlock / kWave; ++w) {
+            t += wsum[w];
+            n += wcount[w];
+        }
+        const double weight = j.reduction == DOT_REDUCE_MEAN ? 1.0 / (n > 0 ? n : 1) : 1.0;
+        if (j.weight) j.weight[b] = float(weight);
+        if (j.reduction != DOT_REDUCE_NONE) {
+            t *= weight;
+            if (j.ref && !j.ref_per_token) t -= float_at(j.ref, j.ref64, b);
+            j.out[b] = float(t);
+        }
+    }
+}
+
+struct GradArgs {
+    float inv_tau;
+    int reduction;
+    const float2* stats;
+    const float* weight;
+    const float* grad_out;
+    int grad_out_scalar;
+    void* grad;
+};
+
+// dx of one span of a row.
+template <class T>
+__global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
+    const int64_t at = blockIdx.x / unsigned(r.splits);
+    const int part = int(blockIdx.x % unsigned(r.splits));
+    constexpr int PN = Pack<T>::N;
+    const int tok = token_of(r, at);
+    T* out = static_cast<T*>(g.grad) + at * r.V;
+    if (tok < 0) {
+        const Span sp = span_of(out, r.V, part, r.splits);
+        const Pack<T> zero{};
+        for (int p = sp.p0 + int(threadIdx.x); p < sp.p1; p += kBlock)
+            store_pack_stream(out + sp.head + int64_t(p) * PN, zero);
+        if (part == 0 && int(threadIdx.x) < sp.head) out[threadIdx.x] = T{};
+        if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) out[sp.tail + threadIdx.x] = T{};
+        return;
+    }
+    const T* row = row_of<T>(r, at);
+    const int64_t b = at / r.S;
+    const float2 st = g.stats[at];
+    const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
+    const float c = up * g.weight[b] * g.inv_tau;
+    const float scale = -c * st.y;
+    auto value = [&](float x, int v) {
+        const float y = __builtin_amdgcn_exp2f((x - st.x) * r.k) * scale;
+        return v == tok ? c + y : y;
+    };
+    const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+    const Span sp = span_of(out, r.V, part, r.splits);
+    auto pack_in = [&](int p) {
+        const T* at_p = row + sp.head + int64_t(p) * PN;
+        if (together) return load_pack(at_p);
+        Pack<T> x;  // a strided view whose rows are not aligned as the gradient's
+#pragma unroll
+        for (int i = 0; i < PN; ++i) x.v[i] = at_p[i];
+        return x;
+    };
+    auto pack_out = [&](int p, const Pack<T>& x) {
+        const int v0 = sp.head + p * PN;
+        Pack<T> y;
+#pragma unroll
+        for (int i = 0; i < PN; ++i) y.v[i] = from_float<T>(value(to_float(x.v[i]), v0 + i));
+        store_pack_stream(out + v0, y);
+    };
+    int p = sp.p0 + int(threadIdx.x);
+    for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
+        Pack<T> x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) x[u] = pack_in(p + u * kBlock);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) pack_out(p + u * kBlock, x[u]);
+    }
+    for (; p < sp.p1; p += kBlock) pack_out(p, pack_in(p));
+    if (part == 0 && int(threadIdx.x) < sp.head)
+        out[threadIdx.x] = from_float<T>(value(to_float(row[threadIdx.x]), int(threadIdx.x)));
+    const int v = sp.tail + int(threadIdx.x);
+    if (part == r.splits - 1 && v < r.V) out[v] = from_float<T>(value(to_float(row[v]), v));
+}
+
+}  // namespace seqlogp
+}  // namespace dot_amd

@@ -1,0 +1,351 @@
+// PyTorch binding of the routing, sequence log-probability and preference
+// entry points of the C ABI (torch.ops.dot_amd.*), for HIP tensors; the CPU
+// implementations are in cpu_training.cpp.  The Python functions check
+// arguments; the operators check again what a kernel's indexing relies on.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include <string>
+#include <vector>
+
+#include "../../include/dot_amd.h"
+
+namespace {
+
+using at::Tensor;
+using c10::optional;
+
+void check_rc(int rc, const char* what) {
+    TORCH_CHECK(rc == DOT_OK, what, " failed (code ", rc, "): ", dot_last_error());
+}
+
+dot_stream_t stream_of(const Tensor& t) {
+    return reinterpret_cast<dot_stream_t>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
+}
+
+Tensor workspace(size_t bytes, const Tensor& like) {
+    return at::empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, like.options().dtype(at::kByte));
+}
+
+int dtype_tag(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return DOT_F32;
+        case at::kHalf: return DOT_F16;
+        case at::kBFloat16: return DOT_BF16;
+        default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16");
+    }
+}
+
+int to_int(int64_t v, const char* name) {
+    TORCH_CHECK(v >= 0 && v <= INT32_MAX, name, " out of range");
+    return int(v);
+}
+
+void check_on(const Tensor& t, const Tensor& with, const char* name) {
+    TORCH_CHECK(t.device() == with.device(), name, " must be on ", with.device(), ", got ", t.device());
+}
+
+// Rows of unit stride, in place where they are so already.
+Tensor unit_rows(const Tensor& t) { return t.stride(2) == 1 || t.size(2) <= 1 ? t : t.contiguous(); }
+
+const float* floats(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+Tensor f32c(const optional<Tensor>& t, const Tensor& like, const char* name) {
+    if (!t.has_value()) return Tensor();
+    check_on(*t, like, name);
+    return t->to(at::kFloat).contiguous();
+}
+
+// An upstream gradient and whether it is one value for all (an expanded
+// scalar, as the gradient of a sum is).
+Tensor upstream(const Tensor& g, const Tensor& like, int& scalar) {
+    check_on(g, like, "grad");
+    bool one = g.numel() > 1;
+    for (int64_t d = 0; d < g.dim(); ++d) one = one && (g.stride(d) == 0 || g.size(d) == 1);
+    scalar = one;
+    if (one) return g.as_strided({1}, {1}).to(at::kFloat);
+    return g.to(at::kFloat).contiguous();
+}
+
+Tensor mask_of(const optional<Tensor>& mask, const Tensor& x) {
+    if (!mask.has_value()) return Tensor();
+    check_on(*mask, x, "mask");
+    TORCH_CHECK(mask->scalar_type() == at::kBool && mask->dim() == 2 && mask->size(0) == x.size(0) &&
+                    mask->size(1) == x.size(1),
+                "mask must be bool of the leading two sizes");
+    return mask->contiguous();
+}
+const uint8_t* mask_ptr(const Tensor& m) {
+    return m.defined() ? reinterpret_cast<const uint8_t*>(m.const_data_ptr()) : nullptr;
+}
+
+Tensor ints_of(const Tensor& t, const Tensor& like, const char* name) {
+    check_on(t, like, name);
+    TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+    return t.contiguous();
+}
+
+void check_rows(const Tensor& x, const char* name) {
+    TORCH_CHECK(x.device().is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(x.dim() == 3, name, " must be 3D");
+}
+
+// -> [weights, experts, counts, tokens, loss]; weights and experts are empty for given experts
+std::vector<Tensor> routing_forward_op(Tensor scores_, int64_t k, int64_t scoring, bool normalize,
+                                       optional<Tensor> bias_, optional<Tensor> mask_, optional<Tensor> given_) {
+    check_rows(scores_, "scores");
+    c10::OptionalDeviceGuard guard(scores_.device());
+    const Tensor scores = unit_rows(scores_);
+    const int64_t B = scores.size(0), N = scores.size(1), E = scores.size(2);
+    const Tensor mask = mask_of(mask_, scores);
+    const Tensor bias = f32c(bias_, scores, "bias");
+    TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == E), "bias must have shape [E]");
+    Tensor given;
+    if (given_.has_value()) {
+        given = ints_of(*given_, scores, "experts");
+        TORCH_CHECK(given.dim() == 3 && given.size(0) == B && given.size(1) == N && given.size(2) == k,
+                    "experts must have shape [B, N, k]");
+    }
+    const auto f32 = scores.options().dtype(at::kFloat), i32 = scores.options().dtype(at::kInt);
+    const bool select = !given.defined();
+    Tensor weights = at::empty(select ? at::IntArrayRef({B, N, k}) : at::IntArrayRef({0}), f32);
+    Tensor experts = at::empty(select ? at::IntArrayRef({B, N, k}) : at::IntArrayRef({0}), i32);
+    Tensor counts = at::empty({B, E}, i32), tokens = at::empty({B}, i32), loss = at::empty({B}, f32);
+    dot_routing_fwd_args a{};
+    a.dtype = dtype_tag(scores, "scores");
+    a.B = to_int(B, "B");
+    a.N = to_int(N, "N");
+    a.E = to_int(E, "E");
+    a.k = to_int(k, "k");
+    a.scores = scores.const_data_ptr();
+    a.stride_b = scores.stride(0);
+    a.stride_n = scores.stride(1);
+    a.scoring = int(scoring);
+    a.normalize = normalize;
+    a.bias = floats(bias);
+    a.mask = mask_ptr(mask);
+    // an empty batch has no entries to point at: any address says "given"
+    a.given = select ? nullptr : given.numel() ? given.const_data_ptr() : counts.const_data_ptr();
+    a.given_is_int64 = !select && given.scalar_type() == at::kLong;
+    a.weights = select ? weights.data_ptr<float>() : nullptr;
+    a.experts = select ? experts.data_ptr<int32_t>() : nullptr;
+    a.counts = counts.data_ptr<int32_t>();
+    a.tokens = tokens.data_ptr<int32_t>();
+    a.loss = loss.data_ptr<float>();
+    a.workspace_bytes = dot_routing_forward_workspace_bytes(a.B, a.N, a.E);
+    Tensor ws = workspace(a.workspace_bytes, scores);
+    a.workspace = ws.data_ptr();
+    check_rc(dot_routing_forward(&a, stream_of(scores)), "dot_routing_forward");
+    return {weights, experts, counts, tokens, loss};
+}
+
+Tensor routing_backward_op(Tensor scores_, int64_t k, int64_t scoring, bool normalize, optional<Tensor> mask_,
+                           Tensor counts, Tensor tokens, optional<Tensor> grad_loss_, optional<Tensor> weights,
+                           optional<Tensor> experts, optional<Tensor> grad_weights_) {
+    check_rows(scores_, "scores");
+    c10::OptionalDeviceGuard guard(scores_.device());
+    const Tensor scores = unit_rows(scores_);
+    const int64_t B = scores.size(0), N = scores.size(1), E = scores.size(2);
+    const Tensor mask = mask_of(mask_, scores);
+    check_on(counts, scores, "counts");
+    check_on(tokens, scores, "tokens");
+    TORCH_CHECK(counts.scalar_type() == at::kInt && counts.is_contiguous() && counts.numel() == B * E &&
+                    tokens.scalar_type() == at::kInt && tokens.is_contiguous() && tokens.numel() == B,
+                "counts and tokens must be as the forward returned them");
+    Tensor grad = at::empty({B, N, E}, scores.options().memory_format(at::MemoryFormat::Contiguous));
+    dot_routing_bwd_args a{};
+    Tensor gl, gw, w, e;
+    if (grad_loss_.has_value()) {
+        gl = upstream(*grad_loss_, scores, a.grad_loss_scalar);
+        TORCH_CHECK(grad_loss_->numel() == B, "grad_loss must have shape [B]");
+    }
+    if (grad_weights_.has_value()) {
+        TORCH_CHECK(weights.has_value() && experts.has_value(), "grad_weights needs weights and experts");
+        gw = f32c(grad_weights_, scores, "grad_weights");
+        w = f32c(weights, scores, "weights");
+        e = ints_of(*experts, scores, "experts");
+        TORCH_CHECK(gw.numel() == B * N * k && w.numel() == B * N * k && e.numel() == B * N * k &&
+                        e.scalar_type() == at::kInt,
+                    "weights, experts and grad_weights must have shape [B, N, k]");
+    }
+    a.scores = scores.const_data_ptr();
+    a.dtype = dtype_tag(scores, "scores");
+    a.stride_b = scores.stride(0);
+    a.stride_n = scores.stride(1);
+    a.B = to_int(B, "B");
+    a.N = to_int(N, "N");
+    a.E = to_int(E, "E");
+    a.k = to_int(k, "k");
+    a.scoring = int(scoring);
+    a.normalize = normalize;
+    a.mask = mask_ptr(mask);
+    a.counts = counts.const_data_ptr<int32_t>();
+    a.tokens = tokens.const_data_ptr<int32_t>();
+    a.grad_loss = floats(gl);
+    a.weights = floats(w);
+    a.experts = e.defined() ? e.const_data_ptr<int32_t>() : nullptr;
+    a.grad_weights = floats(gw);
+    a.grad_scores = grad.data_ptr();
+    check_rc(dot_routing_backward(&a, stream_of(scores)), "dot_routing_backward");
+    return grad;
+}
+
+template <class A>
+void fill_rows(A& a, const Tensor& logits, const Tensor& tokens, const Tensor& mask, double tau, int64_t reduction) {
+    a.logits = logits.const_data_ptr();
+    a.dtype = dtype_tag(logits, "logits");
+    a.stride_b = logits.stride(0);
+    a.stride_s = logits.stride(1);
+    a.B = to_int(logits.size(0), "B");
+    a.S = to_int(logits.size(1), "S");
+    a.V = to_int(logits.size(2), "V");
+    a.tokens = tokens.const_data_ptr();
+    a.tokens_are_int64 = tokens.scalar_type() == at::kLong;
+    a.mask = mask_ptr(mask);
+    a.tau = float(tau);
+    a.reduction = int(reduction);
+}
+
+Tensor tokens_of(const Tensor& tokens, const Tensor& logits) {
+    Tensor t = ints_of(tokens, logits, "tokens");
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == logits.size(0) && t.size(1) == logits.size(1),
+                "tokens must have shape [B, S]");
+    return t;
+}
+
+// -> [out, row_stats [B, S, 2], weight [B]]
+std::vector<Tensor> sequence_logp_forward_op(Tensor logits_, Tensor tokens_, optional<Tensor> ref_,
+                                             optional<Tensor> mask_, double tau, int64_t reduction, bool keep) {
+    check_rows(logits_, "logits");
+    c10::OptionalDeviceGuard guard(logits_.device());
+    const Tensor logits = unit_rows(logits_);
+    const int64_t B = logits.size(0), S = logits.size(1);
+    const Tensor tokens = tokens_of(tokens_, logits), mask = mask_of(mask_, logits);
+    Tensor ref;
+    if (ref_.has_value()) {
+        check_on(*ref_, logits, "ref_logp");
+        ref = ref_->scalar_type() == at::kDouble ? ref_->contiguous() : ref_->to(at::kFloat).contiguous();
+        TORCH_CHECK((ref.dim() == 1 && ref.size(0) == B) || (ref.dim() == 2 && ref.size(0) == B && ref.size(1) == S),
+                    "ref_logp must have shape [B] or [B, S]");
+    }
+    const auto f32 = logits.options().dtype(at::kFloat);
+    Tensor out = at::empty(reduction == DOT_REDUCE_NONE ? at::IntArrayRef({B, S}) : at::IntArrayRef({B}), f32);
+    Tensor stats = at::empty(keep ? at::IntArrayRef({B, S, 2}) : at::IntArrayRef({0}), f32);
+    Tensor weight = at::empty({keep ? B : 0}, f32);
+    dot_seqlogp_fwd_args a{};
+    fill_rows(a, logits, tokens, mask, tau, reduction);
+    a.ref = ref.defined() ? ref.const_data_ptr() : nullptr;
+    a.ref_is_f64 = ref.defined() && ref.scalar_type() == at::kDouble;
+    a.ref_per_token = ref.defined() && ref.dim() == 2;
+    a.out = out.data_ptr<float>();
+    a.row_stats = keep ? stats.data_ptr<float>() : nullptr;
+    a.weight = keep ? weight.data_ptr<float>() : nullptr;
+    a.workspace_bytes = dot_seqlogp_forward_workspace_bytes(a.B, a.S, a.V, a.dtype);
+    Tensor ws = workspace(a.workspace_bytes, logits);
+    a.workspace = ws.data_ptr();
+    check_rc(dot_seqlogp_forward(&a, stream_of(logits)), "dot_seqlogp_forward");
+    return {out, stats, weight};
+}
+
+Tensor sequence_logp_backward_op(Tensor logits_, Tensor tokens_, optional<Tensor> mask_, double tau,
+                                 int64_t reduction, Tensor stats, Tensor weight, Tensor grad_out_) {
+    check_rows(logits_, "logits");
+    c10::OptionalDeviceGuard guard(logits_.device());
+    const Tensor logits = unit_rows(logits_);
+    const int64_t B = logits.size(0), S = logits.size(1), V = logits.size(2);
+    const Tensor tokens = tokens_of(tokens_, logits), mask = mask_of(mask_, logits);
+    stats = f32c(stats, logits, "row_stats");
+    weight = f32c(weight, logits, "weight");
+    TORCH_CHECK(stats.numel() == B * S * 2 && weight.numel() == B,
+                "row_stats and weight must be as the forward returned them");
+    TORCH_CHECK(grad_out_.numel() == (reduction == DOT_REDUCE_NONE ? B * S : B), "grad_out has the wrong size");
+    Tensor grad = at::empty({B, S, V}, logits.options().memory_format(at::MemoryFormat::Contiguous));
+    dot_seqlogp_bwd_args a{};
+    fill_rows(a, logits, tokens, mask, tau, reduction);
+    const Tensor go = upstream(grad_out_, logits, a.grad_out_scalar);
+    a.row_stats = floats(stats);
+    a.weight = floats(weight);
+    a.grad_out = floats(go);
+    a.grad_logits = grad.data_ptr();
+    check_rc(dot_seqlogp_backward(&a, stream_of(logits)), "dot_seqlogp_backward");
+    return grad;
+}
+
+// Sizes of the two sets from [P + Q] ratios and a [P, Q] plan (or pairs).
+template <class A>
+void fill_preference(A& a, const Tensor& ratio, const Tensor& plan, int64_t type, double beta, double smoothing) {
+    TORCH_CHECK(ratio.dim() == 1, "log_ratio must be 1D");
+    const int64_t n = ratio.size(0);
+    const int64_t P = plan.defined() ? plan.size(0) : n / 2, Q = plan.defined() ? plan.size(1) : n / 2;
+    TORCH_CHECK(P + Q == n, "log_ratio must hold the P + Q answers of a [P, Q] plan, or pairs");
+    a.ratio = floats(ratio);
+    a.plan = plan.defined() && plan.numel() ? floats(plan) : nullptr;
+    a.P = to_int(P, "P");
+    a.Q = to_int(Q, "Q");
+    a.loss_type = int(type);
+    a.beta = float(beta);
+    a.smoothing = float(smoothing);
+}
+
+Tensor plan_of(const optional<Tensor>& plan, const Tensor& ratio) {
+    TORCH_CHECK(!plan.has_value() || plan->dim() == 2, "plan must be 2D [P, Q]");
+    return f32c(plan, ratio, "plan");
+}
+
+Tensor preference_forward_op(Tensor ratio_, optional<Tensor> plan_, int64_t type, double beta, double smoothing) {
+    TORCH_CHECK(ratio_.device().is_cuda(), "log_ratio must be a CUDA tensor");
+    c10::OptionalDeviceGuard guard(ratio_.device());
+    const Tensor ratio = f32c(ratio_, ratio_, "log_ratio"), plan = plan_of(plan_, ratio_);
+    dot_preference_fwd_args a{};
+    fill_preference(a, ratio, plan, type, beta, smoothing);
+    Tensor loss = at::empty({a.P}, ratio.options());
+    a.loss = loss.data_ptr<float>();
+    check_rc(dot_preference_forward(&a, stream_of(ratio)), "dot_preference_forward");
+    return loss;
+}
+
+// -> [grad_ratio, grad_plan (empty without want_plan)]
+std::vector<Tensor> preference_backward_op(Tensor ratio_, optional<Tensor> plan_, int64_t type, double beta,
+                                           double smoothing, Tensor grad_loss_, bool want_plan) {
+    TORCH_CHECK(ratio_.device().is_cuda(), "log_ratio must be a CUDA tensor");
+    c10::OptionalDeviceGuard guard(ratio_.device());
+    const Tensor ratio = f32c(ratio_, ratio_, "log_ratio"), plan = plan_of(plan_, ratio_);
+    dot_preference_bwd_args a{};
+    fill_preference(a, ratio, plan, type, beta, smoothing);
+    TORCH_CHECK(grad_loss_.numel() == a.P, "grad_loss must have shape [P]");
+    const Tensor gl = upstream(grad_loss_, ratio, a.grad_loss_scalar);
+    Tensor grad_ratio = at::empty_like(ratio);
+    Tensor grad_plan = want_plan && plan.defined() ? at::empty_like(plan) : at::empty({0}, ratio.options());
+    a.grad_loss = floats(gl);
+    a.grad_ratio = grad_ratio.data_ptr<float>();
+    a.grad_plan = grad_plan.numel() ? grad_plan.data_ptr<float>() : nullptr;
+    a.workspace_bytes = dot_preference_backward_workspace_bytes(a.P, a.Q, plan.defined());
+    Tensor ws;
+    if (a.workspace_bytes) {
+        ws = workspace(a.workspace_bytes, ratio);
+        a.workspace = ws.data_ptr();
+    }
+    check_rc(dot_preference_backward(&a, stream_of(ratio)), "dot_preference_backward");
+    return {grad_ratio, grad_plan};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(dot_amd, m) {
+    m.def("routing_forward(Tensor scores, int k, int scoring, bool normalize, Tensor? bias, Tensor? mask, Tensor? given) -> Tensor[]");
+    m.def("routing_backward(Tensor scores, int k, int scoring, bool normalize, Tensor? mask, Tensor counts, Tensor tokens, Tensor? grad_loss, Tensor? weights, Tensor? experts, Tensor? grad_weights) -> Tensor");
+    m.def("sequence_logp_forward(Tensor logits, Tensor tokens, Tensor? ref, Tensor? mask, float tau, int reduction, bool keep) -> Tensor[]");
+    m.def("sequence_logp_backward(Tensor logits, Tensor tokens, Tensor? mask, float tau, int reduction, Tensor row_stats, Tensor weight, Tensor grad_out) -> Tensor");
+    m.def("preference_forward(Tensor log_ratio, Tensor? plan, int loss_type, float beta, float smoothing) -> Tensor");
+    m.def("preference_backward(Tensor log_ratio, Tensor? plan, int loss_type, float beta, float smoothing, Tensor grad_loss, bool want_plan) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(dot_amd, CUDA, m) {
+    m.impl("routing_forward", routing_forward_op);
+    m.impl("routing_backward", routing_backward_op);
+    m.impl("sequence_logp_forward", sequence_logp_forward_op);
+    m.impl("sequence_logp_backward", sequence_logp_backward_op);
+    m.impl("preference_forward", preference_forward_op);
+    m.impl("preference_backward", preference_backward_op);
+}

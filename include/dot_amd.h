@@ -368,6 +368,158 @@ size_t dot_bidisoftmax_exchange_bytes(void);
 size_t dot_sinkhorn_exchange_bytes(void);
 
 /* ---------------------------------------------------------------------- */
+/* Routing of tokens to experts (no counterpart in the reference)          */
+/* ---------------------------------------------------------------------- */
+/* Element types of the operators below. */
+enum { DOT_F32 = 0, DOT_F16 = 1, DOT_BF16 = 2 };
+
+/* What a score says of an expert's mass q: softmax over the row, the logistic
+ * function of the score, or the score itself (a row of a transport plan). */
+enum { DOT_SCORING_SOFTMAX = 0, DOT_SCORING_SIGMOID = 1, DOT_SCORING_PLAN = 2 };
+
+#define DOT_ROUTING_MAX_EXPERTS 4096
+#define DOT_ROUTING_MAX_K 64
+
+typedef struct {
+    const void* scores;        /* element (b, n, e) at b * stride_b + n * stride_n + e */
+    int dtype;                 /* DOT_F32, DOT_F16 or DOT_BF16 */
+    int64_t stride_b, stride_n; /* in elements */
+    int B, N, E, k;            /* 1 <= E <= DOT_ROUTING_MAX_EXPERTS; with given == NULL: k <= E */
+    int scoring;               /* DOT_SCORING_* */
+    int normalize;             /* weights of a token sum to 1 */
+    const float* bias;         /* [E] added to the scores for the selection only, or NULL */
+    const uint8_t* mask;       /* [B,N]: tokens with 0 are left out, or NULL */
+    const void* given;         /* [B,N,k] experts, int32 (int64 with given_is_int64), or NULL:
+                                  the call selects; entries outside [0, E) are not counted */
+    int given_is_int64;
+    float* weights;            /* [B,N,k] out when the call selects */
+    int32_t* experts;          /* [B,N,k] out when the call selects; -1 in slots without an expert */
+    int32_t* counts;           /* [B,E] out: slots of the unmasked tokens that name e */
+    int32_t* tokens;           /* [B] out: unmasked tokens n_b */
+    float* loss;               /* [B] out: E sum_e counts_e / (k n_b) * sum_n p_ne / n_b, with p = q / sum q;
+                                  0 where n_b = 0 */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_routing_fwd_args;
+
+/* The k experts of the largest keys score + bias of each token, in descending
+ * order, equal keys by the lowest index; an expert is available where its key
+ * is above -inf (and, with DOT_SCORING_PLAN, its score above 0).  Weights are
+ * the masses q of the selected experts.  A masked token gets experts of -1 and
+ * weights of 0. */
+size_t dot_routing_forward_workspace_bytes(int B, int N, int E);
+int dot_routing_forward(const dot_routing_fwd_args* args, dot_stream_t stream);
+
+typedef struct {
+    const void* scores;        /* as in the forward */
+    int dtype;
+    int64_t stride_b, stride_n;
+    int B, N, E, k;
+    int scoring;
+    int normalize;
+    const uint8_t* mask;
+    const int32_t* counts;     /* [B,E] and [B], as the forward wrote them */
+    const int32_t* tokens;
+    const float* grad_loss;    /* [B] (one value with grad_loss_scalar), or NULL */
+    int grad_loss_scalar;
+    const float* weights;      /* [B,N,k] as the forward wrote them, with grad_weights */
+    const int32_t* experts;
+    const float* grad_weights; /* [B,N,k], or NULL */
+    void* grad_scores;         /* [B,N,E] out, contiguous, of type dtype; 0 for masked tokens */
+} dot_routing_bwd_args;
+
+int dot_routing_backward(const dot_routing_bwd_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Log-probabilities of token sequences (no counterpart in the reference)  */
+/* ---------------------------------------------------------------------- */
+enum { DOT_REDUCE_NONE = 0, DOT_REDUCE_SUM = 1, DOT_REDUCE_MEAN = 2 };
+
+typedef struct {
+    const void* logits;        /* element (b, s, v) at b * stride_b + s * stride_s + v */
+    int dtype;
+    int64_t stride_b, stride_s;
+    int B, S, V;
+    const void* tokens;        /* [B,S] int32 (int64 with tokens_are_int64); a position whose token
+                                  is outside [0, V) is left out */
+    int tokens_are_int64;
+    const uint8_t* mask;       /* [B,S]: positions with 0 are left out, or NULL */
+    const void* ref;           /* fp32 (double with ref_is_f64) log-probabilities to subtract: [B,S]
+                                  (ref_per_token) or [B], or NULL */
+    int ref_is_f64, ref_per_token;
+    float tau;                 /* > 0 */
+    int reduction;             /* DOT_REDUCE_* over the positions that are not left out */
+    float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
+    float* row_stats;          /* [B,S,2] out, for the backward: the row's max and
+                                  1 / sum exp((x - max) / tau); not written where left out */
+    float* weight;             /* [B] out, for the backward: 1, or 1 / positions with DOT_REDUCE_MEAN */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_seqlogp_fwd_args;
+
+/* l = x_token / tau - log sum_v exp(x_v / tau) for each position, less the
+ * reference's, summed over each sequence. */
+size_t dot_seqlogp_forward_workspace_bytes(int B, int S, int V, int dtype);
+int dot_seqlogp_forward(const dot_seqlogp_fwd_args* args, dot_stream_t stream);
+
+typedef struct {
+    const void* logits;
+    int dtype;
+    int64_t stride_b, stride_s;
+    int B, S, V;
+    const void* tokens;
+    int tokens_are_int64;
+    const uint8_t* mask;
+    float tau;
+    int reduction;
+    const float* row_stats;
+    const float* weight;
+    const float* grad_out;     /* [B], or [B,S] with DOT_REDUCE_NONE; one value with grad_out_scalar */
+    int grad_out_scalar;
+    void* grad_logits;         /* [B,S,V] out, contiguous, of type dtype; 0 where left out */
+} dot_seqlogp_bwd_args;
+
+int dot_seqlogp_backward(const dot_seqlogp_bwd_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Preference loss over pairs or a transport plan                          */
+/* (no counterpart in the reference)                                       */
+/* ---------------------------------------------------------------------- */
+enum { DOT_PREFER_SIGMOID = 0, DOT_PREFER_HINGE = 1, DOT_PREFER_SQUARE = 2 };
+
+typedef struct {
+    const float* ratio;        /* [P+Q]: log ratios of the P preferred, then of the Q other answers */
+    const float* plan;         /* [P,Q], or NULL: pair i with i (P = Q) */
+    int P, Q;
+    int loss_type;             /* DOT_PREFER_* */
+    float beta;                /* > 0 */
+    float smoothing;           /* in [0, 1), DOT_PREFER_SIGMOID only */
+    float* loss;               /* [P] out: sum_j plan_ij f(ratio_i - ratio_{P+j}), or f of pair i */
+} dot_preference_fwd_args;
+
+/* f(d) = (1 - smoothing) log(1 + exp(-beta d)) + smoothing log(1 + exp(beta d)),
+ * max(0, 1 - beta d), or (d - 1 / (2 beta))^2. */
+int dot_preference_forward(const dot_preference_fwd_args* args, dot_stream_t stream);
+
+typedef struct {
+    const float* ratio;
+    const float* plan;
+    int P, Q;
+    int loss_type;
+    float beta;
+    float smoothing;
+    const float* grad_loss;    /* [P]; one value with grad_loss_scalar */
+    int grad_loss_scalar;
+    float* grad_ratio;         /* [P+Q] out */
+    float* grad_plan;          /* [P,Q] out, or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_preference_bwd_args;
+
+size_t dot_preference_backward_workspace_bytes(int P, int Q, int has_plan);
+int dot_preference_backward(const dot_preference_bwd_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
 /* Diagnostics (no counterpart in the reference)                           */
 /* ---------------------------------------------------------------------- */
 /* Message of the calling thread's most recent failure ("" after success). */
