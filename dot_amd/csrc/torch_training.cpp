@@ -1,12 +1,21 @@
 // PyTorch binding of the routing, sequence log-probability and preference
-// entry points of the C ABI (torch.ops.dot_amd.*), for HIP tensors; the CPU
-// implementations are in cpu_training.cpp.  The Python functions check
-// arguments; the operators check again what a kernel's indexing relies on.
+// entry points of the C ABI (torch.ops.dot_amd.*) for HIP tensors, and their
+// autograd functions for HIP and CPU tensors (the CPU implementations are in
+// cpu_training.cpp).  The Python functions check arguments; the operators
+// check again what a kernel's indexing relies on.
+//
+// The autograd functions are C++: a training step over a small batch is bound
+// by the host's work, and a node that runs without the interpreter takes less
+// of it.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -330,6 +339,154 @@ std::vector<Tensor> preference_backward_op(Tensor ratio_, optional<Tensor> plan_
     return {grad_ratio, grad_plan};
 }
 
+// ---------------------------------------------------------------------------
+// Autograd
+// ---------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Whether a call has to be recorded.
+bool records(const Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
+bool records(const optional<Tensor>& x) { return x.has_value() && records(*x); }
+
+// The gradient of an operator that has no second derivative: a backward
+// through it is an error, not a wrong result.
+Tensor once(const Tensor& grad) {
+    if (!at::GradMode::is_enabled() || !grad.defined()) return grad;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>(
+        "dot_amd operators are differentiable once: no gradient flows through their backward", 1);
+    return (*refuse)({grad})[0];
+}
+
+template <class F>
+auto op_handle(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+std::vector<Tensor> call_routing(const Tensor& scores, int64_t k, int64_t scoring, bool normalize,
+                                 const optional<Tensor>& bias, const optional<Tensor>& mask,
+                                 const optional<Tensor>& given) {
+    static const auto op = op_handle<decltype(routing_forward_op)>("dot_amd::routing_forward");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(scores, k, scoring, normalize, bias, mask, given);
+}
+
+optional<Tensor> maybe(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+struct RoutingFunction : torch::autograd::Function<RoutingFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& scores, int64_t k, int64_t scoring,
+                                 bool normalize, const optional<Tensor>& bias, const optional<Tensor>& mask,
+                                 const optional<Tensor>& given) {
+        std::vector<Tensor> o = call_routing(scores, k, scoring, normalize, bias, mask, given);
+        const bool select = !given.has_value();
+        ctx->save_for_backward({scores, mask.value_or(Tensor()), o[2], o[3], select ? o[0] : Tensor(),
+                                select ? o[1] : Tensor()});
+        ctx->saved_data["k"] = k;
+        ctx->saved_data["scoring"] = scoring;
+        ctx->saved_data["normalize"] = normalize;
+        ctx->mark_non_differentiable(select ? variable_list{o[1], o[2], o[3]} : variable_list{o[0], o[1], o[2], o[3]});
+        ctx->set_materialize_grads(false);
+        return o;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor gw = s[4].defined() ? grads[0] : Tensor(), gl = grads[4];
+        Tensor g;
+        if (gw.defined() || gl.defined()) {
+            static const auto op = op_handle<decltype(routing_backward_op)>("dot_amd::routing_backward");
+            at::AutoDispatchBelowADInplaceOrView below;
+            g = op.call(s[0], ctx->saved_data["k"].toInt(), ctx->saved_data["scoring"].toInt(),
+                        ctx->saved_data["normalize"].toBool(), maybe(s[1]), s[2], s[3], maybe(gl),
+                        gw.defined() ? maybe(s[4]) : c10::nullopt, gw.defined() ? maybe(s[5]) : c10::nullopt,
+                        maybe(gw));
+        }
+        return {once(g), {}, {}, {}, {}, {}, {}};
+    }
+};
+
+std::vector<Tensor> routing_forward_autograd(Tensor scores, int64_t k, int64_t scoring, bool normalize,
+                                             optional<Tensor> bias, optional<Tensor> mask, optional<Tensor> given) {
+    if (!records(scores)) return call_routing(scores, k, scoring, normalize, bias, mask, given);
+    return RoutingFunction::apply(scores, k, scoring, normalize, bias, mask, given);
+}
+
+std::vector<Tensor> call_sequence_logp(const Tensor& logits, const Tensor& tokens, const optional<Tensor>& ref,
+                                       const optional<Tensor>& mask, double tau, int64_t reduction, bool keep) {
+    static const auto op = op_handle<decltype(sequence_logp_forward_op)>("dot_amd::sequence_logp_forward");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(logits, tokens, ref, mask, tau, reduction, keep);
+}
+
+struct SequenceLogpFunction : torch::autograd::Function<SequenceLogpFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens,
+                                 const optional<Tensor>& ref, const optional<Tensor>& mask, double tau,
+                                 int64_t reduction) {
+        std::vector<Tensor> o = call_sequence_logp(logits, tokens, ref, mask, tau, reduction, true);
+        ctx->save_for_backward({logits, tokens, mask.value_or(Tensor()), o[1], o[2]});
+        ctx->saved_data["tau"] = tau;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->mark_non_differentiable({o[1], o[2]});
+        ctx->set_materialize_grads(false);
+        return o;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        Tensor g;
+        if (grads[0].defined()) {
+            static const auto op = op_handle<decltype(sequence_logp_backward_op)>("dot_amd::sequence_logp_backward");
+            at::AutoDispatchBelowADInplaceOrView below;
+            g = op.call(s[0], s[1], maybe(s[2]), ctx->saved_data["tau"].toDouble(),
+                        ctx->saved_data["reduction"].toInt(), s[3], s[4], grads[0]);
+        }
+        return {once(g), {}, {}, {}, {}, {}};
+    }
+};
+
+std::vector<Tensor> sequence_logp_forward_autograd(Tensor logits, Tensor tokens, optional<Tensor> ref,
+                                                   optional<Tensor> mask, double tau, int64_t reduction, bool keep) {
+    if (!records(logits)) return call_sequence_logp(logits, tokens, ref, mask, tau, reduction, keep);
+    return SequenceLogpFunction::apply(logits, tokens, ref, mask, tau, reduction);
+}
+
+Tensor call_preference(const Tensor& ratio, const optional<Tensor>& plan, int64_t type, double beta,
+                       double smoothing) {
+    static const auto op = op_handle<decltype(preference_forward_op)>("dot_amd::preference_forward");
+    at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(ratio, plan, type, beta, smoothing);
+}
+
+struct PreferenceFunction : torch::autograd::Function<PreferenceFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& ratio, const optional<Tensor>& plan, int64_t type,
+                          double beta, double smoothing) {
+        ctx->save_for_backward({ratio, plan.value_or(Tensor())});
+        ctx->saved_data["type"] = type;
+        ctx->saved_data["beta"] = beta;
+        ctx->saved_data["smoothing"] = smoothing;
+        ctx->set_materialize_grads(false);
+        return call_preference(ratio, plan, type, beta, smoothing);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list s = ctx->get_saved_variables();
+        Tensor gr, gp;
+        if (grads[0].defined()) {
+            const bool want_plan = s[1].defined() && ctx->needs_input_grad(1);
+            static const auto op = op_handle<decltype(preference_backward_op)>("dot_amd::preference_backward");
+            at::AutoDispatchBelowADInplaceOrView below;
+            const std::vector<Tensor> g =
+                op.call(s[0], maybe(s[1]), ctx->saved_data["type"].toInt(), ctx->saved_data["beta"].toDouble(),
+                        ctx->saved_data["smoothing"].toDouble(), grads[0], want_plan);
+            gr = g[0].to(s[0].scalar_type());
+            if (want_plan) gp = g[1].to(s[1].scalar_type());
+        }
+        return {once(gr), once(gp), {}, {}, {}};
+    }
+};
+
+Tensor preference_forward_autograd(Tensor ratio, optional<Tensor> plan, int64_t type, double beta, double smoothing) {
+    if (!records(ratio) && !records(plan)) return call_preference(ratio, plan, type, beta, smoothing);
+    return PreferenceFunction::apply(ratio, plan, type, beta, smoothing);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(dot_amd, m) {
@@ -348,4 +505,10 @@ TORCH_LIBRARY_IMPL(dot_amd, CUDA, m) {
     m.impl("sequence_logp_backward", sequence_logp_backward_op);
     m.impl("preference_forward", preference_forward_op);
     m.impl("preference_backward", preference_backward_op);
+}
+
+TORCH_LIBRARY_IMPL(dot_amd, Autograd, m) {
+    m.impl("routing_forward", routing_forward_autograd);
+    m.impl("sequence_logp_forward", sequence_logp_forward_autograd);
+    m.impl("preference_forward", preference_forward_autograd);
 }

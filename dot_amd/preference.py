@@ -18,34 +18,12 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _ops
 
 _REDUCTION = {"none": 0, "sum": 1, "mean": 2}
 _LOSS = {"sigmoid": 0, "hinge": 1, "square": 2}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
-
-
-class _SequenceLogpFunction(torch.autograd.Function):
-    """Saves the logits and two statistics per position; the backward reads the logits again."""
-
-    @staticmethod
-    def forward(ctx, logits, tokens, ref, mask, tau, reduction):
-        keep = ctx.needs_input_grad[0]
-        out, stats, weight = _ops.fused.sequence_logp_forward(logits, tokens, ref, mask, tau, reduction, keep)
-        if keep:
-            ctx.save_for_backward(logits, tokens, mask, stats, weight)
-            ctx.args = (tau, reduction)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, tokens, mask, stats, weight = ctx.saved_tensors
-        tau, reduction = ctx.args
-        g = _ops.fused.sequence_logp_backward(logits, tokens, mask, tau, reduction, stats, weight, grad)
-        return g, None, None, None, None, None
 
 
 def sequence_logp(
@@ -108,25 +86,8 @@ def sequence_logp(
         logits, tokens = logits.unsqueeze(0), tokens.unsqueeze(0)
         mask = None if mask is None else mask.unsqueeze(0)
         ref_logp = None if ref_logp is None else ref_logp.unsqueeze(0)
-    out = _SequenceLogpFunction.apply(logits, tokens, ref_logp, mask, tau, _REDUCTION[reduction])
+    out = _ops.fused.sequence_logp_forward(logits, tokens, ref_logp, mask, tau, _REDUCTION[reduction], False)[0]
     return out if batched else out.squeeze(0)
-
-
-class _PreferenceFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ratio, plan, loss_type, beta, smoothing):
-        ctx.save_for_backward(ratio, plan)
-        ctx.args = (loss_type, beta, smoothing)
-        return _ops.fused.preference_forward(ratio, plan, loss_type, beta, smoothing)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        ratio, plan = ctx.saved_tensors
-        loss_type, beta, smoothing = ctx.args
-        want_plan = ctx.needs_input_grad[1]
-        g_ratio, g_plan = _ops.fused.preference_backward(ratio, plan, loss_type, beta, smoothing, grad, want_plan)
-        return (g_ratio.to(ratio.dtype), g_plan.to(plan.dtype) if want_plan else None, None, None, None)
 
 
 def preference_loss(
@@ -175,7 +136,7 @@ def preference_loss(
         raise ValueError(f"label_smoothing must be in [0, 1), got {label_smoothing}")
     if label_smoothing and loss_type != "sigmoid":
         raise ValueError("label_smoothing needs loss_type='sigmoid'")
-    return _PreferenceFunction.apply(log_ratio, plan, _LOSS[loss_type], beta, label_smoothing)
+    return _ops.fused.preference_forward(log_ratio, plan, _LOSS[loss_type], beta, label_smoothing)
 
 
 class SequenceLogp(nn.Module):

@@ -23,7 +23,6 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _ops
 
@@ -57,35 +56,6 @@ class BalanceResult:
 
     loss: torch.Tensor
     counts: torch.Tensor
-
-
-class _RoutingFunction(torch.autograd.Function):
-    """Selection (or given experts), counts and balance loss; the backward reads the scores again."""
-
-    @staticmethod
-    def forward(ctx, scores, k, scoring, normalize, bias, mask, given):
-        weights, experts, counts, tokens, loss = _ops.fused.routing_forward(scores, k, scoring, normalize, bias, mask,
-                                                                            given)
-        if given is None:
-            ctx.save_for_backward(scores, mask, counts, tokens, weights, experts)
-        else:
-            ctx.save_for_backward(scores, mask, counts, tokens)
-        ctx.args = (k, scoring, normalize)
-        ctx.mark_non_differentiable(experts, counts)
-        ctx.set_materialize_grads(False)
-        return weights, experts, counts, loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_weights, _experts, _counts, grad_loss):
-        if grad_weights is None and grad_loss is None:
-            return (None,) * 7
-        scores, mask, counts, tokens, *selected = ctx.saved_tensors
-        weights, experts = selected if selected and grad_weights is not None else (None, None)
-        k, scoring, normalize = ctx.args
-        grad = _ops.fused.routing_backward(scores, k, scoring, normalize, mask, counts, tokens, grad_loss, weights,
-                                           experts, grad_weights if selected else None)
-        return grad, None, None, None, None, None, None
 
 
 def _check_scores(scores, scoring, mask):
@@ -140,10 +110,13 @@ def topk_routing(
             raise ValueError(f"bias must be floating point of shape ({scores.size(-1)},), got {tuple(bias.shape)}")
         bias = bias.detach()
     if scores.dim() == 3:
-        return RoutingResult(*_RoutingFunction.apply(scores, k, _SCORING[scoring], normalize, bias, mask, None))
-    out = _RoutingFunction.apply(scores.unsqueeze(0), k, _SCORING[scoring], normalize, bias,
-                                 None if mask is None else mask.unsqueeze(0), None)
-    return RoutingResult(*(x.squeeze(0) for x in out))
+        weights, experts, counts, _, loss = _ops.fused.routing_forward(scores, k, _SCORING[scoring], normalize, bias,
+                                                                       mask, None)
+        return RoutingResult(weights, experts, counts, loss)
+    out = _ops.fused.routing_forward(scores.unsqueeze(0), k, _SCORING[scoring], normalize, bias,
+                                     None if mask is None else mask.unsqueeze(0), None)
+    weights, experts, counts, _, loss = (x.squeeze(0) for x in out)
+    return RoutingResult(weights, experts, counts, loss)
 
 
 def balance_loss(
@@ -177,7 +150,8 @@ def balance_loss(
     if not batched:
         scores, experts = scores.unsqueeze(0), experts.unsqueeze(0)
         mask = None if mask is None else mask.unsqueeze(0)
-    _, _, counts, loss = _RoutingFunction.apply(scores, experts.size(-1), _SCORING[scoring], False, None, mask, experts)
+    _, _, counts, _, loss = _ops.fused.routing_forward(scores, experts.size(-1), _SCORING[scoring], False, None, mask,
+                                                       experts)
     return BalanceResult(loss, counts) if batched else BalanceResult(loss.squeeze(0), counts.squeeze(0))
 
 
