@@ -2,7 +2,9 @@
 // the gradient of the logits.
 //
 // The forward reads each row once with a running maximum m and sum
-// s = sum_v 2^((x_v - m) k), k = log2(e) / tau; a row may be split over several
+// s = sum_v 2^((x_v - m) k), k = log2(e) / tau.  Terms are added pairwise within
+// a pack, and those sums in 64 bits: next to a likely token's 1, terms
+// of 1e-7 each would be lost one by one in 32.  A row may be split over several
 // workgroups, whose (m, s) the second kernel joins.  That kernel also forms
 // the position's value and the sequence's sum in 64 bits: the log ratio of two
 // models is a small difference of large sums.  x - m is formed before the
@@ -28,9 +30,15 @@ struct Rows {
     const void* tokens;
     int tokens64;
     const uint8_t* mask;
-    float k;     // log2(e) / tau
+    // log2(e) / tau = k + klo, both > 0.  One float is off by up to 6e-8 of
+    // itself, which shifts every position's value the same way: 1e-7 each on
+    // typical rows, 1e-4 over a thousand positions.
+    float k, klo;
     int splits;  // workgroups per row
 };
+
+// d log2(e) / tau of a difference d <= 0 (-inf stays -inf: klo is not 0).
+__device__ __forceinline__ float scaled(const Rows& r, float d) { return fmaf(d, r.k, d * r.klo); }
 
 // The token of a position, or -1 where it is left out.
 __device__ __forceinline__ int token_of(const Rows& r, int64_t at) {
@@ -66,27 +74,52 @@ __device__ __forceinline__ Span span_of(const T* row, int V, int part, int parts
     return s;
 }
 
+// Sum of N values, pairwise.
+template <int N>
+__device__ __forceinline__ float pairwise(const float* x) {
+    if constexpr (N == 1) return x[0];
+    else return pairwise<N / 2>(x) + pairwise<N - N / 2>(x + N / 2);
+}
+
 // Largest value and sum of 2^((x - m) k) so far; m = -inf: nothing but -inf.
 struct MaxSum {
     float m = -__builtin_inff();
-    float s = 0.0f;
+    double s = 0.0;
     __device__ __forceinline__ float base() const { return m == -__builtin_inff() ? 0.0f : m; }
-    __device__ __forceinline__ void raise(float to, float k) {
+    __device__ __forceinline__ void raise(float to, const Rows& r) {
         const float old = m;
         m = fmaxf(m, to);
-        s *= __builtin_amdgcn_exp2f((old - base()) * k);
+        s *= double(__builtin_amdgcn_exp2f(scaled(r, old - base())));
     }
-    __device__ __forceinline__ void add(float x, float k) { s += __builtin_amdgcn_exp2f((x - base()) * k); }
-    __device__ __forceinline__ void join(float om, float os, float k) {
-        raise(om, k);
-        s += os * __builtin_amdgcn_exp2f((om - base()) * k);
+    // N values at once, in 32 bits over M of them
+    template <int M, int N>
+    __device__ __forceinline__ void add(const float (&x)[N], const Rows& r) {
+        float most = x[0], e[N];
+#pragma unroll
+        for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
+        raise(most, r);
+        const float c = base();
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f(scaled(r, x[i] - c));
+#pragma unroll
+        for (int i = 0; i < N; i += M) s += double(pairwise<M>(e + i));
+    }
+    __device__ __forceinline__ void join(float om, double os, const Rows& r) {
+        raise(om, r);
+        s += os * double(__builtin_amdgcn_exp2f(scaled(r, om - base())));
     }
 };
 
-// Partial statistics of every row: parts[row * splits + split] = (m, s).
+struct Part {
+    double s;
+    float m;
+};
+
+// Partial statistics of every row: one for each split.
 template <class T>
-__global__ __launch_bounds__(kBlock) void row_stats(Rows r, float2* parts) {
-    __shared__ float sm[kWavesPerBlock], ss[kWavesPerBlock];
+__global__ __launch_bounds__(kBlock) void row_stats(Rows r, Part* parts) {
+    __shared__ float sm[kWavesPerBlock];
+    __shared__ double ss[kWavesPerBlock];
     const int64_t at = blockIdx.x / unsigned(r.splits);
     const int part = int(blockIdx.x % unsigned(r.splits));
     if (token_of(r, at) < 0) return;
@@ -98,41 +131,33 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, float2* parts) {
     int p = sp.p0 + int(threadIdx.x);
     for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
         Pack<T> x[kUnroll];
+        float f[kUnroll * PN];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) x[u] = load_pack(body + int64_t(p + u * kBlock) * PN);
-        float most = to_float(x[0].v[0]);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < PN; ++i) most = fmaxf(most, to_float(x[u].v[i]));
-        a.raise(most, r.k);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-            for (int i = 0; i < PN; ++i) a.add(to_float(x[u].v[i]), r.k);
+        for (int i = 0; i < kUnroll * PN; ++i) f[i] = to_float(x[i / PN].v[i % PN]);
+        a.add<PN>(f, r);
     }
     for (; p < sp.p1; p += kBlock) {
         const Pack<T> x = load_pack(body + int64_t(p) * PN);
-        float most = to_float(x.v[0]);
+        float f[PN];
 #pragma unroll
-        for (int i = 1; i < PN; ++i) most = fmaxf(most, to_float(x.v[i]));
-        a.raise(most, r.k);
-#pragma unroll
-        for (int i = 0; i < PN; ++i) a.add(to_float(x.v[i]), r.k);
+        for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
+        a.add<PN>(f, r);
     }
     if (part == 0 && int(threadIdx.x) < sp.head) {
-        const float x = to_float(row[threadIdx.x]);
-        a.raise(x, r.k);
-        a.add(x, r.k);
+        const float f[1] = {to_float(row[threadIdx.x])};
+        a.add<1>(f, r);
     }
     if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) {
-        const float x = to_float(row[sp.tail + threadIdx.x]);
-        a.raise(x, r.k);
-        a.add(x, r.k);
+        const float f[1] = {to_float(row[sp.tail + threadIdx.x])};
+        a.add<1>(f, r);
     }
     const float m = wave_max(a.m);
-    a.raise(m, r.k);
-    const float s = wave_sum(a.s);
+    a.raise(m, r);
+    double s = a.s;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
     if (threadIdx.x % kWave == 0) {
         sm[threadIdx.x / kWave] = m;
         ss[threadIdx.x / kWave] = s;
@@ -140,8 +165,8 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, float2* parts) {
     __syncthreads();
     if (threadIdx.x == 0) {
         MaxSum t;
-        for (int w = 0; w < kWavesPerBlock; ++w) t.join(sm[w], ss[w], r.k);
-        parts[blockIdx.x] = make_float2(t.m, t.s);
+        for (int w = 0; w < kWavesPerBlock; ++w) t.join(sm[w], ss[w], r);
+        parts[blockIdx.x] = Part{t.s, t.m};
     }
 }
 
@@ -161,7 +186,7 @@ __device__ __forceinline__ double float_at(const void* p, int is64, int64_t i) {
 // One workgroup per sequence: joins the parts of its rows, forms the values of
 // its positions and their sum.
 template <class T>
-__global__ __launch_bounds__(kJoinBlock) void join(Rows r, const float2* parts, JoinArgs j) {
+__global__ __launch_bounds__(kJoinBlock) void join(Rows r, const Part* parts, JoinArgs j) {
     __shared__ double wsum[kJoinBlock / kWave];
     __shared__ int wcount[kJoinBlock / kWave];
     const int b = batch_of_block();
@@ -175,12 +200,12 @@ __global__ __launch_bounds__(kJoinBlock) void join(Rows r, const float2* parts, 
         if (tok >= 0) {
             MaxSum t;
             for (int i = 0; i < r.splits; ++i) {
-                const float2 p = parts[at * r.splits + i];
-                t.join(p.x, p.y, r.k);
+                const Part p = parts[at * r.splits + i];
+                t.join(p.m, p.s, r);
             }
             const float x = to_float(row_of<T>(r, at)[tok]);
-            if (j.stats) j.stats[at] = make_float2(t.base(), 1.0f / t.s);
-            v = (double(x) - double(t.base())) * (double(r.k) * 0.693147180559945309417) - log(double(t.s));
+            if (j.stats) j.stats[at] = make_float2(t.base(), float(1.0 / t.s));
+            v = (double(x) - double(t.base())) * ((double(r.k) + double(r.klo)) * 0.693147180559945309417) - log(t.s);
             if (j.ref && j.ref_per_token) v -= float_at(j.ref, j.ref64, at);
             sum += v;
             ++count;
@@ -248,7 +273,7 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     const float c = up * g.weight[b] * g.inv_tau;
     const float scale = -c * st.y;
     auto value = [&](float x, int v) {
-        const float y = __builtin_amdgcn_exp2f((x - st.x) * r.k) * scale;
+        const float y = __builtin_amdgcn_exp2f(scaled(r, x - st.x)) * scale;
         return v == tok ? c + y : y;
     };
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;

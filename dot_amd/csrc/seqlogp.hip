@@ -26,6 +26,8 @@ int check_shape(int dtype, int B, int S, int V, float tau, int reduction) {
     if (V > (1 << 30) || int64_t(B) * S > (1 << 23))
         return fail(DOT_ERR_UNSUPPORTED, "V must be at most 2^30 and B * S at most 2^23");
     if (!(tau > 0.0f) || !std::isfinite(tau)) return fail(DOT_ERR_INVALID_ARG, "tau must be > 0");
+    // log2(e) / tau and its rest are normal floats
+    if (tau < 1e-20f || tau > 1e20f) return fail(DOT_ERR_UNSUPPORTED, "tau must be in [1e-20, 1e20]");
     if (reduction != DOT_REDUCE_NONE && reduction != DOT_REDUCE_SUM && reduction != DOT_REDUCE_MEAN)
         return fail(DOT_ERR_INVALID_ARG, "reduction must be a DOT_REDUCE_* value");
     return DOT_OK;
@@ -43,7 +45,10 @@ seqlogp::Rows rows_of(const A* a) {
     r.tokens = a->tokens;
     r.tokens64 = a->tokens_are_int64;
     r.mask = a->mask;
-    r.k = float(1.4426950408889634 / double(a->tau));
+    const double k = 1.4426950408889634074 / double(a->tau);
+    r.k = float(k);
+    if (double(r.k) >= k) r.k = std::nextafter(r.k, 0.0f);
+    r.klo = float(k - double(r.k));
     r.splits = splits_of(a->B, a->S, a->V, a->dtype);
     return r;
 }
@@ -55,7 +60,7 @@ using namespace dot_amd;
 
 extern "C" size_t dot_seqlogp_forward_workspace_bytes(int B, int S, int V, int dtype) {
     if (B < 0 || S < 0 || V < 1 || !known_dtype(dtype)) return 0;
-    return size_t(B) * S * splits_of(B, S, V, dtype) * sizeof(float2);
+    return size_t(B) * S * splits_of(B, S, V, dtype) * sizeof(seqlogp::Part);
 }
 
 extern "C" int dot_seqlogp_forward(const dot_seqlogp_fwd_args* a, dot_stream_t stream_) {
@@ -73,7 +78,7 @@ extern "C" int dot_seqlogp_forward(const dot_seqlogp_fwd_args* a, dot_stream_t s
                      a->workspace_bytes < dot_seqlogp_forward_workspace_bytes(a->B, a->S, a->V, a->dtype)))
         return fail(DOT_ERR_WORKSPACE, "workspace smaller than dot_seqlogp_forward_workspace_bytes()");
     const seqlogp::Rows r = rows_of(a);
-    float2* parts = static_cast<float2*>(a->workspace);
+    auto* parts = static_cast<seqlogp::Part*>(a->workspace);
     seqlogp::JoinArgs j{};
     j.ref = a->ref;
     j.ref64 = a->ref_is_f64;
