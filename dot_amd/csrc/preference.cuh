@@ -20,27 +20,28 @@ namespace preference {
 constexpr int kVec = 4;                  // columns of a thread
 constexpr int kCols = kBlock * kVec;     // columns of a workgroup's tile
 constexpr int kMaxStrip = 32;            // rows of a strip at most
-constexpr int kFoldCols = 64;            // columns (or rows) of a fold workgroup
+constexpr int kFoldBlock = 1024;         // threads of a fold workgroup,
+constexpr int kFoldCols = 64;            // of as many columns (or rows)
 
 struct Loss {
     int type;
     float beta, smoothing;
 };
 
-// log(1 + e) for e in [0, 1]: 2 atanh(z) with z = e / (2 + e) <= 1/3, by its
-// series to z^15 (the rest is below 2e-9 of the value); relative error of a
-// few ulp down to the smallest e, where 1 + e would round it away.
+// log(1 + e) for e in [0, 1]: 2 atanh(z) with z = e / (2 + e) <= 1/3, as
+// 2 z (1 + w p(w)), w = z^2.  p has the cubic's coefficients that fit
+// (atanh(z) / z - 1) / w on [0, 1/9] best in the maximum norm of the result
+// (iterated least squares): 5e-9 relative, so a few ulp down to the smallest e,
+// where 1 + e would round it away.
 __device__ __forceinline__ float log1p_unit(float e) {
     const float z = e * __builtin_amdgcn_rcpf(2.0f + e);
     const float w = z * z;
-    float s = 1.0f / 15.0f;
-    s = fmaf(s, w, 1.0f / 13.0f);
-    s = fmaf(s, w, 1.0f / 11.0f);
-    s = fmaf(s, w, 1.0f / 9.0f);
-    s = fmaf(s, w, 1.0f / 7.0f);
-    s = fmaf(s, w, 1.0f / 5.0f);
-    s = fmaf(s, w, 1.0f / 3.0f);
-    return 2.0f * fmaf(z * w, s, z);
+    float s = 0.1401222944f;
+    s = fmaf(s, w, 0.1399957091f);
+    s = fmaf(s, w, 0.2001084983f);
+    s = fmaf(s, w, 0.3333320618f);
+    const float z2 = z + z;
+    return fmaf(z2 * w, s, z2);
 }
 
 // f(gap) and, with SLOPE, df / dgap.
@@ -48,8 +49,7 @@ template <bool SLOPE>
 __device__ __forceinline__ float loss_of(const Loss& l, float gap, float& slope) {
     if (l.type == DOT_PREFER_SIGMOID) {
         const float d = l.beta * gap;
-        const float a = -fabsf(d);
-        const float e = a < -88.0f ? 0.0f : exp_compensated(a);
+        const float e = fast_exp(-fabsf(d));
         if (SLOPE) {
             const float u = __builtin_amdgcn_rcpf(1.0f + e);
             const float up = d < 0.0f ? e * u : u;    // 1 / (1 + exp(-d))
@@ -217,20 +217,23 @@ __global__ __launch_bounds__(kBlock) void plan_backward(PlanBwd a) {
 
 // grad_ratio from the partials: workgroups before `row_blocks` add up rows'
 // column tiles, the others columns' strips (with the other sign).
-__global__ __launch_bounds__(kBlock) void plan_fold(PlanBwd a, int row_blocks, float* grad_ratio) {
-    __shared__ float sm[kBlock / kFoldCols][kFoldCols];
+__global__ __launch_bounds__(kFoldBlock) void plan_fold(PlanBwd a, int row_blocks, float* grad_ratio) {
+    constexpr int kSlices = kFoldBlock / kFoldCols;
+    __shared__ float sm[kSlices][kFoldCols];
     const bool rows = int(blockIdx.x) < row_blocks;
     const int lane = threadIdx.x % kFoldCols, slice = threadIdx.x / kFoldCols;
     const int at = (rows ? int(blockIdx.x) : int(blockIdx.x) - row_blocks) * kFoldCols + lane;
     const int len = rows ? a.P : a.Q, parts = rows ? a.ncols : a.nstrips;
     const float* src = rows ? a.rowpart : a.colpart;
     float s = 0.0f;
-    if (at < len)
-        for (int p = slice; p < parts; p += kBlock / kFoldCols) s += src[int64_t(p) * len + at];
+    if (at < len) {
+#pragma unroll 8
+        for (int p = slice; p < parts; p += kSlices) s += src[int64_t(p) * len + at];
+    }
     sm[slice][lane] = s;
     __syncthreads();
     if (slice == 0 && at < len) {
-        for (int t = 1; t < kBlock / kFoldCols; ++t) s += sm[t][lane];
+        for (int t = 1; t < kSlices; ++t) s += sm[t][lane];
         if (rows) grad_ratio[at] = s;
         else grad_ratio[a.P + at] = -s;
     }

