@@ -33,35 +33,58 @@ struct Shape {
     }
 };
 
-// f(Shape) of the smallest group that holds E <= DOT_ROUTING_MAX_EXPERTS elements.
-template <bool VEC, class F>
+// f(Shape) of a group that holds E <= DOT_ROUTING_MAX_EXPERTS elements.  A round
+// of the selection costs a wave about 8 + 1.5 EL + log2(G) instructions for its
+// 64 / G rows, so the forward (PAIRS) takes two vectors per lane from 128 experts
+// on; the backward, bound by its loads, is faster with twice the lanes.
+template <bool VEC, bool PAIRS, class F>
 void dispatch_shape(int E, F&& f) {
     if (E <= 8) f(Shape<1, 1, VEC>{});
     else if (E <= 16) f(Shape<2, 1, VEC>{});
     else if (E <= 32) f(Shape<4, 1, VEC>{});
     else if (E <= 64) f(Shape<8, 1, VEC>{});
     else if (E <= 128) f(Shape<16, 1, VEC>{});
-    else if (E <= 256) f(Shape<32, 1, VEC>{});
-    else if (E <= 512) f(Shape<64, 1, VEC>{});
+    else if (E <= 256) f(Shape<PAIRS ? 16 : 32, PAIRS ? 2 : 1, VEC>{});
+    else if (E <= 512) f(Shape<PAIRS ? 32 : 64, PAIRS ? 2 : 1, VEC>{});
     else if (E <= 1024) f(Shape<64, 2, VEC>{});
     else if (E <= 2048) f(Shape<64, 4, VEC>{});
     else f(Shape<64, 8, VEC>{});
 }
 
-// Rows that a workgroup visits at once.
-inline int rows_per_pass(int E) {
-    int g = 1;
-    while (g < kWave && g * kV < E) g *= 2;
-    return kWavesPerBlock * (kWave / g);
+// Threads of a forward workgroup.  Few partial rows make `finish` short, so
+// workgroups are large where a lane's registers allow it (up to two vectors).
+constexpr int fwd_block(int R) { return R <= 2 ? 512 : 256; }
+// Waves per SIMD that the registers have to leave room for: two workgroups per CU.
+constexpr int fwd_waves(int R) { return R <= 2 ? 4 : 1; }
+// Rows of column sums in LDS: one per wave, or, for the longest rows, one that
+// the waves add to in turn.
+constexpr int fwd_col_rows(int R) { return R <= 2 ? fwd_block(R) / kWave : 1; }
+
+// Workgroups per batch element: `total` over the whole grid, none without a
+// full pass of rows.
+inline int chunks_of(int B, int N, int rows_per_pass, int total) {
+    const int most = (N + rows_per_pass - 1) / rows_per_pass;
+    const int want = (total + B - 1) / (B > 0 ? B : 1);
+    return most < want ? (most > 0 ? most : 1) : want;
 }
 
-// Workgroups per batch element: four per CU over the whole grid, none without
-// a full pass of rows.
-inline int chunks_of(int B, int N, int E) {
-    const int rpp = rows_per_pass(E);
-    const int most = (N + rpp - 1) / rpp;
-    const int want = (1024 + B - 1) / (B > 0 ? B : 1);
-    return most < want ? (most > 0 ? most : 1) : want;
+// x of a lane combined with that of the lane in the other row of its pair of
+// rows of 16 (or in the other half of the wave): the swap instructions exchange
+// the odd rows of one operand with the even rows of the other, so with x in
+// both, one result holds the even row's value and the other the odd row's in
+// every lane.
+template <int D, class X, class Op>
+__device__ __forceinline__ X swapped(X x, Op op) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    unsigned even, odd;
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        even = r[0], odd = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        even = r[0], odd = r[1];
+    }
+    return op(__builtin_bit_cast(X, even), __builtin_bit_cast(X, odd));
 }
 
 // All-reduce over the groups of G lanes of a wave; every lane is active.
@@ -73,14 +96,44 @@ __device__ __forceinline__ X group_reduce(X x, Op op) {
     if constexpr (G >= 4) x = op(x, as_x(dpp_move<kDppQuadXor2>(as_f(x))));
     if constexpr (G >= 8) x = op(x, as_x(dpp_move<kDppRowHalfMirror>(as_f(x))));
     if constexpr (G >= 16) x = op(x, as_x(dpp_move<kDppRowMirror>(as_f(x))));
-    if constexpr (G >= 32) x = op(x, as_x(swizzle_xor16(as_f(x))));
-    if constexpr (G >= 64) x = op(as_x(read_lane(as_f(x), 0)), as_x(read_lane(as_f(x), 32)));
+    if constexpr (G >= 32) x = swapped<16>(x, op);
+    if constexpr (G >= 64) x = swapped<32>(x, op);
     return x;
 }
 
+// Floats as integers of the same order, and back (-0 counts as 0).  Integer
+// maxima fuse with the lane exchanges, those of floats do not.
+constexpr int kTaken = INT32_MIN;  // below every float
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __builtin_bit_cast(int, x + 0.0f);
+    return i ^ ((i >> 31) & INT32_MAX);
+}
+__device__ __forceinline__ float unordered(int i) {
+    return __builtin_bit_cast(float, i ^ ((i >> 31) & INT32_MAX));
+}
+
+struct OpMaxInt {
+    __device__ __forceinline__ int operator()(int a, int b) const { return a > b ? a : b; }
+};
+struct OpMaxUint {
+    __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; }
+};
 struct OpMinInt {
     __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
 };
+
+// All-reduce by sums over the lanes with the same place in their groups of G.
+template <int G>
+__device__ __forceinline__ float across_groups(float x) {
+    constexpr int kRowRor = 0x120;  // rotation inside a row of 16 lanes
+    if constexpr (G <= 8) x += dpp_move<kRowRor + 8>(x);
+    if constexpr (G <= 4) x += dpp_move<kRowRor + 4>(x);
+    if constexpr (G <= 2) x += dpp_move<kRowRor + 2>(x);
+    if constexpr (G <= 1) x += dpp_move<kRowRor + 1>(x);
+    if constexpr (G <= 16) x = swapped<16>(x, OpSum{});
+    if constexpr (G <= 32) x = swapped<32>(x, OpSum{});
+    return x;
+}
 
 // Orders this wave's LDS writes before its later LDS reads.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -90,34 +143,42 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 constexpr float kNegInf = -__builtin_inff();
 
-// A row in registers; elements beyond E, and rows that are not live, are -inf.
+// A row as it lies in memory, in registers.
 template <class T, class S>
-__device__ __forceinline__ void load_row(const T* row, int gl, int E, bool live, float (&x)[S::EL]) {
-#pragma unroll
-    for (int r = 0; r < S::R; ++r) {
+struct RawRow {
+    static constexpr int PN = Pack<T>::N, PACKS = S::EL / PN;
+    union {
+        Pack<T> pack[PACKS];
+        T one[S::EL];
+    };
+    bool live;
+
+    __device__ __forceinline__ void load(const T* row, int gl, int E, bool live_) {
+        live = live_;
+        if (!live) return;
         if constexpr (S::VEC) {
-            const int c = (r * S::G + gl) * kV;
-            if (live && c < E) {
-                constexpr int PN = Pack<T>::N;
 #pragma unroll
-                for (int h = 0; h < kV / PN; ++h) {
-                    const Pack<T> p = load_pack(row + c + h * PN);
+            for (int r = 0; r < S::R; ++r) {
+                const int c = (r * S::G + gl) * kV;
+                if (c < E) {
 #pragma unroll
-                    for (int i = 0; i < PN; ++i) x[r * kV + h * PN + i] = to_float(p.v[i]);
+                    for (int h = 0; h < kV / PN; ++h) pack[r * (kV / PN) + h] = load_pack(row + c + h * PN);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kV; ++i) x[r * kV + i] = kNegInf;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                const int c = S::expert(gl, r * kV + i);
-                x[r * kV + i] = (live && c < E) ? to_float(row[c]) : kNegInf;
+            for (int j = 0; j < S::EL; ++j) {
+                const int c = S::expert(gl, j);
+                if (c < E) one[j] = row[c];
             }
         }
     }
-}
+    // As floats; elements beyond E, and rows that are not live, are -inf.
+    __device__ __forceinline__ void get(int gl, int E, float (&x)[S::EL]) const {
+#pragma unroll
+        for (int j = 0; j < S::EL; ++j) x[j] = live && S::expert(gl, j) < E ? to_float(one[j]) : kNegInf;
+    }
+};
 
 template <class T, class S>
 __device__ __forceinline__ void store_row(T* row, int gl, int E, const float (&x)[S::EL]) {
@@ -145,22 +206,22 @@ __device__ __forceinline__ void store_row(T* row, int gl, int E, const float (&x
     }
 }
 
-// exp(-|x|) and 1 / (1 + exp(-|x|)), from which the logistic function and its
-// slope follow without cancellation; NaN stays NaN.
+// t = exp(-|x|) and u = 1 / (1 + t), from which the logistic function and its
+// slope t u^2 follow without cancellation; NaN stays NaN.
 __device__ __forceinline__ void logistic_parts(float x, float& t, float& u) {
-    const float d = -fabsf(x);
-    t = d < -88.0f ? 0.0f : exp_compensated(d);
+    t = fast_exp(-fabsf(x));
     u = __builtin_amdgcn_rcpf(1.0f + t);
+}
+
+__device__ __forceinline__ float logistic(float x) {
+    float t, u;
+    logistic_parts(x, t, u);
+    return x < 0.0f ? t * u : u;
 }
 
 // The mass of one score where it needs no row statistics.
 __device__ __forceinline__ float mass_of(float x, int scoring) {
-    if (scoring == DOT_SCORING_SIGMOID) {
-        float t, u;
-        logistic_parts(x, t, u);
-        return x < 0.0f ? t * u : u;
-    }
-    return x == kNegInf ? 0.0f : x;
+    return scoring == DOT_SCORING_SIGMOID ? logistic(x) : x == kNegInf ? 0.0f : x;
 }
 
 // Masses q of a row (softmax: exp(x - top), not yet divided), and 1 / sum q
@@ -174,13 +235,16 @@ __device__ __forceinline__ void row_masses(const float (&x)[S::EL], int scoring,
         float m = kNegInf;
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) m = fmaxf(m, x[j]);
-        m = group_reduce<S::G>(m, OpMax{});
+        m = unordered(group_reduce<S::G>(ordered(m), OpMaxInt{}));
         top = m == kNegInf ? 0.0f : m;
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) q[j] = fast_exp(x[j] - top);
+    } else if (scoring == DOT_SCORING_SIGMOID) {
+#pragma unroll
+        for (int j = 0; j < S::EL; ++j) q[j] = logistic(x[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) q[j] = mass_of(x[j], scoring);
+        for (int j = 0; j < S::EL; ++j) q[j] = x[j] == kNegInf ? 0.0f : x[j];
     }
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) sum += q[j];
@@ -200,46 +264,135 @@ struct FwdArgs {
     float* weights;
     int32_t* experts;
     int nchunks, chunk_rows;
+    // one row of partials per workgroup: column sums, counts, tokens
     float* psum;       // [B, nchunks, E]
     int32_t* pcount;   // [B, nchunks, E]
     int32_t* ptokens;  // [B, nchunks]
+    uint32_t* done;    // [B] column blocks that `finish` is through with; cleared here
+    int32_t* counts;   // the results, written here where there is one chunk
+    int32_t* tokens;
+    float* loss;
 };
 
-// LDS words of forward: column sums and counts, and per wave the (expert,
-// score) of the selected slots of its rows.
-inline size_t fwd_lds_bytes(int E, int k, int rows, bool select) {
-    return (2 * size_t(E) + (select ? 2 * size_t(rows) * size_t(k) : 0)) * 4;
+struct Slot {
+    int e;
+    float s;
+};
+
+// LDS of forward: column sums, counts, the bias, and the selected slots of each
+// row (8-byte aligned) from word slots_at() on.
+__host__ __device__ constexpr int slots_at(int col_rows, int E) { return ((col_rows + 2) * E + 1) & ~1; }
+inline size_t fwd_lds_bytes(int E, int k, int R, int rows, bool select) {
+    return size_t(slots_at(fwd_col_rows(R), E)) * 4 + (select ? size_t(rows) * size_t(k) * sizeof(Slot) : 0);
+}
+
+__device__ __forceinline__ float loss_value(double dot, int E, int k, int n) {
+    return n > 0 ? float(dot * E / (double(k) * n * n)) : 0.0f;
+}
+
+__device__ __forceinline__ double wave_sum_f64(double x) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+// The experts of the k largest keys score + bias of a row to stage[0..k), equal
+// keys by the lowest expert, -1 where none is left.
+//
+// Keys are 31-bit integers, the ordered key above and the inverted expert below,
+// so that no two are the same.  A round then needs no search and no marking of
+// what was taken: with m the last winner, u - m as an unsigned number is large
+// only for the u below m, and largest for the one next to it.  16-bit scores
+// without a bias fit whole.  A 32-bit key loses its low bits; where two winners
+// in a row agree in what is left (the one behind the last among them), their
+// wave selects again by whole keys.  65536 rows of 256 fp32 scores, k = 8:
+// 52 us for the forward with the whole keys alone.
+template <class T, class S>
+__device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, const float* bias, bool plan, int gl,
+                                       int E, int k, Slot* stage) {
+    constexpr unsigned kMask = S::G * S::EL - 1;  // a power of two less one
+    constexpr int kBits = __builtin_popcount(kMask);
+    // Ordered keys of a row, kTaken where an expert is not available.
+    auto keys = [&](const RawRow<T, S>& from, int (&key)[S::EL]) {
+        float x[S::EL];
+        from.get(gl, E, x);
+#pragma unroll
+        for (int j = 0; j < S::EL; ++j) {
+            const int e = S::expert(gl, j);
+            const float t = x[j] + (bias && e < E ? bias[e] : 0.0f);
+            key[j] = t > kNegInf && (!plan || x[j] > 0.0f) ? ordered(t) : kTaken;
+        }
+    };
+    int key[S::EL];
+    unsigned u[S::EL];
+    keys(raw, key);
+#pragma unroll
+    for (int j = 0; j < S::EL; ++j) {
+        // kTaken becomes 0; the low bits of a 16-bit score's key are all alike
+        const unsigned upper = (unsigned(key[j]) ^ 0x80000000u) >> (kBits + 1);
+        u[j] = key[j] == kTaken ? 0u : (upper << kBits) | (kMask - unsigned(S::expert(gl, j)));
+    }
+    unsigned m = 0x80000000u;
+    bool close = false;  // winners that agree in the key's upper bits
+    for (int r = 0; r <= k; ++r) {
+        unsigned d = u[0] - m;
+#pragma unroll
+        for (int j = 1; j < S::EL; ++j) d = max(d, u[j] - m);
+        d = group_reduce<S::G>(d, OpMaxUint{});
+        const unsigned next = m == 0u ? 0u : m + d;
+        close |= next != 0u && ((next ^ m) >> kBits) == 0u;
+        m = next;
+        if (r < k && gl == (r & (S::G - 1))) stage[r].e = m ? int(kMask - (m & kMask)) : -1;
+    }
+    wave_lds_fence();
+    const bool whole = sizeof(T) == 2 && !bias;
+    if (whole || !__any(close)) return;
+
+    // Whole keys; the row is read again rather than kept over the rounds above.
+    RawRow<T, S> again;
+    again.load(row, gl, E, raw.live);
+    keys(again, key);
+    for (int r = 0; r < k; ++r) {
+        int top = key[0];
+#pragma unroll
+        for (int j = 1; j < S::EL; ++j) top = max(top, key[j]);
+        top = group_reduce<S::G>(top, OpMaxInt{});
+        int first = INT32_MAX;  // this lane's first element with that key
+#pragma unroll
+        for (int j = S::EL - 1; j >= 0; --j) first = key[j] == top ? j : first;
+        const int mine = first == INT32_MAX ? INT32_MAX : S::expert(gl, first);
+        const int e = group_reduce<S::G>(mine, OpMinInt{});
+        const int take = e == mine ? first : -1;
+#pragma unroll
+        for (int j = 0; j < S::EL; ++j) key[j] = j == take ? kTaken : key[j];
+        if (gl == (r & (S::G - 1))) stage[r].e = top == kTaken ? -1 : e;
+    }
+    wave_lds_fence();
 }
 
 template <class T, class S, bool SELECT>
-__global__ __launch_bounds__(kBlock) void forward(FwdArgs a) {
+__global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdArgs a) {
+    constexpr int kThreads = fwd_block(S::R), kWaves = kThreads / kWave;
     extern __shared__ float lds[];
     __shared__ int ntokens;
+    __shared__ double wdot[kWaves];
     const int b = batch_of_block();
     if (b >= a.B) return;
     const int E = a.E, k = a.k;
+    constexpr int kColRows = fwd_col_rows(S::R);
     float* col = lds;
-    int* hist = reinterpret_cast<int*>(lds + E);
-    for (int e = threadIdx.x; e < E; e += kBlock) {
-        col[e] = 0.0f;
+    int* hist = reinterpret_cast<int*>(lds + kColRows * E);
+    float* bias = lds + (kColRows + 1) * E;
+    for (int e = threadIdx.x; e < E; e += kThreads) {
         hist[e] = 0;
+        if (SELECT && a.bias) bias[e] = a.bias[e];
     }
     if (threadIdx.x == 0) ntokens = 0;
     __syncthreads();
 
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const int gl = lane % S::G, sub = lane / S::G;
-    struct Slot {
-        int e;
-        float s;
-    };
-    Slot* stage = reinterpret_cast<Slot*>(lds + 2 * E) + size_t(wave) * S::RPW * k + size_t(sub) * k;
-    float bias[S::EL];
-#pragma unroll
-    for (int j = 0; j < S::EL; ++j) {
-        const int e = S::expert(gl, j);
-        bias[j] = (SELECT && a.bias && e < E) ? a.bias[e] : 0.0f;
-    }
+    Slot* stage = reinterpret_cast<Slot*>(lds + slots_at(kColRows, E)) + size_t(wave * S::RPW + sub) * k;
     float acc[S::EL];
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) acc[j] = 0.0f;
@@ -247,67 +400,59 @@ __global__ __launch_bounds__(kBlock) void forward(FwdArgs a) {
 
     const int begin = int(blockIdx.x) * a.chunk_rows;
     const int end = min(begin + a.chunk_rows, a.N);
-    for (int base = begin + wave * S::RPW; base < end; base += kWavesPerBlock * S::RPW) {
+    const T* scores = static_cast<const T*>(a.scores) + int64_t(b) * a.sb;
+    const int64_t row0 = int64_t(b) * a.N;
+
+    RawRow<T, S> next;
+    auto fetch = [&](int base) {
+        const int n = base + sub;
+        const bool live = n < end && (!a.mask || a.mask[row0 + n]);
+        next.load(scores + int64_t(n) * a.sn, gl, E, live);
+    };
+    fetch(begin + wave * S::RPW);
+    if constexpr (!SELECT) {
+        const int64_t first = (row0 + begin) * k, count = int64_t(max(end - begin, 0)) * k;
+        for (int64_t i = threadIdx.x; i < count; i += kThreads) {
+            const int64_t e = int_at(a.given, a.given64, first + i);
+            if (e >= 0 && e < E && (!a.mask || a.mask[(first + i) / k])) atomicAdd(&hist[e], 1);
+        }
+    }
+    for (int base = begin + wave * S::RPW; base < end; base += kWaves * S::RPW) {
+        const RawRow<T, S> raw = next;
+        fetch(base + kWaves * S::RPW);
         const int n = base + sub;
         const bool in = n < end;
-        const int64_t at = int64_t(b) * a.N + n;
-        const bool live = in && (!a.mask || a.mask[at]);
-        live_rows += live && gl == 0;
+        live_rows += raw.live && gl == 0;
         float x[S::EL], q[S::EL], top, inv;
-        load_row<T, S>(static_cast<const T*>(a.scores) + int64_t(b) * a.sb + int64_t(n) * a.sn, gl, E, live, x);
+        raw.get(gl, E, x);
         row_masses<S>(x, a.scoring, q, top, inv);
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) acc[j] = fmaf(q[j], inv, acc[j]);
 
-        if constexpr (!SELECT) {
+        if constexpr (SELECT) {
+            const T* row = scores + int64_t(n) * a.sn;
+            select<T, S>(row, raw, a.bias ? bias : nullptr, a.scoring == DOT_SCORING_PLAN, gl, E, k, stage);
+            // Each slot's expert and score.
             for (int r = gl; r < k; r += S::G) {
-                const int64_t e = live ? int_at(a.given, a.given64, at * k + r) : -1;
-                if (e >= 0 && e < E) atomicAdd(&hist[e], 1);
-            }
-        } else {
-            // Keys; what is not available, or already taken, is -inf.
-            float key[S::EL];
-#pragma unroll
-            for (int j = 0; j < S::EL; ++j) {
-                const float t = x[j] + bias[j];
-                const bool open = t > kNegInf && (a.scoring != DOT_SCORING_PLAN || x[j] > 0.0f);
-                key[j] = open ? t : kNegInf;
-            }
-            float most = kNegInf;  // largest selected score of this lane
-            for (int r = 0; r < k; ++r) {
-                float m = key[0];
-#pragma unroll
-                for (int j = 1; j < S::EL; ++j) m = fmaxf(m, key[j]);
-                m = group_reduce<S::G>(m, OpMax{});
-                const bool any = m > kNegInf;
-                int e = INT32_MAX;
-#pragma unroll
-                for (int j = S::EL - 1; j >= 0; --j) e = key[j] == m ? S::expert(gl, j) : e;
-                e = group_reduce<S::G>(e, OpMinInt{});
+                const int e = stage[r].e;
                 float s = 0.0f;
-                bool owner = false;
-#pragma unroll
-                for (int j = 0; j < S::EL; ++j) {
-                    const bool hit = any && S::expert(gl, j) == e;
-                    owner |= hit;
-                    s = hit ? x[j] : s;
-                    key[j] = hit ? kNegInf : key[j];
-                }
-                if (owner) {
-                    stage[r] = Slot{e, s};
-                    most = fmaxf(most, s);
+                if (e >= 0) {
+                    s = to_float(row[e]);
                     atomicAdd(&hist[e], 1);
-                } else if (!any && gl == 0) {
-                    stage[r] = Slot{-1, 0.0f};
                 }
+                stage[r].s = s;
             }
-            wave_lds_fence();
             // Weights: exp(s - top) or q(s), over the row's or the selected ones' sum.
             const bool soft = a.scoring == DOT_SCORING_SOFTMAX;
-            float scale = soft ? inv : 1.0f;
+            float scale = soft ? inv : 1.0f, over = 1.0f;
             if (a.normalize) {
                 if (soft) {
-                    const float m = group_reduce<S::G>(most, OpMax{});
+                    float m = kNegInf;
+                    for (int r = gl; r < k; r += S::G) {
+                        const Slot t = stage[r];
+                        if (t.e >= 0) m = fmaxf(m, t.s);
+                    }
+                    m = group_reduce<S::G>(m, OpMax{});
                     top = m == kNegInf ? 0.0f : m;
                 }
                 float z = 0.0f;
@@ -316,78 +461,136 @@ __global__ __launch_bounds__(kBlock) void forward(FwdArgs a) {
                     if (t.e >= 0) z += soft ? fast_exp(t.s - top) : mass_of(t.s, a.scoring);
                 }
                 z = group_reduce<S::G>(z, OpSum{});
-                scale = z == 0.0f ? 0.0f : 1.0f / z;
-                if (soft) scale += inv - inv;  // a row with NaN has no weights
+                // a division, so that a single expert's weight is 1 and its gradient 0
+                over = z == 0.0f ? 1.0f : z;
+                scale = soft ? 1.0f + (inv - inv) : 1.0f;  // a row with NaN has no weights
             }
+            const int64_t at = (row0 + n) * k;
             for (int r = gl; r < k; r += S::G) {
                 const Slot t = stage[r];
-                const float w = soft ? fast_exp(t.s - top) : mass_of(t.s, a.scoring);
                 if (in) {
-                    a.weights[at * k + r] = t.e >= 0 ? w * scale : 0.0f;
-                    a.experts[at * k + r] = t.e;
+                    const float w = soft ? fast_exp(t.s - top) : mass_of(t.s, a.scoring);
+                    a.weights[at + r] = t.e >= 0 ? w * scale / over : 0.0f;
+                    a.experts[at + r] = t.e;
                 }
             }
             wave_lds_fence();  // the next rows write the slots again
         }
     }
 
-    // Column sums of this workgroup: over the rows of a wave, then wave by wave.
+    // Column sums of this workgroup: over the rows of a wave, then over the waves in order.
 #pragma unroll
-    for (int j = 0; j < S::EL; ++j) {
-#pragma unroll
-        for (int d = S::G; d < kWave; d *= 2) acc[j] += __shfl_xor(acc[j], d);
-    }
+    for (int j = 0; j < S::EL; ++j) acc[j] = across_groups<S::G>(acc[j]);
     if (live_rows) atomicAdd(&ntokens, live_rows);
-    for (int w = 0; w < kWavesPerBlock; ++w) {
-        if (wave == w && sub == 0) {
+    for (int w = 0; w < kWaves; w += kColRows) {
+        if (wave >= w && wave < w + kColRows && sub == 0) {
 #pragma unroll
             for (int j = 0; j < S::EL; ++j) {
                 const int e = S::expert(gl, j);
-                if (e < E) col[e] += acc[j];
+                if (e < E) col[(wave - w) * E + e] = acc[j] + (w ? col[(wave - w) * E + e] : 0.0f);
             }
         }
         __syncthreads();
     }
+    if constexpr (kColRows > 1) {
+        for (int e = threadIdx.x; e < E; e += kThreads) {
+            float s = col[e];
+            for (int w = 1; w < kColRows; ++w) s += col[w * E + e];
+            col[e] = s;
+        }
+        // the thread that adds up a column is the one that reads it below
+    }
+    if (a.nchunks == 1) {  // nothing to join
+        double dot = 0.0;
+        for (int e = threadIdx.x; e < E; e += kThreads) {
+            a.counts[int64_t(b) * E + e] = hist[e];
+            dot += double(col[e]) * hist[e];
+        }
+        dot = wave_sum_f64(dot);
+        if (lane == 0) wdot[wave] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kWaves; ++w) dot += wdot[w];
+            a.tokens[b] = ntokens;
+            a.loss[b] = loss_value(dot, E, k, ntokens);
+        }
+        return;
+    }
     const int64_t part = int64_t(b) * a.nchunks + blockIdx.x;
-    for (int e = threadIdx.x; e < E; e += kBlock) {
+    for (int e = threadIdx.x; e < E; e += kThreads) {
         a.psum[part * E + e] = col[e];
         a.pcount[part * E + e] = hist[e];
     }
-    if (threadIdx.x == 0) a.ptokens[part] = ntokens;
+    if (threadIdx.x == 0) {
+        a.ptokens[part] = ntokens;
+        if (blockIdx.x == 0) a.done[b] = 0;
+    }
 }
 
-// Counts, tokens and the loss of a batch element from its chunks' partials.
-__global__ __launch_bounds__(kBlock) void finish(int B, int E, int k, int nchunks, const float* psum,
-                                                 const int32_t* pcount, const int32_t* ptokens, int32_t* counts,
-                                                 int32_t* tokens, float* loss) {
-    __shared__ double wsum[kWavesPerBlock];
+constexpr int kFinishBlock = 1024, kFinishCols = 64, kSlices = kFinishBlock / kFinishCols;
+
+struct FinishArgs {
+    int B, E, k, nchunks;
+    const float* psum;
+    const int32_t* pcount;
+    const int32_t* ptokens;
+    double* dots;    // [B, gridDim.x]
+    uint32_t* done;  // [B], 0
+    int32_t* counts;
+    int32_t* tokens;
+    float* loss;
+};
+
+// Counts and loss of a batch element from its chunks' partials: kFinishCols
+// experts per workgroup, whose shares of the loss the last workgroup of the
+// element to arrive adds up in order.
+__global__ __launch_bounds__(kFinishBlock) void finish(FinishArgs a) {
+    __shared__ double sums[kSlices][kFinishCols];
+    __shared__ int cnts[kSlices][kFinishCols];
+    __shared__ int ntok[kFinishBlock / kWave];
     const int b = batch_of_block();
-    if (b >= B) return;
-    const int64_t first = int64_t(b) * nchunks;
-    int n = 0;
-    for (int c = 0; c < nchunks; ++c) n += ptokens[first + c];
-    double dot = 0.0;
-    for (int e = threadIdx.x; e < E; e += kBlock) {
-        double s = 0.0;
-        int cnt = 0;
-        for (int c = 0; c < nchunks; ++c) {
-            s += psum[(first + c) * E + e];
-            cnt += pcount[(first + c) * E + e];
+    if (b >= a.B) return;
+    const int lane = threadIdx.x % kFinishCols, slice = threadIdx.x / kFinishCols;
+    const int e = int(blockIdx.x) * kFinishCols + lane;
+    const int64_t first = int64_t(b) * a.nchunks;
+    double s = 0.0;
+    int cnt = 0, n = 0;
+    if (e < a.E) {
+#pragma unroll 8
+        for (int c = slice; c < a.nchunks; c += kSlices) {
+            s += a.psum[(first + c) * a.E + e];
+            cnt += a.pcount[(first + c) * a.E + e];
         }
-        counts[int64_t(b) * E + e] = cnt;
-        dot += s * cnt;
     }
+    for (int c = threadIdx.x; c < a.nchunks; c += kFinishBlock) n += a.ptokens[first + c];
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) dot += __shfl_xor(dot, d);
-    if (threadIdx.x % kWave == 0) wsum[threadIdx.x / kWave] = dot;
+    for (int d = 1; d < kWave; d *= 2) n += __shfl_xor(n, d);
+    sums[slice][lane] = s;
+    cnts[slice][lane] = cnt;
+    if (lane == 0) ntok[slice] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int w = 0; w < kWavesPerBlock; ++w) t += wsum[w];
-        tokens[b] = n;
-        loss[b] = n > 0 ? float(t * E / (double(k) * n * n)) : 0.0f;
+    if (slice != 0) return;
+    for (int t = 1; t < kSlices; ++t) {
+        s += sums[t][lane];
+        cnt += cnts[t][lane];
+        n += ntok[t];
     }
+    if (e < a.E) a.counts[int64_t(b) * a.E + e] = cnt;
+    double dot = wave_sum_f64(s * cnt);
+    if (lane != 0) return;
+    if (gridDim.x > 1) {
+        double* dots = a.dots + int64_t(b) * gridDim.x;
+        __hip_atomic_store(dots + blockIdx.x, dot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t before = __hip_atomic_fetch_add(a.done + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (before + 1 < gridDim.x) return;
+        dot = 0.0;
+        for (unsigned i = 0; i < gridDim.x; ++i)
+            dot += __hip_atomic_load(dots + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    a.tokens[b] = n;
+    a.loss[b] = loss_value(dot, a.E, a.k, n);
 }
+static_assert(kFinishCols == kWave, "a slice is one wave");
 
 struct BwdArgs {
     const void* scores;
@@ -439,45 +642,75 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
 
     const int begin = int(blockIdx.x) * a.chunk_rows;
     const int end = min(begin + a.chunk_rows, a.N);
-    for (int base = begin + wave * S::RPW; base < end; base += kWavesPerBlock * S::RPW) {
+    const T* scores = static_cast<const T*>(a.scores) + int64_t(b) * a.sb;
+    // The next row: its scores, and the first of this lane's slots.
+    struct Slot {
+        int e;
+        float w, dw;
+    };
+    auto slot = [&](int64_t at, int r, bool live) {
+        Slot s{-1, 0.0f, 0.0f};
+        if (live && r < k) {
+            s.e = a.experts[at * k + r];
+            s.dw = a.grad_weights[at * k + r];
+            if (a.normalize) s.w = a.weights[at * k + r];
+            if (unsigned(s.e) >= unsigned(E)) s = Slot{-1, 0.0f, 0.0f};
+        }
+        return s;
+    };
+    RawRow<T, S> next;
+    Slot next_slot{};
+    auto fetch = [&](int base) {
         const int n = base + sub;
-        const bool in = n < end;
         const int64_t at = int64_t(b) * a.N + n;
-        const bool live = in && (!a.mask || a.mask[at]);
-        const T* row = static_cast<const T*>(a.scores) + int64_t(b) * a.sb + int64_t(n) * a.sn;
+        const bool live = n < end && (!a.mask || a.mask[at]);
+        next.load(scores + int64_t(n) * a.sn, gl, E, live);
+        if constexpr (WEIGHTS) next_slot = slot(at, gl, live);
+    };
+    fetch(begin + wave * S::RPW);
+    for (int base = begin + wave * S::RPW; base < end; base += kWavesPerBlock * S::RPW) {
+        const RawRow<T, S> raw = next;
+        const Slot first = next_slot;
+        fetch(base + kWavesPerBlock * S::RPW);
+        const int n = base + sub;
+        const bool in = n < end, live = raw.live;
+        const int64_t at = int64_t(b) * a.N + n;
         float x[S::EL], q[S::EL], top, inv;
-        load_row<T, S>(row, gl, E, live, x);
+        raw.get(gl, E, x);
         row_masses<S>(x, a.scoring, q, top, inv);
         float add[S::EL];
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) add[j] = 0.0f;
         if constexpr (WEIGHTS) {
-#pragma unroll
-            for (int j = 0; j < S::EL; ++j) spread[S::expert(gl, j)] = 0.0f;
-            float dot = 0.0f, scale = 1.0f;
+            float dot = 0.0f, over = 1.0f;
             if (a.normalize) {
                 float mass = 0.0f;
+                if (!soft) {  // the selected masses, from their lanes
+#pragma unroll
+                    for (int j = 0; j < S::EL; ++j) spread[S::expert(gl, j)] = q[j];
+                    wave_lds_fence();
+                }
                 for (int r = gl; r < k; r += S::G) {
-                    const int e = live ? a.experts[at * k + r] : -1;
-                    if (e >= 0 && e < E) {
-                        dot = fmaf(a.weights[at * k + r], a.grad_weights[at * k + r], dot);
-                        if (!soft) mass += mass_of(to_float(row[e]), a.scoring);
-                    }
+                    const Slot s = r == gl ? first : slot(at, r, live);
+                    if (s.e < 0) continue;
+                    dot = fmaf(s.w, s.dw, dot);
+                    if (!soft) mass += spread[s.e];
                 }
                 dot = group_reduce<S::G>(dot, OpSum{});
                 if (!soft) {
                     mass = group_reduce<S::G>(mass, OpSum{});
-                    scale = mass == 0.0f ? 0.0f : 1.0f / mass;
+                    over = mass == 0.0f ? __builtin_inff() : mass;
+                    wave_lds_fence();
                 }
             }
+#pragma unroll
+            for (int j = 0; j < S::EL; ++j) spread[S::expert(gl, j)] = 0.0f;
             wave_lds_fence();
             for (int r = gl; r < k; r += S::G) {
-                const int e = live ? a.experts[at * k + r] : -1;
-                if (e >= 0 && e < E) {
-                    float v = (a.grad_weights[at * k + r] - dot) * scale;
-                    if (soft && a.normalize) v *= a.weights[at * k + r];
-                    spread[e] = v;
-                }
+                const Slot s = r == gl ? first : slot(at, r, live);
+                if (s.e < 0) continue;
+                const float v = s.dw - dot;
+                spread[s.e] = !a.normalize ? s.dw : soft ? s.w * v : v / over;
             }
             wave_lds_fence();
 #pragma unroll

@@ -11,18 +11,40 @@ struct FwdLayout {
     float* psum;
     int32_t* pcount;
     int32_t* ptokens;
-    int nchunks;
+    double* dots;
+    uint32_t* done;
+    int vectors, threads, rows, nchunks, colblocks;
     size_t bytes;
 };
 
+// Lanes of a row and vectors of a lane for E experts.
+struct Lanes {
+    int g, r;
+};
+template <bool PAIRS>
+Lanes lanes_of(int E) {
+    Lanes l{};
+    routing::dispatch_shape<true, PAIRS>(E, [&](auto s) { l = {decltype(s)::G, decltype(s)::R}; });
+    return l;
+}
+
+// About 512 workgroups, two per CU.
 FwdLayout fwd_layout(void* ws, int B, int N, int E) {
     Carver c(ws);
     FwdLayout L{};
-    L.nchunks = routing::chunks_of(B, N, E);
+    const Lanes lanes = lanes_of<true>(E);
+    L.vectors = lanes.r;
+    L.threads = routing::fwd_block(lanes.r);
+    L.rows = L.threads / lanes.g;
+    L.nchunks = routing::chunks_of(B, N, L.rows, 512);
+    L.colblocks = (E + routing::kFinishCols - 1) / routing::kFinishCols;
+    if (L.nchunks == 1) return L;
     const size_t parts = size_t(B) * L.nchunks;
     L.psum = c.take<float>(parts * E);
     L.pcount = c.take<int32_t>(parts * E);
     L.ptokens = c.take<int32_t>(parts);
+    L.dots = c.take<double>(size_t(B) * L.colblocks);
+    L.done = c.take<uint32_t>(B);
     L.bytes = c.used();
     return L;
 }
@@ -46,11 +68,11 @@ bool rows_aligned(const void* p, int64_t sb, int64_t sn, int E, int dtype) {
     return E % routing::kV == 0 && aligned16(p) && (sb * bytes) % 16 == 0 && (sn * bytes) % 16 == 0;
 }
 
-template <class F>
+template <bool PAIRS, class F>
 void dispatch(int dtype, int E, bool vec, F&& f) {
     dispatch_dtype(dtype, [&](auto t) {
-        if (vec) routing::dispatch_shape<true>(E, [&](auto s) { f(t, s); });
-        else routing::dispatch_shape<false>(E, [&](auto s) { f(t, s); });
+        if (vec) routing::dispatch_shape<true, PAIRS>(E, [&](auto s) { f(t, s); });
+        else routing::dispatch_shape<false, PAIRS>(E, [&](auto s) { f(t, s); });
     });
 }
 
@@ -76,7 +98,7 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     if (a->N > 0 && (!a->scores || (select && (!a->weights || !a->experts))))
         return fail(DOT_ERR_INVALID_ARG, "scores, weights and experts must be non-NULL");
     const FwdLayout L = fwd_layout(a->workspace, a->B, a->N, a->E);
-    if (!a->workspace || a->workspace_bytes < L.bytes)
+    if (L.bytes > 0 && (!a->workspace || a->workspace_bytes < L.bytes))
         return fail(DOT_ERR_WORKSPACE, "workspace smaller than dot_routing_forward_workspace_bytes()");
     routing::FwdArgs x{};
     x.scores = a->scores;
@@ -99,20 +121,27 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     x.psum = L.psum;
     x.pcount = L.pcount;
     x.ptokens = L.ptokens;
+    x.done = L.done;
+    x.counts = a->counts;
+    x.tokens = a->tokens;
+    x.loss = a->loss;
     const dim3 grid = batch_grid(unsigned(L.nchunks), a->B);
-    const size_t lds = routing::fwd_lds_bytes(a->E, a->k, routing::rows_per_pass(a->E), select);
-    dispatch(a->dtype, a->E, rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype), [&](auto t, auto s) {
+    const size_t lds = routing::fwd_lds_bytes(a->E, a->k, L.vectors, L.rows, select);
+    dispatch<true>(a->dtype, a->E, rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype), [&](auto t, auto s) {
         ProfScope prof("routing_forward", stream);
         if (select)
-            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), true>), grid, dim3(kBlock), lds, stream, x);
+            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), true>), grid, dim3(L.threads), lds, stream,
+                               x);
         else
-            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), false>), grid, dim3(kBlock), lds, stream,
+            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), false>), grid, dim3(L.threads), lds, stream,
                                x);
     });
-    {
+    if (L.nchunks > 1) {
         ProfScope prof("routing_finish", stream);
-        hipLaunchKernelGGL(routing::finish, batch_grid(1, a->B), dim3(kBlock), 0, stream, a->B, a->E, a->k, L.nchunks,
-                           L.psum, L.pcount, L.ptokens, a->counts, a->tokens, a->loss);
+        const routing::FinishArgs f{a->B, a->E, a->k, L.nchunks, L.psum, L.pcount, L.ptokens, L.dots, L.done,
+                                    a->counts, a->tokens, a->loss};
+        hipLaunchKernelGGL(routing::finish, batch_grid(unsigned(L.colblocks), a->B), dim3(routing::kFinishBlock), 0,
+                           stream, f);
     }
     return check_launch("dot_routing_forward");
 }
@@ -146,11 +175,11 @@ extern "C" int dot_routing_backward(const dot_routing_bwd_args* a, dot_stream_t 
     x.experts = a->experts;
     x.grad_weights = a->grad_weights;
     x.grad_scores = a->grad_scores;
-    x.nchunks = routing::chunks_of(a->B, a->N, a->E);
+    x.nchunks = routing::chunks_of(a->B, a->N, kBlock / lanes_of<false>(a->E).g, 2048);
     x.chunk_rows = (a->N + x.nchunks - 1) / x.nchunks;
     const dim3 grid = batch_grid(unsigned(x.nchunks), a->B);
     const bool vec = rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype) && aligned16(a->grad_scores);
-    dispatch(a->dtype, a->E, vec, [&](auto t, auto s) {
+    dispatch<false>(a->dtype, a->E, vec, [&](auto t, auto s) {
         using S = decltype(s);
         ProfScope prof("routing_backward", stream);
         const size_t lds = routing::bwd_lds_bytes(kWave * S::EL, a->grad_weights != nullptr);

@@ -277,10 +277,11 @@ def test_c_abi_refusals(lib):
     refused(lib, f, INVALID, "scoring", RoutingFwd(**{**ok, "scoring": 3}))
     refused(lib, f, INVALID, "non-NULL", RoutingFwd(**{**ok, "loss": None}))
     refused(lib, f, INVALID, "non-NULL", RoutingFwd(**{**ok, "experts": None}))
-    refused(lib, f, WORKSPACE, "workspace", RoutingFwd(**ok))
-    need = lib.dot_routing_forward_workspace_bytes(2, 4, 8)
+    many = {**ok, "N": 100000}  # few tokens are joined in one workgroup and need none
+    refused(lib, f, WORKSPACE, "workspace", RoutingFwd(**many))
+    need = lib.dot_routing_forward_workspace_bytes(2, 100000, 8)
     assert need > 0 and lib.dot_routing_forward_workspace_bytes(-1, 4, 8) == 0
-    refused(lib, f, WORKSPACE, "workspace", RoutingFwd(**ok, workspace=some, workspace_bytes=need - 1))
+    refused(lib, f, WORKSPACE, "workspace", RoutingFwd(**many, workspace=some, workspace_bytes=need - 1))
     b = dict(scores=some, B=2, N=4, E=8, k=2, counts=some, tokens=some, grad_loss=some, grad_scores=some)
     f = "dot_routing_backward"
     refused(lib, f, INVALID, "non-NULL", RoutingBwd(**{**b, "grad_scores": None}))
