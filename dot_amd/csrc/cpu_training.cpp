@@ -165,18 +165,23 @@ std::vector<Tensor> routing_forward_cpu(Tensor scores_, int64_t k, int64_t scori
             lp[b] = n > 0 ? float(dot * E / (k * n * n)) : 0.0f;
         }
     });
-    return {weights, experts, counts, tokens, loss};
+    std::vector<Tensor> out{counts, loss};
+    if (select) out.insert(out.end(), {weights, experts});
+    if (mask.defined()) out.push_back(tokens);
+    return out;
 }
 
 Tensor routing_backward_cpu(Tensor scores_, int64_t k, int64_t scoring, bool normalize, optional<Tensor> mask_,
-                            Tensor counts_, Tensor tokens_, optional<Tensor> grad_loss_, optional<Tensor> weights_,
-                            optional<Tensor> experts_, optional<Tensor> grad_weights_) {
+                            Tensor counts_, optional<Tensor> tokens_, optional<Tensor> grad_loss_,
+                            optional<Tensor> weights_, optional<Tensor> experts_, optional<Tensor> grad_weights_) {
     check_floats(scores_, "scores");
     const Tensor scores = scores_.to(at::kFloat).contiguous();
     const int64_t B = scores.size(0), N = scores.size(1), E = scores.size(2);
     check_routing(E, k, scoring, false);
     const Tensor mask = mask_of(mask_, scores);
-    const Tensor counts = longs(counts_, "counts"), tokens = longs(tokens_, "tokens");
+    const Tensor counts = longs(counts_, "counts");
+    TORCH_CHECK(tokens_.has_value() == mask.defined(), "tokens come with a mask");
+    const Tensor tokens = tokens_.has_value() ? longs(*tokens_, "tokens") : at::full({B}, N, counts.options());
     const Tensor gl = f32c(grad_loss_, "grad_loss"), gw = f32c(grad_weights_, "grad_weights");
     TORCH_CHECK(counts.numel() == B * E && tokens.numel() == B && (!gl.defined() || gl.numel() == B),
                 "counts, tokens and grad_loss must have shapes [B, E], [B] and [B]");
@@ -283,8 +288,8 @@ std::vector<Tensor> sequence_logp_forward_cpu(Tensor logits, Tensor tokens, opti
                     "ref_logp must have shape [B] or [B, S]");
     }
     Tensor value = at::zeros({p.B, p.S}, f32.dtype(at::kDouble));
-    Tensor stats = at::zeros(keep ? at::IntArrayRef({p.B, p.S, 2}) : at::IntArrayRef({0}), f32);
-    Tensor weight = at::ones({keep ? p.B : 0}, f32);
+    // as for HIP tensors: row statistics (which the backward here forms again), then weights
+    Tensor saved = at::ones({keep ? (2 * p.S + 1) * p.B : 0}, f32);
     double* vp = value.data_ptr<double>();
     at::parallel_for(0, p.B * p.S, 1, [&](int64_t r0, int64_t r1) {
         for (int64_t r = r0; r < r1; ++r) {
@@ -293,13 +298,9 @@ std::vector<Tensor> sequence_logp_forward_cpu(Tensor logits, Tensor tokens, opti
             const auto [top, sum] = row_lse(p.row(r), p.V, tau);
             vp[r] = (double(p.row(r)[t]) - top) / tau - std::log(sum);
             if (ref.defined() && ref.dim() == 2) vp[r] -= ref.const_data_ptr<double>()[r];
-            if (keep) {
-                stats.data_ptr<float>()[2 * r] = float(top);
-                stats.data_ptr<float>()[2 * r + 1] = float(1.0 / sum);
-            }
         }
     });
-    if (reduction == DOT_REDUCE_NONE) return {value.to(at::kFloat), stats, weight};
+    if (reduction == DOT_REDUCE_NONE) return {value.to(at::kFloat), saved};
     Tensor out = at::empty({p.B}, f32);
     for (int64_t b = 0; b < p.B; ++b) {
         double sum = 0.0;
@@ -313,17 +314,18 @@ std::vector<Tensor> sequence_logp_forward_cpu(Tensor logits, Tensor tokens, opti
         sum *= w;
         if (ref.defined() && ref.dim() == 1) sum -= ref.const_data_ptr<double>()[b];
         out.data_ptr<float>()[b] = float(sum);
-        if (keep) weight.data_ptr<float>()[b] = float(w);
+        if (keep) saved.data_ptr<float>()[2 * p.B * p.S + b] = float(w);
     }
-    return {out, stats, weight};
+    return {out, saved};
 }
 
 Tensor sequence_logp_backward_cpu(Tensor logits, Tensor tokens, optional<Tensor> mask, double tau, int64_t reduction,
-                                  Tensor, Tensor weight_, Tensor grad_out_) {
+                                  Tensor saved_, Tensor grad_out_) {
     const Positions p(logits, tokens, mask);
-    const Tensor go = f32c(grad_out_, "grad_out"), weight = f32c(weight_, "weight");
+    const Tensor go = f32c(grad_out_, "grad_out"), saved = f32c(saved_, "saved");
     const bool per_token = reduction == DOT_REDUCE_NONE;
-    TORCH_CHECK(go.numel() == (per_token ? p.B * p.S : p.B) && weight.numel() == p.B, "grad_out has the wrong size");
+    TORCH_CHECK(go.numel() == (per_token ? p.B * p.S : p.B) && saved.numel() == (2 * p.S + 1) * p.B, "grad_out has the wrong size");
+    const float* weight = saved.const_data_ptr<float>() + 2 * p.B * p.S;
     Tensor grad = at::zeros({p.B, p.S, p.V}, p.logits.options());
     float* out = grad.data_ptr<float>();
     at::parallel_for(0, p.B * p.S, 1, [&](int64_t r0, int64_t r1) {
@@ -331,7 +333,7 @@ Tensor sequence_logp_backward_cpu(Tensor logits, Tensor tokens, optional<Tensor>
             const int64_t t = p.token(r);
             if (t < 0) continue;
             const int64_t b = r / p.S;
-            const double c = double(go.const_data_ptr<float>()[per_token ? r : b]) * weight.const_data_ptr<float>()[b] / tau;
+            const double c = double(go.const_data_ptr<float>()[per_token ? r : b]) * weight[b] / tau;
             const float* x = p.row(r);
             const auto [top, sum] = row_lse(x, p.V, tau);
             for (int64_t v = 0; v < p.V; ++v)

@@ -101,11 +101,11 @@ __device__ __forceinline__ X group_reduce(X x, Op op) {
     return x;
 }
 
-// Floats as integers of the same order, and back (-0 counts as 0).  Integer
+// Floats as integers of the same order (-0 below 0), and back.  Integer
 // maxima fuse with the lane exchanges, those of floats do not.
 constexpr int kTaken = INT32_MIN;  // below every float
 __device__ __forceinline__ int ordered(float x) {
-    const int i = __builtin_bit_cast(int, x + 0.0f);
+    const int i = __builtin_bit_cast(int, x);
     return i ^ ((i >> 31) & INT32_MAX);
 }
 __device__ __forceinline__ float unordered(int i) {
@@ -175,8 +175,17 @@ struct RawRow {
     }
     // As floats; elements beyond E, and rows that are not live, are -inf.
     __device__ __forceinline__ void get(int gl, int E, float (&x)[S::EL]) const {
+        if constexpr (S::VEC) {
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) x[j] = live && S::expert(gl, j) < E ? to_float(one[j]) : kNegInf;
+            for (int r = 0; r < S::R; ++r) {
+                const bool in = live && (r * S::G + gl) * kV < E;
+#pragma unroll
+                for (int j = r * kV; j < (r + 1) * kV; ++j) x[j] = in ? to_float(one[j]) : kNegInf;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S::EL; ++j) x[j] = live && S::expert(gl, j) < E ? to_float(one[j]) : kNegInf;
+        }
     }
 };
 
@@ -279,11 +288,13 @@ struct Slot {
     float s;
 };
 
-// LDS of forward: column sums, counts, the bias, and the selected slots of each
-// row (8-byte aligned) from word slots_at() on.
-__host__ __device__ constexpr int slots_at(int col_rows, int E) { return ((col_rows + 2) * E + 1) & ~1; }
-inline size_t fwd_lds_bytes(int E, int k, int R, int rows, bool select) {
-    return size_t(slots_at(fwd_col_rows(R), E)) * 4 + (select ? size_t(rows) * size_t(k) * sizeof(Slot) : 0);
+// LDS of forward: column sums and counts, from word bias_at() on (16-byte
+// aligned) the bias, with a place for every element of a group, and the selected
+// slots of each row.
+__host__ __device__ constexpr int bias_at(int col_rows, int E) { return ((col_rows + 1) * E + 3) & ~3; }
+inline size_t fwd_lds_bytes(int E, int k, int G, int R, int rows, bool select) {
+    const size_t words = size_t(bias_at(fwd_col_rows(R), E)) + size_t(G) * R * kV;
+    return words * 4 + (select ? size_t(rows) * size_t(k) * sizeof(Slot) : 0);
 }
 
 __device__ __forceinline__ float loss_value(double dot, int E, int k, int n) {
@@ -312,15 +323,18 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
                                        int E, int k, Slot* stage) {
     constexpr unsigned kMask = S::G * S::EL - 1;  // a power of two less one
     constexpr int kBits = __builtin_popcount(kMask);
-    // Ordered keys of a row, kTaken where an expert is not available.
+    // Ordered keys of a row, kTaken where an expert is not available.  (The bias
+    // has a place for every element; adding it, or 0, makes -0 a 0.)
     auto keys = [&](const RawRow<T, S>& from, int (&key)[S::EL]) {
         float x[S::EL];
         from.get(gl, E, x);
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) {
-            const int e = S::expert(gl, j);
-            const float t = x[j] + (bias && e < E ? bias[e] : 0.0f);
-            key[j] = t > kNegInf && (!plan || x[j] > 0.0f) ? ordered(t) : kTaken;
+            const float t = x[j] + (bias ? bias[S::expert(gl, j)] : 0.0f);
+            const int o = ordered(t);
+            bool open = t > kNegInf;
+            if (plan) open = x[j] > 0.0f;
+            key[j] = open ? o : kTaken;
         }
     };
     int key[S::EL];
@@ -328,21 +342,27 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
     keys(raw, key);
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) {
-        // kTaken becomes 0; the low bits of a 16-bit score's key are all alike
-        const unsigned upper = (unsigned(key[j]) ^ 0x80000000u) >> (kBits + 1);
-        u[j] = key[j] == kTaken ? 0u : (upper << kBits) | (kMask - unsigned(S::expert(gl, j)));
+        // the key's low bits give way to the expert (those of a 16-bit score are all alike); kTaken becomes 0
+        const unsigned upper = (unsigned(key[j]) ^ 0x80000000u) >> 1;
+        const unsigned both = (upper & ~kMask) | (kMask - unsigned(S::expert(gl, j)));
+        u[j] = key[j] == kTaken ? 0u : both;
     }
     unsigned m = 0x80000000u;
     bool close = false;  // winners that agree in the key's upper bits
-    for (int r = 0; r <= k; ++r) {
-        unsigned d = u[0] - m;
+    for (int r0 = 0; r0 <= k; r0 += S::G) {
+        unsigned mine = 0;  // the winner of round r0 + gl
+        const int rounds = min(k + 1 - r0, S::G);
+        for (int r = 0; r < rounds; ++r) {
+            unsigned d = u[0] - m;
 #pragma unroll
-        for (int j = 1; j < S::EL; ++j) d = max(d, u[j] - m);
-        d = group_reduce<S::G>(d, OpMaxUint{});
-        const unsigned next = m == 0u ? 0u : m + d;
-        close |= next != 0u && ((next ^ m) >> kBits) == 0u;
-        m = next;
-        if (r < k && gl == (r & (S::G - 1))) stage[r].e = m ? int(kMask - (m & kMask)) : -1;
+            for (int j = 1; j < S::EL; ++j) d = max(d, u[j] - m);
+            d = group_reduce<S::G>(d, OpMaxUint{});
+            const unsigned next = m == 0u ? 0u : m + d;
+            close |= next != 0u && ((next ^ m) >> kBits) == 0u;
+            m = next;
+            mine = r == gl ? m : mine;
+        }
+        if (r0 + gl < k) stage[r0 + gl].e = mine ? int(kMask - (mine & kMask)) : -1;
     }
     wave_lds_fence();
     const bool whole = sizeof(T) == 2 && !bias;
@@ -382,17 +402,16 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
     constexpr int kColRows = fwd_col_rows(S::R);
     float* col = lds;
     int* hist = reinterpret_cast<int*>(lds + kColRows * E);
-    float* bias = lds + (kColRows + 1) * E;
-    for (int e = threadIdx.x; e < E; e += kThreads) {
-        hist[e] = 0;
-        if (SELECT && a.bias) bias[e] = a.bias[e];
-    }
+    float* bias = lds + bias_at(kColRows, E);
+    for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
+    if (SELECT && a.bias)
+        for (int e = threadIdx.x; e < S::G * S::EL; e += kThreads) bias[e] = e < E ? a.bias[e] + 0.0f : 0.0f;
     if (threadIdx.x == 0) ntokens = 0;
     __syncthreads();
 
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const int gl = lane % S::G, sub = lane / S::G;
-    Slot* stage = reinterpret_cast<Slot*>(lds + slots_at(kColRows, E)) + size_t(wave * S::RPW + sub) * k;
+    Slot* stage = reinterpret_cast<Slot*>(lds + bias_at(kColRows, E) + S::G * S::EL) + size_t(wave * S::RPW + sub) * k;
     float acc[S::EL];
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) acc[j] = 0.0f;
@@ -511,7 +530,7 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < kWaves; ++w) dot += wdot[w];
-            a.tokens[b] = ntokens;
+            if (a.tokens) a.tokens[b] = ntokens;
             a.loss[b] = loss_value(dot, E, k, ntokens);
         }
         return;
@@ -587,7 +606,7 @@ __global__ __launch_bounds__(kFinishBlock) void finish(FinishArgs a) {
         for (unsigned i = 0; i < gridDim.x; ++i)
             dot += __hip_atomic_load(dots + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    a.tokens[b] = n;
+    if (a.tokens) a.tokens[b] = n;
     a.loss[b] = loss_value(dot, a.E, a.k, n);
 }
 static_assert(kFinishCols == kWave, "a slice is one wave");
@@ -629,10 +648,10 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
     // sum to 1, and does not lose the digits that balanced counts share.
     float slope[S::EL];
     double coef = 0.0, mean = 0.0;
-    if (a.grad_loss && a.tokens[b] > 0) {
-        const double n = a.tokens[b];
-        coef = double(a.grad_loss[a.grad_loss_scalar ? 0 : b]) * E / (double(k) * n * n);
-        mean = double(k) * n / E;
+    const double n_b = a.tokens ? a.tokens[b] : a.N;
+    if (a.grad_loss && n_b > 0) {
+        coef = double(a.grad_loss[a.grad_loss_scalar ? 0 : b]) * E / (double(k) * n_b * n_b);
+        mean = double(k) * n_b / E;
     }
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) {

@@ -7,16 +7,6 @@
 namespace dot_amd {
 namespace {
 
-struct FwdLayout {
-    float* psum;
-    int32_t* pcount;
-    int32_t* ptokens;
-    double* dots;
-    uint32_t* done;
-    int vectors, threads, rows, nchunks, colblocks;
-    size_t bytes;
-};
-
 // Lanes of a row and vectors of a lane for E experts.
 struct Lanes {
     int g, r;
@@ -28,12 +18,23 @@ Lanes lanes_of(int E) {
     return l;
 }
 
+struct FwdLayout {
+    float* psum;
+    int32_t* pcount;
+    int32_t* ptokens;
+    double* dots;
+    uint32_t* done;
+    Lanes lanes;
+    int threads, rows, nchunks, colblocks;
+    size_t bytes;
+};
+
 // About 512 workgroups, two per CU.
 FwdLayout fwd_layout(void* ws, int B, int N, int E) {
     Carver c(ws);
     FwdLayout L{};
     const Lanes lanes = lanes_of<true>(E);
-    L.vectors = lanes.r;
+    L.lanes = lanes;
     L.threads = routing::fwd_block(lanes.r);
     L.rows = L.threads / lanes.g;
     L.nchunks = routing::chunks_of(B, N, L.rows, 512);
@@ -93,8 +94,7 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     const bool select = a->given == nullptr;
     if (select && a->k > a->E) return fail(DOT_ERR_INVALID_ARG, "k must be at most E");
     if (a->B == 0) return ok();
-    if (!a->counts || !a->tokens || !a->loss)
-        return fail(DOT_ERR_INVALID_ARG, "counts, tokens and loss must be non-NULL");
+    if (!a->counts || !a->loss) return fail(DOT_ERR_INVALID_ARG, "counts and loss must be non-NULL");
     if (a->N > 0 && (!a->scores || (select && (!a->weights || !a->experts))))
         return fail(DOT_ERR_INVALID_ARG, "scores, weights and experts must be non-NULL");
     const FwdLayout L = fwd_layout(a->workspace, a->B, a->N, a->E);
@@ -126,7 +126,7 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     x.tokens = a->tokens;
     x.loss = a->loss;
     const dim3 grid = batch_grid(unsigned(L.nchunks), a->B);
-    const size_t lds = routing::fwd_lds_bytes(a->E, a->k, L.vectors, L.rows, select);
+    const size_t lds = routing::fwd_lds_bytes(a->E, a->k, L.lanes.g, L.lanes.r, L.rows, select);
     dispatch<true>(a->dtype, a->E, rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype), [&](auto t, auto s) {
         ProfScope prof("routing_forward", stream);
         if (select)
@@ -152,8 +152,8 @@ extern "C" int dot_routing_backward(const dot_routing_bwd_args* a, dot_stream_t 
     if (int rc = check_shape(a->dtype, a->B, a->N, a->E, a->k, a->scoring)) return rc;
     if (a->B == 0 || a->N == 0) return ok();
     if (!a->scores || !a->grad_scores) return fail(DOT_ERR_INVALID_ARG, "scores and grad_scores must be non-NULL");
-    if (a->grad_loss && (!a->counts || !a->tokens))
-        return fail(DOT_ERR_INVALID_ARG, "grad_loss needs counts and tokens");
+    if (a->grad_loss && (!a->counts || (a->mask && !a->tokens)))
+        return fail(DOT_ERR_INVALID_ARG, "grad_loss needs counts, and tokens where there is a mask");
     if (a->grad_weights && (!a->weights || !a->experts))
         return fail(DOT_ERR_INVALID_ARG, "grad_weights needs weights and experts");
     routing::BwdArgs x{};

@@ -34,9 +34,12 @@ dot_stream_t stream_of(const Tensor& t) {
     return reinterpret_cast<dot_stream_t>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
 }
 
+// Scratch of a call, none where it needs none (an allocation takes the host
+// over a microsecond).
 Tensor workspace(size_t bytes, const Tensor& like) {
-    return at::empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, like.options().dtype(at::kByte));
+    return bytes ? at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte)) : Tensor();
 }
+void* ptr_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 int dtype_tag(const Tensor& t, const char* name) {
     switch (t.scalar_type()) {
@@ -100,7 +103,8 @@ void check_rows(const Tensor& x, const char* name) {
     TORCH_CHECK(x.dim() == 3, name, " must be 3D");
 }
 
-// -> [weights, experts, counts, tokens, loss]; weights and experts are empty for given experts
+// -> [counts, loss], then [weights, experts] where the call selects, then [tokens]
+// where there is a mask (all N without one)
 std::vector<Tensor> routing_forward_op(Tensor scores_, int64_t k, int64_t scoring, bool normalize,
                                        optional<Tensor> bias_, optional<Tensor> mask_, optional<Tensor> given_) {
     check_rows(scores_, "scores");
@@ -118,9 +122,12 @@ std::vector<Tensor> routing_forward_op(Tensor scores_, int64_t k, int64_t scorin
     }
     const auto f32 = scores.options().dtype(at::kFloat), i32 = scores.options().dtype(at::kInt);
     const bool select = !given.defined();
-    Tensor weights = at::empty(select ? at::IntArrayRef({B, N, k}) : at::IntArrayRef({0}), f32);
-    Tensor experts = at::empty(select ? at::IntArrayRef({B, N, k}) : at::IntArrayRef({0}), i32);
-    Tensor counts = at::empty({B, E}, i32), tokens = at::empty({B}, i32), loss = at::empty({B}, f32);
+    std::vector<Tensor> out{at::empty({B, E}, i32), at::empty({B}, f32)};
+    if (select) {
+        out.push_back(at::empty({B, N, k}, f32));
+        out.push_back(at::empty({B, N, k}, i32));
+    }
+    if (mask.defined()) out.push_back(at::empty({B}, i32));
     dot_routing_fwd_args a{};
     a.dtype = dtype_tag(scores, "scores");
     a.B = to_int(B, "B");
@@ -135,33 +142,37 @@ std::vector<Tensor> routing_forward_op(Tensor scores_, int64_t k, int64_t scorin
     a.bias = floats(bias);
     a.mask = mask_ptr(mask);
     // an empty batch has no entries to point at: any address says "given"
-    a.given = select ? nullptr : given.numel() ? given.const_data_ptr() : counts.const_data_ptr();
+    a.given = select ? nullptr : given.numel() ? given.const_data_ptr() : out[0].const_data_ptr();
     a.given_is_int64 = !select && given.scalar_type() == at::kLong;
-    a.weights = select ? weights.data_ptr<float>() : nullptr;
-    a.experts = select ? experts.data_ptr<int32_t>() : nullptr;
-    a.counts = counts.data_ptr<int32_t>();
-    a.tokens = tokens.data_ptr<int32_t>();
-    a.loss = loss.data_ptr<float>();
+    a.counts = out[0].data_ptr<int32_t>();
+    a.loss = out[1].data_ptr<float>();
+    a.weights = select ? out[2].data_ptr<float>() : nullptr;
+    a.experts = select ? out[3].data_ptr<int32_t>() : nullptr;
+    a.tokens = mask.defined() ? out.back().data_ptr<int32_t>() : nullptr;
     a.workspace_bytes = dot_routing_forward_workspace_bytes(a.B, a.N, a.E);
-    Tensor ws = workspace(a.workspace_bytes, scores);
-    a.workspace = ws.data_ptr();
+    const Tensor ws = workspace(a.workspace_bytes, scores);
+    a.workspace = ptr_of(ws);
     check_rc(dot_routing_forward(&a, stream_of(scores)), "dot_routing_forward");
-    return {weights, experts, counts, tokens, loss};
+    return out;
 }
 
 Tensor routing_backward_op(Tensor scores_, int64_t k, int64_t scoring, bool normalize, optional<Tensor> mask_,
-                           Tensor counts, Tensor tokens, optional<Tensor> grad_loss_, optional<Tensor> weights,
-                           optional<Tensor> experts, optional<Tensor> grad_weights_) {
+                           Tensor counts, optional<Tensor> tokens, optional<Tensor> grad_loss_,
+                           optional<Tensor> weights, optional<Tensor> experts, optional<Tensor> grad_weights_) {
     check_rows(scores_, "scores");
     c10::OptionalDeviceGuard guard(scores_.device());
     const Tensor scores = unit_rows(scores_);
     const int64_t B = scores.size(0), N = scores.size(1), E = scores.size(2);
     const Tensor mask = mask_of(mask_, scores);
     check_on(counts, scores, "counts");
-    check_on(tokens, scores, "tokens");
-    TORCH_CHECK(counts.scalar_type() == at::kInt && counts.is_contiguous() && counts.numel() == B * E &&
-                    tokens.scalar_type() == at::kInt && tokens.is_contiguous() && tokens.numel() == B,
-                "counts and tokens must be as the forward returned them");
+    TORCH_CHECK(counts.scalar_type() == at::kInt && counts.is_contiguous() && counts.numel() == B * E,
+                "counts must be as the forward returned them");
+    TORCH_CHECK(tokens.has_value() == mask.defined(), "tokens come with a mask");
+    if (tokens.has_value()) {
+        check_on(*tokens, scores, "tokens");
+        TORCH_CHECK(tokens->scalar_type() == at::kInt && tokens->is_contiguous() && tokens->numel() == B,
+                    "tokens must be as the forward returned them");
+    }
     Tensor grad = at::empty({B, N, E}, scores.options().memory_format(at::MemoryFormat::Contiguous));
     dot_routing_bwd_args a{};
     Tensor gl, gw, w, e;
@@ -190,7 +201,7 @@ Tensor routing_backward_op(Tensor scores_, int64_t k, int64_t scoring, bool norm
     a.normalize = normalize;
     a.mask = mask_ptr(mask);
     a.counts = counts.const_data_ptr<int32_t>();
-    a.tokens = tokens.const_data_ptr<int32_t>();
+    a.tokens = tokens.has_value() ? tokens->const_data_ptr<int32_t>() : nullptr;
     a.grad_loss = floats(gl);
     a.weights = floats(w);
     a.experts = e.defined() ? e.const_data_ptr<int32_t>() : nullptr;
@@ -223,7 +234,8 @@ Tensor tokens_of(const Tensor& tokens, const Tensor& logits) {
     return t;
 }
 
-// -> [out, row_stats [B, S, 2], weight [B]]
+// -> [out], with keep [out, saved]: the row statistics [B, S, 2] and the sequences'
+// weights [B] that the backward takes, one after the other
 std::vector<Tensor> sequence_logp_forward_op(Tensor logits_, Tensor tokens_, optional<Tensor> ref_,
                                              optional<Tensor> mask_, double tau, int64_t reduction, bool keep) {
     check_rows(logits_, "logits");
@@ -240,41 +252,40 @@ std::vector<Tensor> sequence_logp_forward_op(Tensor logits_, Tensor tokens_, opt
     }
     const auto f32 = logits.options().dtype(at::kFloat);
     Tensor out = at::empty(reduction == DOT_REDUCE_NONE ? at::IntArrayRef({B, S}) : at::IntArrayRef({B}), f32);
-    Tensor stats = at::empty(keep ? at::IntArrayRef({B, S, 2}) : at::IntArrayRef({0}), f32);
-    Tensor weight = at::empty({keep ? B : 0}, f32);
+    const Tensor saved = keep ? at::empty({(2 * S + 1) * B}, f32) : Tensor();
     dot_seqlogp_fwd_args a{};
     fill_rows(a, logits, tokens, mask, tau, reduction);
     a.ref = ref.defined() ? ref.const_data_ptr() : nullptr;
     a.ref_is_f64 = ref.defined() && ref.scalar_type() == at::kDouble;
     a.ref_per_token = ref.defined() && ref.dim() == 2;
     a.out = out.data_ptr<float>();
-    a.row_stats = keep ? stats.data_ptr<float>() : nullptr;
-    a.weight = keep ? weight.data_ptr<float>() : nullptr;
+    a.row_stats = keep ? saved.data_ptr<float>() : nullptr;
+    a.weight = keep ? saved.data_ptr<float>() + 2 * B * S : nullptr;
     a.workspace_bytes = dot_seqlogp_forward_workspace_bytes(a.B, a.S, a.V, a.dtype);
-    Tensor ws = workspace(a.workspace_bytes, logits);
-    a.workspace = ws.data_ptr();
+    const Tensor ws = workspace(a.workspace_bytes, logits);
+    a.workspace = ptr_of(ws);
     check_rc(dot_seqlogp_forward(&a, stream_of(logits)), "dot_seqlogp_forward");
-    return {out, stats, weight};
+    if (!keep) return {out};
+    return {out, saved};
 }
 
 Tensor sequence_logp_backward_op(Tensor logits_, Tensor tokens_, optional<Tensor> mask_, double tau,
-                                 int64_t reduction, Tensor stats, Tensor weight, Tensor grad_out_) {
+                                 int64_t reduction, Tensor saved, Tensor grad_out_) {
     check_rows(logits_, "logits");
     c10::OptionalDeviceGuard guard(logits_.device());
     const Tensor logits = unit_rows(logits_);
     const int64_t B = logits.size(0), S = logits.size(1), V = logits.size(2);
     const Tensor tokens = tokens_of(tokens_, logits), mask = mask_of(mask_, logits);
-    stats = f32c(stats, logits, "row_stats");
-    weight = f32c(weight, logits, "weight");
-    TORCH_CHECK(stats.numel() == B * S * 2 && weight.numel() == B,
-                "row_stats and weight must be as the forward returned them");
+    check_on(saved, logits, "saved");
+    TORCH_CHECK(saved.scalar_type() == at::kFloat && saved.is_contiguous() && saved.numel() == (2 * S + 1) * B,
+                "saved must be as the forward returned it");
     TORCH_CHECK(grad_out_.numel() == (reduction == DOT_REDUCE_NONE ? B * S : B), "grad_out has the wrong size");
     Tensor grad = at::empty({B, S, V}, logits.options().memory_format(at::MemoryFormat::Contiguous));
     dot_seqlogp_bwd_args a{};
     fill_rows(a, logits, tokens, mask, tau, reduction);
     const Tensor go = upstream(grad_out_, logits, a.grad_out_scalar);
-    a.row_stats = floats(stats);
-    a.weight = floats(weight);
+    a.row_stats = saved.const_data_ptr<float>();
+    a.weight = a.row_stats + 2 * B * S;
     a.grad_out = floats(go);
     a.grad_logits = grad.data_ptr();
     check_rc(dot_seqlogp_backward(&a, stream_of(logits)), "dot_seqlogp_backward");
@@ -330,11 +341,8 @@ std::vector<Tensor> preference_backward_op(Tensor ratio_, optional<Tensor> plan_
     a.grad_ratio = grad_ratio.data_ptr<float>();
     a.grad_plan = grad_plan.numel() ? grad_plan.data_ptr<float>() : nullptr;
     a.workspace_bytes = dot_preference_backward_workspace_bytes(a.P, a.Q, plan.defined());
-    Tensor ws;
-    if (a.workspace_bytes) {
-        ws = workspace(a.workspace_bytes, ratio);
-        a.workspace = ws.data_ptr();
-    }
+    const Tensor ws = workspace(a.workspace_bytes, ratio);
+    a.workspace = ptr_of(ws);
     check_rc(dot_preference_backward(&a, stream_of(ratio)), "dot_preference_backward");
     return {grad_ratio, grad_plan};
 }
@@ -378,25 +386,27 @@ struct RoutingFunction : torch::autograd::Function<RoutingFunction> {
                                  bool normalize, const optional<Tensor>& bias, const optional<Tensor>& mask,
                                  const optional<Tensor>& given) {
         std::vector<Tensor> o = call_routing(scores, k, scoring, normalize, bias, mask, given);
-        const bool select = !given.has_value();
-        ctx->save_for_backward({scores, mask.value_or(Tensor()), o[2], o[3], select ? o[0] : Tensor(),
-                                select ? o[1] : Tensor()});
-        ctx->saved_data["k"] = k;
-        ctx->saved_data["scoring"] = scoring;
-        ctx->saved_data["normalize"] = normalize;
-        ctx->mark_non_differentiable(select ? variable_list{o[1], o[2], o[3]} : variable_list{o[0], o[1], o[2], o[3]});
+        const bool select = !given.has_value(), masked = mask.has_value();
+        ctx->save_for_backward({scores, mask.value_or(Tensor()), o[0], masked ? o.back() : Tensor(),
+                                select ? o[2] : Tensor(), select ? o[3] : Tensor()});
+        ctx->saved_data["args"] = k * 8 + scoring * 2 + normalize;
+        variable_list counts{o[0]};
+        if (select) counts.push_back(o[3]);
+        if (masked) counts.push_back(o.back());
+        ctx->mark_non_differentiable(counts);
         ctx->set_materialize_grads(false);
         return o;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         const variable_list s = ctx->get_saved_variables();
-        const Tensor gw = s[4].defined() ? grads[0] : Tensor(), gl = grads[4];
+        const bool select = s[4].defined();
+        const Tensor gw = select ? grads[2] : Tensor(), gl = grads[1];
+        const int64_t args = ctx->saved_data["args"].toInt();
         Tensor g;
         if (gw.defined() || gl.defined()) {
             static const auto op = op_handle<decltype(routing_backward_op)>("dot_amd::routing_backward");
             at::AutoDispatchBelowADInplaceOrView below;
-            g = op.call(s[0], ctx->saved_data["k"].toInt(), ctx->saved_data["scoring"].toInt(),
-                        ctx->saved_data["normalize"].toBool(), maybe(s[1]), s[2], s[3], maybe(gl),
+            g = op.call(s[0], args / 8, args / 2 % 4, args % 2, maybe(s[1]), s[2], maybe(s[3]), maybe(gl),
                         gw.defined() ? maybe(s[4]) : c10::nullopt, gw.defined() ? maybe(s[5]) : c10::nullopt,
                         maybe(gw));
         }
@@ -422,10 +432,10 @@ struct SequenceLogpFunction : torch::autograd::Function<SequenceLogpFunction> {
                                  const optional<Tensor>& ref, const optional<Tensor>& mask, double tau,
                                  int64_t reduction) {
         std::vector<Tensor> o = call_sequence_logp(logits, tokens, ref, mask, tau, reduction, true);
-        ctx->save_for_backward({logits, tokens, mask.value_or(Tensor()), o[1], o[2]});
+        ctx->save_for_backward({logits, tokens, mask.value_or(Tensor()), o[1]});
         ctx->saved_data["tau"] = tau;
         ctx->saved_data["reduction"] = reduction;
-        ctx->mark_non_differentiable({o[1], o[2]});
+        ctx->mark_non_differentiable({o[1]});
         ctx->set_materialize_grads(false);
         return o;
     }
@@ -436,7 +446,7 @@ struct SequenceLogpFunction : torch::autograd::Function<SequenceLogpFunction> {
             static const auto op = op_handle<decltype(sequence_logp_backward_op)>("dot_amd::sequence_logp_backward");
             at::AutoDispatchBelowADInplaceOrView below;
             g = op.call(s[0], s[1], maybe(s[2]), ctx->saved_data["tau"].toDouble(),
-                        ctx->saved_data["reduction"].toInt(), s[3], s[4], grads[0]);
+                        ctx->saved_data["reduction"].toInt(), s[3], grads[0]);
         }
         return {once(g), {}, {}, {}, {}, {}};
     }
@@ -491,9 +501,9 @@ Tensor preference_forward_autograd(Tensor ratio, optional<Tensor> plan, int64_t 
 
 TORCH_LIBRARY_FRAGMENT(dot_amd, m) {
     m.def("routing_forward(Tensor scores, int k, int scoring, bool normalize, Tensor? bias, Tensor? mask, Tensor? given) -> Tensor[]");
-    m.def("routing_backward(Tensor scores, int k, int scoring, bool normalize, Tensor? mask, Tensor counts, Tensor tokens, Tensor? grad_loss, Tensor? weights, Tensor? experts, Tensor? grad_weights) -> Tensor");
+    m.def("routing_backward(Tensor scores, int k, int scoring, bool normalize, Tensor? mask, Tensor counts, Tensor? tokens, Tensor? grad_loss, Tensor? weights, Tensor? experts, Tensor? grad_weights) -> Tensor");
     m.def("sequence_logp_forward(Tensor logits, Tensor tokens, Tensor? ref, Tensor? mask, float tau, int reduction, bool keep) -> Tensor[]");
-    m.def("sequence_logp_backward(Tensor logits, Tensor tokens, Tensor? mask, float tau, int reduction, Tensor row_stats, Tensor weight, Tensor grad_out) -> Tensor");
+    m.def("sequence_logp_backward(Tensor logits, Tensor tokens, Tensor? mask, float tau, int reduction, Tensor saved, Tensor grad_out) -> Tensor");
     m.def("preference_forward(Tensor log_ratio, Tensor? plan, int loss_type, float beta, float smoothing) -> Tensor");
     m.def("preference_backward(Tensor log_ratio, Tensor? plan, int loss_type, float beta, float smoothing, Tensor grad_loss, bool want_plan) -> Tensor[]");
 }

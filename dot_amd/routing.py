@@ -109,13 +109,13 @@ def topk_routing(
         if bias.shape != scores.shape[-1:] or not bias.is_floating_point():
             raise ValueError(f"bias must be floating point of shape ({scores.size(-1)},), got {tuple(bias.shape)}")
         bias = bias.detach()
-    if scores.dim() == 3:
-        weights, experts, counts, _, loss = _ops.fused.routing_forward(scores, k, _SCORING[scoring], normalize, bias,
-                                                                       mask, None)
-        return RoutingResult(weights, experts, counts, loss)
-    out = _ops.fused.routing_forward(scores.unsqueeze(0), k, _SCORING[scoring], normalize, bias,
-                                     None if mask is None else mask.unsqueeze(0), None)
-    weights, experts, counts, _, loss = (x.squeeze(0) for x in out)
+    batched = scores.dim() == 3
+    if not batched:
+        scores, mask = scores.unsqueeze(0), None if mask is None else mask.unsqueeze(0)
+    counts, loss, weights, experts = _ops.fused.routing_forward(scores, k, _SCORING[scoring], normalize, bias, mask,
+                                                                None)[:4]
+    if not batched:
+        weights, experts, counts, loss = (x.squeeze(0) for x in (weights, experts, counts, loss))
     return RoutingResult(weights, experts, counts, loss)
 
 
@@ -150,8 +150,8 @@ def balance_loss(
     if not batched:
         scores, experts = scores.unsqueeze(0), experts.unsqueeze(0)
         mask = None if mask is None else mask.unsqueeze(0)
-    _, _, counts, _, loss = _ops.fused.routing_forward(scores, experts.size(-1), _SCORING[scoring], False, None, mask,
-                                                       experts)
+    counts, loss = _ops.fused.routing_forward(scores, experts.size(-1), _SCORING[scoring], False, None, mask,
+                                              experts)[:2]
     return BalanceResult(loss, counts) if batched else BalanceResult(loss.squeeze(0), counts.squeeze(0))
 
 

@@ -395,7 +395,7 @@ typedef struct {
     float* weights;            /* [B,N,k] out when the call selects */
     int32_t* experts;          /* [B,N,k] out when the call selects; -1 in slots without an expert */
     int32_t* counts;           /* [B,E] out: slots of the unmasked tokens that name e */
-    int32_t* tokens;           /* [B] out: unmasked tokens n_b */
+    int32_t* tokens;           /* [B] out: unmasked tokens n_b, or NULL */
     float* loss;               /* [B] out: E sum_e counts_e / (k n_b) * sum_n p_ne / n_b, with p = q / sum q;
                                   0 where n_b = 0 */
     void* workspace;
@@ -418,8 +418,8 @@ typedef struct {
     int scoring;
     int normalize;
     const uint8_t* mask;
-    const int32_t* counts;     /* [B,E] and [B], as the forward wrote them */
-    const int32_t* tokens;
+    const int32_t* counts;     /* [B,E], as the forward wrote it */
+    const int32_t* tokens;     /* [B], as the forward wrote it; NULL: all N */
     const float* grad_loss;    /* [B] (one value with grad_loss_scalar), or NULL */
     int grad_loss_scalar;
     const float* weights;      /* [B,N,k] as the forward wrote them, with grad_weights */

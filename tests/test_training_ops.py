@@ -286,6 +286,7 @@ def test_c_abi_refusals(lib):
     f = "dot_routing_backward"
     refused(lib, f, INVALID, "non-NULL", RoutingBwd(**{**b, "grad_scores": None}))
     refused(lib, f, INVALID, "counts", RoutingBwd(**{**b, "counts": None}))
+    refused(lib, f, INVALID, "tokens", RoutingBwd(**{**b, "tokens": None, "mask": some}))
     refused(lib, f, INVALID, "weights", RoutingBwd(**{**b, "grad_weights": some}))
 
     s = dict(logits=some, B=2, S=3, V=16, tokens=some, tau=1.0, reduction=1, out=some)
