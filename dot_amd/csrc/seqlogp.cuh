@@ -115,14 +115,47 @@ struct Part {
     float m;
 };
 
-// Partial statistics of every row: one for each split.
+struct JoinArgs {
+    const void* ref;
+    int ref64, ref_per_token;
+    int reduction;
+    float* out;
+    float2* stats;
+    float* weight;
+};
+
+__device__ __forceinline__ double float_at(const void* p, int is64, int64_t i) {
+    return is64 ? static_cast<const double*>(p)[i] : double(static_cast<const float*>(p)[i]);
+}
+
+// The value of a position from its row's statistics, which are kept for the
+// backward.
 template <class T>
-__global__ __launch_bounds__(kBlock) void row_stats(Rows r, Part* parts) {
+__device__ __forceinline__ double position(const Rows& r, const JoinArgs& j, int64_t at, int tok, const MaxSum& t) {
+    const float x = to_float(row_of<T>(r, at)[tok]);
+    if (j.stats) j.stats[at] = make_float2(t.base(), float(1.0 / t.s));
+    double v = (double(x) - double(t.base())) * ((double(r.k) + double(r.klo)) * 0.693147180559945309417) - log(t.s);
+    if (j.ref && j.ref_per_token) v -= float_at(j.ref, j.ref64, at);
+    return v;
+}
+
+// Partial statistics of every row, one for each split; a row that is not split
+// gets its position's value at once (in the place of s, or in the output).
+template <class T>
+__global__ __launch_bounds__(kBlock) void row_stats(Rows r, JoinArgs j, Part* parts) {
     __shared__ float sm[kWavesPerBlock];
     __shared__ double ss[kWavesPerBlock];
     const int64_t at = blockIdx.x / unsigned(r.splits);
     const int part = int(blockIdx.x % unsigned(r.splits));
-    if (token_of(r, at) < 0) return;
+    const int tok = token_of(r, at);
+    auto put = [&](double v) {
+        if (j.reduction == DOT_REDUCE_NONE) j.out[at] = float(v);
+        else parts[at].s = v;
+    };
+    if (tok < 0) {
+        if (r.splits == 1 && threadIdx.x == 0) put(0.0);
+        return;
+    }
     const T* row = row_of<T>(r, at);
     const Span sp = span_of(row, r.V, part, r.splits);
     const T* body = row + sp.head;
@@ -166,25 +199,13 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Part* parts) {
     if (threadIdx.x == 0) {
         MaxSum t;
         for (int w = 0; w < kWavesPerBlock; ++w) t.join(sm[w], ss[w], r);
-        parts[blockIdx.x] = Part{t.s, t.m};
+        if (r.splits == 1) put(position<T>(r, j, at, tok, t));
+        else parts[blockIdx.x] = Part{t.s, t.m};
     }
 }
 
-struct JoinArgs {
-    const void* ref;
-    int ref64, ref_per_token;
-    int reduction;
-    float* out;
-    float2* stats;
-    float* weight;
-};
-
-__device__ __forceinline__ double float_at(const void* p, int is64, int64_t i) {
-    return is64 ? static_cast<const double*>(p)[i] : double(static_cast<const float*>(p)[i]);
-}
-
-// One workgroup per sequence: joins the parts of its rows, forms the values of
-// its positions and their sum.
+// One workgroup per sequence: joins the parts of its split rows, and adds up the
+// values of its positions.
 template <class T>
 __global__ __launch_bounds__(kJoinBlock) void join(Rows r, const Part* parts, JoinArgs j) {
     __shared__ double wsum[kJoinBlock / kWave];
@@ -195,21 +216,22 @@ __global__ __launch_bounds__(kJoinBlock) void join(Rows r, const Part* parts, Jo
     int count = 0;
     for (int s = threadIdx.x; s < r.S; s += kJoinBlock) {
         const int64_t at = int64_t(b) * r.S + s;
-        const int tok = token_of(r, at);
+        const bool whole = r.splits == 1;
+        // positions are counted for the mean; an unsplit row has its value already
+        const int tok = !whole || j.reduction == DOT_REDUCE_MEAN ? token_of(r, at) : -1;
         double v = 0.0;
-        if (tok >= 0) {
+        if (whole) {
+            v = parts[at].s;
+        } else if (tok >= 0) {
             MaxSum t;
             for (int i = 0; i < r.splits; ++i) {
                 const Part p = parts[at * r.splits + i];
                 t.join(p.m, p.s, r);
             }
-            const float x = to_float(row_of<T>(r, at)[tok]);
-            if (j.stats) j.stats[at] = make_float2(t.base(), float(1.0 / t.s));
-            v = (double(x) - double(t.base())) * ((double(r.k) + double(r.klo)) * 0.693147180559945309417) - log(t.s);
-            if (j.ref && j.ref_per_token) v -= float_at(j.ref, j.ref64, at);
-            sum += v;
-            ++count;
+            v = position<T>(r, j, at, tok, t);
         }
+        sum += v;
+        count += tok >= 0;
         if (j.reduction == DOT_REDUCE_NONE) j.out[at] = float(v);
     }
 #pragma unroll
@@ -230,7 +252,7 @@ __global__ __launch_bounds__(kJoinBlock) void join(Rows r, const Part* parts, Jo
             n += wcount[w];
         }
         const double weight = j.reduction == DOT_REDUCE_MEAN ? 1.0 / (n > 0 ? n : 1) : 1.0;
-        if (j.weight) j.weight[b] = float(weight);
+        if (j.reduction == DOT_REDUCE_MEAN && j.weight) j.weight[b] = float(weight);
         if (j.reduction != DOT_REDUCE_NONE) {
             t *= weight;
             if (j.ref && !j.ref_per_token) t -= float_at(j.ref, j.ref64, b);
@@ -270,7 +292,7 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     const int64_t b = at / r.S;
     const float2 st = g.stats[at];
     const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
-    const float c = up * g.weight[b] * g.inv_tau;
+    const float c = (g.reduction == DOT_REDUCE_MEAN ? up * g.weight[b] : up) * g.inv_tau;
     const float scale = -c * st.y;
     auto value = [&](float x, int v) {
         const float y = __builtin_amdgcn_exp2f(scaled(r, x - st.x)) * scale;

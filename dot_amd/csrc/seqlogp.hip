@@ -91,9 +91,11 @@ extern "C" int dot_seqlogp_forward(const dot_seqlogp_fwd_args* a, dot_stream_t s
         using T = decltype(t);
         if (rows > 0) {
             ProfScope prof("seqlogp_row_stats", stream);
-            hipLaunchKernelGGL((seqlogp::row_stats<T>), dim3(unsigned(rows * r.splits)), dim3(kBlock), 0, stream, r,
+            hipLaunchKernelGGL((seqlogp::row_stats<T>), dim3(unsigned(rows * r.splits)), dim3(kBlock), 0, stream, r, j,
                                parts);
         }
+        // unsplit rows write their positions' values themselves
+        if (a->reduction == DOT_REDUCE_NONE && r.splits == 1) return;
         ProfScope prof("seqlogp_join", stream);
         hipLaunchKernelGGL((seqlogp::join<T>), batch_grid(1, a->B), dim3(seqlogp::kJoinBlock), 0, stream, r, parts, j);
     });
@@ -106,8 +108,10 @@ extern "C" int dot_seqlogp_backward(const dot_seqlogp_bwd_args* a, dot_stream_t 
     if (int rc = check_shape(a->dtype, a->B, a->S, a->V, a->tau, a->reduction)) return rc;
     const int64_t rows = int64_t(a->B) * a->S;
     if (rows == 0) return ok();
-    if (!a->logits || !a->tokens || !a->row_stats || !a->weight || !a->grad_out || !a->grad_logits)
-        return fail(DOT_ERR_INVALID_ARG, "logits, tokens, row_stats, weight, grad_out and grad_logits must be non-NULL");
+    if (!a->logits || !a->tokens || !a->row_stats || !a->grad_out || !a->grad_logits)
+        return fail(DOT_ERR_INVALID_ARG, "logits, tokens, row_stats, grad_out and grad_logits must be non-NULL");
+    if (a->reduction == DOT_REDUCE_MEAN && !a->weight)
+        return fail(DOT_ERR_INVALID_ARG, "the gradient of a mean needs weight");
     const seqlogp::Rows r = rows_of(a);
     seqlogp::GradArgs g{};
     g.inv_tau = 1.0f / a->tau;

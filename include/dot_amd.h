@@ -452,7 +452,7 @@ typedef struct {
     float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
     float* row_stats;          /* [B,S,2] out, for the backward: the row's max and
                                   1 / sum exp((x - max) / tau); not written where left out */
-    float* weight;             /* [B] out, for the backward: 1, or 1 / positions with DOT_REDUCE_MEAN */
+    float* weight;             /* [B] out with DOT_REDUCE_MEAN, for the backward: 1 / positions */
     void* workspace;
     size_t workspace_bytes;
 } dot_seqlogp_fwd_args;
@@ -473,7 +473,7 @@ typedef struct {
     float tau;
     int reduction;
     const float* row_stats;
-    const float* weight;
+    const float* weight;       /* with DOT_REDUCE_MEAN */
     const float* grad_out;     /* [B], or [B,S] with DOT_REDUCE_NONE; one value with grad_out_scalar */
     int grad_out_scalar;
     void* grad_logits;         /* [B,S,V] out, contiguous, of type dtype; 0 where left out */
