@@ -53,6 +53,12 @@ __device__ __forceinline__ Pack<T> load_pack(const T* p) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(Pack<T>, *reinterpret_cast<const u4*>(p));
 }
+// As load_pack, for inputs that nothing reads again soon.
+template <class T>
+__device__ __forceinline__ Pack<T> load_pack_stream(const T* p) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(Pack<T>, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
+}
 template <class T>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T>& x) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));

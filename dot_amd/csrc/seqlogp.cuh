@@ -20,7 +20,8 @@
 namespace dot_amd {
 namespace seqlogp {
 
-constexpr int kUnroll = 4;       // packs of a thread in flight
+constexpr int kReadUnroll = 8;   // packs of a thread in flight: where a row is only read,
+constexpr int kUnroll = 4;       // and where it is written as well
 constexpr int kJoinBlock = 1024; // threads of the per-sequence kernel
 
 struct Rows {
@@ -35,6 +36,10 @@ struct Rows {
     // typical rows, 1e-4 over a thousand positions.
     float k, klo;
     int splits;  // workgroups per row
+    // Rows from here on are read through the caches and may stay in the last
+    // level for the backward, which takes the rows in the other order; those
+    // before are read past the caches.
+    int64_t cached;
 };
 
 // d log2(e) / tau of a difference d <= 0 (-inf stays -inf: klo is not 0).
@@ -72,6 +77,13 @@ __device__ __forceinline__ Span span_of(const T* row, int V, int part, int parts
     s.p0 = min(part * per, packs);
     s.p1 = min(s.p0 + per, packs);
     return s;
+}
+
+// A pack of logits, through the caches or (STREAM) past them.
+template <bool STREAM, class T>
+__device__ __forceinline__ Pack<T> row_pack(const T* p) {
+    if constexpr (STREAM) return load_pack_stream(p);
+    else return load_pack(p);
 }
 
 // Sum of N values, pairwise.
@@ -161,23 +173,28 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, JoinArgs j, Part* pa
     const T* body = row + sp.head;
     constexpr int PN = Pack<T>::N;
     MaxSum a;
-    int p = sp.p0 + int(threadIdx.x);
-    for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
-        Pack<T> x[kUnroll];
-        float f[kUnroll * PN];
+    auto packs = [&](auto stream) {
+        constexpr bool STREAM = decltype(stream)::value;
+        int p = sp.p0 + int(threadIdx.x);
+        for (; p + (kReadUnroll - 1) * kBlock < sp.p1; p += kReadUnroll * kBlock) {
+            Pack<T> x[kReadUnroll];
+            float f[kReadUnroll * PN];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) x[u] = load_pack(body + int64_t(p + u * kBlock) * PN);
+            for (int u = 0; u < kReadUnroll; ++u) x[u] = row_pack<STREAM>(body + int64_t(p + u * kBlock) * PN);
 #pragma unroll
-        for (int i = 0; i < kUnroll * PN; ++i) f[i] = to_float(x[i / PN].v[i % PN]);
-        a.add<PN>(f, r);
-    }
-    for (; p < sp.p1; p += kBlock) {
-        const Pack<T> x = load_pack(body + int64_t(p) * PN);
-        float f[PN];
+            for (int i = 0; i < kReadUnroll * PN; ++i) f[i] = to_float(x[i / PN].v[i % PN]);
+            a.add<PN>(f, r);
+        }
+        for (; p < sp.p1; p += kBlock) {
+            const Pack<T> x = row_pack<STREAM>(body + int64_t(p) * PN);
+            float f[PN];
 #pragma unroll
-        for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
-        a.add<PN>(f, r);
-    }
+            for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
+            a.add<PN>(f, r);
+        }
+    };
+    if (at < r.cached) packs(std::true_type{});
+    else packs(std::false_type{});
     if (part == 0 && int(threadIdx.x) < sp.head) {
         const float f[1] = {to_float(row[threadIdx.x])};
         a.add<1>(f, r);
@@ -274,7 +291,8 @@ struct GradArgs {
 // dx of one span of a row.
 template <class T>
 __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
-    const int64_t at = blockIdx.x / unsigned(r.splits);
+    // last rows first: the forward has just read them
+    const int64_t at = int64_t(r.B) * r.S - 1 - blockIdx.x / unsigned(r.splits);
     const int part = int(blockIdx.x % unsigned(r.splits));
     constexpr int PN = Pack<T>::N;
     const int tok = token_of(r, at);
@@ -300,9 +318,9 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     };
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     const Span sp = span_of(out, r.V, part, r.splits);
-    auto pack_in = [&](int p) {
+    auto pack_in = [&](int p, auto stream) {
         const T* at_p = row + sp.head + int64_t(p) * PN;
-        if (together) return load_pack(at_p);
+        if (together) return row_pack<decltype(stream)::value>(at_p);
         Pack<T> x;  // a strided view whose rows are not aligned as the gradient's
 #pragma unroll
         for (int i = 0; i < PN; ++i) x.v[i] = at_p[i];
@@ -315,15 +333,19 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
         for (int i = 0; i < PN; ++i) y.v[i] = from_float<T>(value(to_float(x.v[i]), v0 + i));
         store_pack_stream(out + v0, y);
     };
-    int p = sp.p0 + int(threadIdx.x);
-    for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
-        Pack<T> x[kUnroll];
+    auto packs = [&](auto stream) {
+        int p = sp.p0 + int(threadIdx.x);
+        for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
+            Pack<T> x[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) x[u] = pack_in(p + u * kBlock);
+            for (int u = 0; u < kUnroll; ++u) x[u] = pack_in(p + u * kBlock, stream);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) pack_out(p + u * kBlock, x[u]);
-    }
-    for (; p < sp.p1; p += kBlock) pack_out(p, pack_in(p));
+            for (int u = 0; u < kUnroll; ++u) pack_out(p + u * kBlock, x[u]);
+        }
+        for (; p < sp.p1; p += kBlock) pack_out(p, pack_in(p, stream));
+    };
+    if (at < r.cached) packs(std::true_type{});
+    else packs(std::false_type{});
     if (part == 0 && int(threadIdx.x) < sp.head)
         out[threadIdx.x] = from_float<T>(value(to_float(row[threadIdx.x]), int(threadIdx.x)));
     const int v = sp.tail + int(threadIdx.x);
