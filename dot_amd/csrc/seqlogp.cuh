@@ -2,9 +2,10 @@
 // the gradient of the logits.
 //
 // The forward reads each row once with a running maximum m and sum
-// s = sum_v 2^((x_v - m) k), k = log2(e) / tau.  Terms are added pairwise within
-// a pack, and those sums in 64 bits: next to a likely token's 1, terms
-// of 1e-7 each would be lost one by one in 32.  A row may be split over several
+// s = sum_v 2^((x_v - m) k), k = log2(e) / tau, over the vocabulary without the
+// position's own token, which is added in 64 bits: next to a likely token's 1
+// the others' terms of 1e-7 each would lose their digits.  Terms are added
+// pairwise within a pack, and those sums in 64 bits.  A row may be split over several
 // workgroups, whose (m, s) the second kernel joins.  That kernel also forms
 // the position's value and the sequence's sum in 64 bits: the log ratio of two
 // models is a small difference of large sums.  x - m is formed before the
@@ -20,8 +21,7 @@
 namespace dot_amd {
 namespace seqlogp {
 
-constexpr int kReadUnroll = 8;   // packs of a thread in flight: where a row is only read,
-constexpr int kUnroll = 4;       // and where it is written as well
+constexpr int kUnroll = 4;       // packs of a thread in flight (8: 2 % slower)
 constexpr int kJoinBlock = 1024; // threads of the per-sequence kernel
 
 struct Rows {
@@ -86,6 +86,15 @@ __device__ __forceinline__ Pack<T> row_pack(const T* p) {
     else return load_pack(p);
 }
 
+// 16 bytes of -inf of each type.
+__device__ const uint32_t kNothing[3][4] __attribute__((aligned(16))) = {
+    {0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u},
+    {0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u},
+    {0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u}};
+__device__ __forceinline__ const void* nothing_of(float) { return kNothing[DOT_F32]; }
+__device__ __forceinline__ const void* nothing_of(F16) { return kNothing[DOT_F16]; }
+__device__ __forceinline__ const void* nothing_of(BF16) { return kNothing[DOT_BF16]; }
+
 // Sum of N values, pairwise.
 template <int N>
 __device__ __forceinline__ float pairwise(const float* x) {
@@ -140,15 +149,24 @@ __device__ __forceinline__ double float_at(const void* p, int is64, int64_t i) {
     return is64 ? static_cast<const double*>(p)[i] : double(static_cast<const float*>(p)[i]);
 }
 
-// The value of a position from its row's statistics, which are kept for the
-// backward.
+// What a position needs besides its row's statistics.
+struct Own {
+    float x;     // its token's logit
+    double ref;  // the reference's log-probability
+};
 template <class T>
-__device__ __forceinline__ double position(const Rows& r, const JoinArgs& j, int64_t at, int tok, const MaxSum& t) {
-    const float x = to_float(row_of<T>(r, at)[tok]);
-    if (j.stats) j.stats[at] = make_float2(t.base(), float(1.0 / t.s));
-    double v = (double(x) - double(t.base())) * ((double(r.k) + double(r.klo)) * 0.693147180559945309417) - log(t.s);
-    if (j.ref && j.ref_per_token) v -= float_at(j.ref, j.ref64, at);
-    return v;
+__device__ __forceinline__ Own own_of(const Rows& r, const JoinArgs& j, int64_t at, int tok) {
+    return Own{to_float(row_of<T>(r, at)[tok]), j.ref && j.ref_per_token ? float_at(j.ref, j.ref64, at) : 0.0};
+}
+
+// The value of a position from the statistics of its row's other logits.  Those
+// of the whole row are kept for the backward.
+__device__ __forceinline__ double position(const Rows& r, const JoinArgs& j, int64_t at, const Own& own, MaxSum t) {
+    const double kn = (double(r.k) + double(r.klo)) * 0.693147180559945309417;  // 1 / tau
+    t.join(own.x, 1.0, r);
+    const float base = t.base();
+    if (j.stats) j.stats[at] = make_float2(base, float(1.0 / t.s));
+    return (double(own.x) - double(base)) * kn - log(t.s) - own.ref;
 }
 
 // Partial statistics of every row, one for each split; a row that is not split
@@ -168,25 +186,38 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, JoinArgs j, Part* pa
         if (r.splits == 1 && threadIdx.x == 0) put(0.0);
         return;
     }
+    Own own{};
+    if (r.splits == 1) own = own_of<T>(r, j, at, tok);  // on its way while the row is read
     const T* row = row_of<T>(r, at);
     const Span sp = span_of(row, r.V, part, r.splits);
     const T* body = row + sp.head;
     constexpr int PN = Pack<T>::N;
+    // The token's pack is read as logits of -inf; its other logits are added one
+    // by one at the end.  They are on their way while the row is read.
+    const int tok_pack = tok < sp.head || tok >= sp.tail ? -1 : (tok - sp.head) / PN;
+    float beside = -__builtin_inff();
+    if (tok_pack >= sp.p0 && tok_pack < sp.p1 && int(threadIdx.x) < PN) {
+        const int v = sp.head + tok_pack * PN + int(threadIdx.x);
+        if (v != tok) beside = to_float(row[v]);
+    }
+    const T* nothing = reinterpret_cast<const T*>(nothing_of(T{}));
     MaxSum a;
     auto packs = [&](auto stream) {
-        constexpr bool STREAM = decltype(stream)::value;
+        auto pack = [&](int p) {
+            return row_pack<decltype(stream)::value>(p == tok_pack ? nothing : body + int64_t(p) * PN);
+        };
         int p = sp.p0 + int(threadIdx.x);
-        for (; p + (kReadUnroll - 1) * kBlock < sp.p1; p += kReadUnroll * kBlock) {
-            Pack<T> x[kReadUnroll];
-            float f[kReadUnroll * PN];
+        for (; p + (kUnroll - 1) * kBlock < sp.p1; p += kUnroll * kBlock) {
+            Pack<T> x[kUnroll];
+            float f[kUnroll * PN];
 #pragma unroll
-            for (int u = 0; u < kReadUnroll; ++u) x[u] = row_pack<STREAM>(body + int64_t(p + u * kBlock) * PN);
+            for (int u = 0; u < kUnroll; ++u) x[u] = pack(p + u * kBlock);
 #pragma unroll
-            for (int i = 0; i < kReadUnroll * PN; ++i) f[i] = to_float(x[i / PN].v[i % PN]);
+            for (int i = 0; i < kUnroll * PN; ++i) f[i] = to_float(x[i / PN].v[i % PN]);
             a.add<PN>(f, r);
         }
         for (; p < sp.p1; p += kBlock) {
-            const Pack<T> x = row_pack<STREAM>(body + int64_t(p) * PN);
+            const Pack<T> x = pack(p);
             float f[PN];
 #pragma unroll
             for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
@@ -195,11 +226,15 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, JoinArgs j, Part* pa
     };
     if (at < r.cached) packs(std::true_type{});
     else packs(std::false_type{});
-    if (part == 0 && int(threadIdx.x) < sp.head) {
+    {
+        const float f[1] = {beside};
+        a.add<1>(f, r);
+    }
+    if (part == 0 && int(threadIdx.x) < sp.head && int(threadIdx.x) != tok) {
         const float f[1] = {to_float(row[threadIdx.x])};
         a.add<1>(f, r);
     }
-    if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) {
+    if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V && sp.tail + int(threadIdx.x) != tok) {
         const float f[1] = {to_float(row[sp.tail + threadIdx.x])};
         a.add<1>(f, r);
     }
@@ -216,7 +251,7 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, JoinArgs j, Part* pa
     if (threadIdx.x == 0) {
         MaxSum t;
         for (int w = 0; w < kWavesPerBlock; ++w) t.join(sm[w], ss[w], r);
-        if (r.splits == 1) put(position<T>(r, j, at, tok, t));
+        if (r.splits == 1) put(position(r, j, at, own, t));
         else parts[blockIdx.x] = Part{t.s, t.m};
     }
 }
@@ -245,7 +280,7 @@ __global__ __launch_bounds__(kJoinBlock) void join(Rows r, const Part* parts, Jo
                 const Part p = parts[at * r.splits + i];
                 t.join(p.m, p.s, r);
             }
-            v = position<T>(r, j, at, tok, t);
+            v = position(r, j, at, own_of<T>(r, j, at, tok), t);
         }
         sum += v;
         count += tok >= 0;
