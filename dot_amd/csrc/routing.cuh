@@ -234,9 +234,10 @@ __device__ __forceinline__ float mass_of(float x, int scoring) {
 }
 
 // Masses q of a row (softmax: exp(x - top), not yet divided), and 1 / sum q
-// (0 where the row has no mass; NaN stays NaN).
-template <class S>
-__device__ __forceinline__ void row_masses(const float (&x)[S::EL], int scoring, float (&q)[S::EL], float& top,
+// (0 where the row has no mass; NaN stays NaN).  SLOPE: x becomes dq/dx of the
+// masses that need no row statistics.
+template <class S, bool SLOPE = false>
+__device__ __forceinline__ void row_masses(float (&x)[S::EL], int scoring, float (&q)[S::EL], float& top,
                                            float& inv) {
     float sum = 0.0f;
     top = 0.0f;
@@ -250,10 +251,18 @@ __device__ __forceinline__ void row_masses(const float (&x)[S::EL], int scoring,
         for (int j = 0; j < S::EL; ++j) q[j] = fast_exp(x[j] - top);
     } else if (scoring == DOT_SCORING_SIGMOID) {
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) q[j] = logistic(x[j]);
+        for (int j = 0; j < S::EL; ++j) {
+            float t, u;
+            logistic_parts(x[j], t, u);
+            q[j] = x[j] < 0.0f ? t * u : u;
+            if (SLOPE) x[j] = t * u * u;  // q (1 - q), exact where q is near 1
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) q[j] = x[j] == kNegInf ? 0.0f : x[j];
+        for (int j = 0; j < S::EL; ++j) {
+            q[j] = x[j] == kNegInf ? 0.0f : x[j];
+            if (SLOPE) x[j] = 1.0f;
+        }
     }
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) sum += q[j];
@@ -696,7 +705,7 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
         const int64_t at = int64_t(b) * a.N + n;
         float x[S::EL], q[S::EL], top, inv;
         raw.get(gl, E, x);
-        row_masses<S>(x, a.scoring, q, top, inv);
+        row_masses<S, true>(x, a.scoring, q, top, inv);
         float add[S::EL];
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) add[j] = 0.0f;
@@ -751,13 +760,7 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
                 const float h = slope[j] + (in_h ? add[j] : 0.0f);
                 g[j] = fmaf(q[j] * inv, h - ph, in_h ? 0.0f : add[j]);
             } else {
-                g[j] = fmaf(slope[j] - ph, inv, add[j]);
-                if (a.scoring == DOT_SCORING_SIGMOID) {
-                    // q (1 - q) = t u^2: exact where q is near 1
-                    float t, u;
-                    logistic_parts(x[j], t, u);
-                    g[j] *= t * u * u;
-                }
+                g[j] = fmaf(slope[j] - ph, inv, add[j]) * x[j];
             }
             g[j] = live ? g[j] : 0.0f;
         }
