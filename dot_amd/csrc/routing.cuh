@@ -234,7 +234,7 @@ __device__ __forceinline__ float mass_of(float x, int scoring) {
 }
 
 // Masses q of a row (softmax: exp(x - top), not yet divided), and 1 / sum q
-// (0 where the row has no mass; NaN stays NaN).  SLOPE: x becomes dq/dx of the
+// (0 where the row has no mass: below the smallest normal float; NaN stays NaN).  SLOPE: x becomes dq/dx of the
 // masses that need no row statistics.
 template <class S, bool SLOPE = false>
 __device__ __forceinline__ void row_masses(float (&x)[S::EL], int scoring, float (&q)[S::EL], float& top,
@@ -267,7 +267,7 @@ __device__ __forceinline__ void row_masses(float (&x)[S::EL], int scoring, float
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) sum += q[j];
     sum = group_reduce<S::G>(sum, OpSum{});
-    inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    inv = fabsf(sum) < FLT_MIN ? 0.0f : 1.0f / sum;
 }
 
 struct FwdArgs {
@@ -342,7 +342,7 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
             const float t = x[j] + (bias ? bias[S::expert(gl, j)] : 0.0f);
             const int o = ordered(t);
             bool open = t > kNegInf;
-            if (plan) open = x[j] > 0.0f;
+            if (plan) open = open & (x[j] > 0.0f);
             key[j] = open ? o : kTaken;
         }
     };
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
                 }
                 z = group_reduce<S::G>(z, OpSum{});
                 // a division, so that a single expert's weight is 1 and its gradient 0
-                over = z == 0.0f ? 1.0f : z;
+                over = fabsf(z) < FLT_MIN ? __builtin_inff() : z;
                 scale = soft ? 1.0f + (inv - inv) : 1.0f;  // a row with NaN has no weights
             }
             const int64_t at = (row0 + n) * k;
@@ -727,7 +727,7 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
                 dot = group_reduce<S::G>(dot, OpSum{});
                 if (!soft) {
                     mass = group_reduce<S::G>(mass, OpSum{});
-                    over = mass == 0.0f ? __builtin_inff() : mass;
+                    over = fabsf(mass) < FLT_MIN ? __builtin_inff() : mass;
                     wave_lds_fence();
                 }
             }

@@ -97,7 +97,8 @@ def topk_routing(
 
     Experts are ordered by ``score + bias`` in fp32, equal ones by the lowest index.
     One is available where that is above -inf (and, with ``"plan"``, its mass above
-    0); a token with fewer than ``k`` has empty slots.  A NaN score is never
+    0); a token with fewer than ``k`` has empty slots.  Masses that sum to less than
+    the smallest normal fp32 count as none.  A NaN score is never
     selected; its token's softmax weights and the loss are NaN.
 
     Gradients reach ``scores`` from ``weights`` and ``balance_loss``.

@@ -109,6 +109,41 @@ def test_ties_go_to_the_lowest_index():
             check(scores.to(dtype), min(E, 12))
 
 
+def test_near_ties():
+    """Keys that differ in their last bits, among many equal ones, with and without a bias."""
+    rng = np.random.default_rng(11)
+    for E in (8, 61, 256, 1024, 4096):
+        k = min(E, 16)
+        near = torch.as_tensor((1 + rng.integers(0, 40, (2, 9, E)) * 2.0**-23).astype(np.float32))
+        near[0, 0] *= -1
+        near[1, 3] = torch.as_tensor(rng.standard_normal(E).astype(np.float32))
+        check(near, k, normalize=True)
+        check(near, k, "sigmoid", bias=(rng.integers(-1, 2, E) * 2.0**-24).astype(np.float32))
+        for dtype in (torch.float16, torch.bfloat16):  # every 16-bit value next to its neighbours
+            eps = torch.finfo(dtype).eps
+            half = torch.as_tensor((1 + rng.integers(-3, 4, (2, 9, E)) * eps / 2).astype(np.float32)).to(dtype)
+            half[0, 1] = half[0, 1] * torch.finfo(dtype).smallest_normal * eps * 3  # denormals
+            check(half, k)
+            check(half, k, bias=(rng.standard_normal(E) * 1e-6).astype(np.float32))
+
+
+def test_many_batch_elements():
+    """More batch elements than one grid dimension holds."""
+    B = 70001
+    x = torch.randn(B, 2, 8, device=DEV, generator=torch.Generator(DEV).manual_seed(0)).requires_grad_()
+    r = dot_amd.topk_routing(x, 2)
+    (g,) = torch.autograd.grad(r.balance_loss.sum(), x)
+    d = x.detach().double()
+    p = torch.softmax(d, -1)
+    counts = torch.zeros(B, 8, dtype=torch.int32, device=DEV)
+    counts.scatter_add_(1, r.experts.flatten(1).long(), torch.ones(B, 4, dtype=torch.int32, device=DEV))
+    assert torch.equal(r.counts, counts)
+    h = 8 * counts.double() / (2 * 2)  # E counts / (k n)
+    assert rel_err(r.balance_loss, (h * p.mean(1)).sum(1)) < TOL
+    h = h[:, None] / 2
+    assert rel_err(g, p * (h - (p * h).sum(-1, keepdim=True))) < TOL
+
+
 def test_unavailable_experts():
     """-inf scores are never taken; a token without experts has none; a row of the lowest value is a row like others."""
     rng = np.random.default_rng(5)
@@ -136,6 +171,22 @@ def test_unavailable_experts():
     for normalize in (False, True):
         r, g = check(plan, 4, "plan", normalize)
         assert (r.experts[0, 2] == -1).all() and (g[0, 2] == 0).all()
+        shut = np.zeros(16, np.float32)
+        shut[:14] = -np.inf
+        r, _ = check(plan, 4, "plan", normalize, bias=shut)
+        assert not ((r.experts >= 0) & (r.experts < 14)).any()
+    plan[0, 4] = 1e-42  # masses that no fp32 reciprocal holds
+    r = dot_amd.topk_routing(plan.to(DEV), 4, scoring="plan", normalize=True)
+    assert torch.isfinite(r.weights).all() and torch.isfinite(r.balance_loss).all()
+
+
+def test_a_single_expert_has_no_weight_gradient():
+    """k = 1, normalised: the weight is exactly 1, so that only the balance loss moves the scores."""
+    rng = np.random.default_rng(12)
+    for scoring in ("softmax", "sigmoid", "plan"):
+        scores = make_scores(rng, 2, 400, 24, scoring, torch.float32)
+        r, _ = check(scores, 1, scoring, True)
+        assert (r.weights == 1).all()
 
 
 def test_masked_tokens_are_not_read():

@@ -112,6 +112,24 @@ def test_long_sum_keeps_its_digits():
     assert np.abs(got - want).max() < 1e-3  # errors of single positions have both signs; sums in fp32 are off by 4e-3
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_likely_tokens_keep_their_digits(dtype):
+    """The value of a token that is nearly certain is small: its error is relative to it (and half a step of fp32).
+
+    sum of the others / own: each term to 2^-22, their sum to 2^-21 of itself, so 1e-6 of log(1 + that)."""
+    rng = np.random.default_rng(9)
+    for V in (8, 100, 4099, 40000):
+        x = torch.as_tensor(rng.standard_normal((2, 9, V)).astype(np.float32))
+        tokens = rng.integers(0, V, (2, 9))
+        for s in range(9):
+            x[:, s].scatter_(1, torch.as_tensor(tokens[:, s])[:, None], 12.0 + 2 * s)
+        x = x.to(DTYPES[dtype])
+        got = call(x.to(DEV), tokens, reduction="none").cpu().double().numpy()
+        want = torch.log_softmax(x.double(), -1).numpy()[np.arange(2)[:, None], np.arange(9)[None], tokens]
+        # log_softmax in 64 bits is itself off by 1e-15 of the largest logit
+        assert (np.abs(got - want) <= 2e-6 * np.abs(want) + 1e-14).all()
+
+
 def test_tokens_outside_are_left_out():
     rng = np.random.default_rng(3)
     logits, tokens = make(rng, 2, 12, 77, torch.bfloat16)
