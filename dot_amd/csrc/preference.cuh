@@ -9,6 +9,8 @@
 // `fold` adds the partials in strip order.
 #pragma once
 
+#include <type_traits>
+
 #include "row.cuh"
 #include "wave.cuh"
 
@@ -24,9 +26,21 @@ constexpr int kFoldBlock = 1024;         // threads of a fold workgroup,
 constexpr int kFoldCols = 64;            // of as many columns (or rows)
 
 struct Loss {
-    int type;
     float beta, smoothing;
 };
+
+// The loss types of the kernels: those of the C ABI, and the sigmoid loss
+// without smoothing.
+constexpr int kPlain = 3;
+
+// f(integral_constant) of a loss type.
+template <class F>
+void dispatch_type(int loss_type, float smoothing, F&& f) {
+    if (loss_type == DOT_PREFER_HINGE) f(std::integral_constant<int, DOT_PREFER_HINGE>{});
+    else if (loss_type == DOT_PREFER_SQUARE) f(std::integral_constant<int, DOT_PREFER_SQUARE>{});
+    else if (smoothing > 0.0f) f(std::integral_constant<int, DOT_PREFER_SIGMOID>{});
+    else f(std::integral_constant<int, kPlain>{});
+}
 
 // log(1 + e) for e in [0, 1]: 2 atanh(z) with z = e / (2 + e) <= 1/3, as
 // 2 z (1 + w p(w)), w = z^2.  p has the cubic's coefficients that fit
@@ -45,77 +59,75 @@ __device__ __forceinline__ float log1p_unit(float e) {
 }
 
 // f(gap) and, with SLOPE, df / dgap.
-template <bool SLOPE>
+template <int TYPE, bool SLOPE>
 __device__ __forceinline__ float loss_of(const Loss& l, float gap, float& slope) {
-    if (l.type == DOT_PREFER_SIGMOID) {
+    if constexpr (TYPE == DOT_PREFER_HINGE) {
+        const float room = fmaf(-l.beta, gap, 1.0f);
+        const bool shut = room <= 0.0f;  // not NaN
+        if (SLOPE) slope = shut ? 0.0f : room == room ? -l.beta : room;
+        return shut ? 0.0f : room;
+    } else if constexpr (TYPE == DOT_PREFER_SQUARE) {
+        const float miss = gap - 0.5f / l.beta;
+        if (SLOPE) slope = 2.0f * miss;
+        return miss * miss;
+    } else {
+        const float keep = TYPE == kPlain ? 1.0f : 1.0f - l.smoothing;
         const float d = l.beta * gap;
         const float e = fast_exp(-fabsf(d));
         if (SLOPE) {
-            const float u = __builtin_amdgcn_rcpf(1.0f + e);
-            const float up = d < 0.0f ? e * u : u;    // 1 / (1 + exp(-d))
-            const float down = d < 0.0f ? u : e * u;  // 1 - up, without the difference
-            slope = l.beta * (l.smoothing * up - (1.0f - l.smoothing) * down);
+            const float u = __builtin_amdgcn_rcpf(1.0f + e), eu = e * u;
+            const float down = d < 0.0f ? u : eu;  // 1 / (1 + exp(d)); the other one without a difference
+            slope = -l.beta * keep * down;
+            if constexpr (TYPE != kPlain) slope = fmaf(l.beta * l.smoothing, d < 0.0f ? eu : u, slope);
         }
         // log(1 + exp(-d)) and log(1 + exp(d)) share their tail
-        float f = fmaf(1.0f - l.smoothing, fmaxf(-d, 0.0f), log1p_unit(e));
-        if (l.smoothing > 0.0f) f = fmaf(l.smoothing, fmaxf(d, 0.0f), f);
+        float f = fmaf(keep, fmaxf(-d, 0.0f), log1p_unit(e));
+        if constexpr (TYPE != kPlain) f = fmaf(l.smoothing, fmaxf(d, 0.0f), f);
         return f;
     }
-    if (l.type == DOT_PREFER_HINGE) {
-        const float room = fmaf(-l.beta, gap, 1.0f);
-        if (SLOPE) slope = room > 0.0f ? -l.beta : (room == room ? 0.0f : room);
-        return room > 0.0f ? room : (room == room ? 0.0f : room);
-    }
-    const float miss = gap - 0.5f / l.beta;
-    if (SLOPE) slope = 2.0f * miss;
-    return miss * miss;
 }
 
+template <int TYPE>
 __global__ __launch_bounds__(kBlock) void pairs_forward(const float* ratio, int P, Loss l, float* loss) {
     const int i = int(blockIdx.x) * kBlock + int(threadIdx.x);
     float slope;
-    if (i < P) loss[i] = loss_of<false>(l, ratio[i] - ratio[P + i], slope);
+    if (i < P) loss[i] = loss_of<TYPE, false>(l, ratio[i] - ratio[P + i], slope);
 }
 
+template <int TYPE>
 __global__ __launch_bounds__(kBlock) void pairs_backward(const float* ratio, int P, Loss l, const float* grad,
                                                          int grad_scalar, float* grad_ratio) {
     const int i = int(blockIdx.x) * kBlock + int(threadIdx.x);
     if (i >= P) return;
     float slope;
-    loss_of<true>(l, ratio[i] - ratio[P + i], slope);
+    loss_of<TYPE, true>(l, ratio[i] - ratio[P + i], slope);
     const float g = grad[grad_scalar ? 0 : i] * slope;
     grad_ratio[i] = g;
     grad_ratio[P + i] = -g;
 }
 
-// kVec columns from j on; a column beyond Q is `fill`.
+// A thread's kVec columns of the tile from c0 on: four in a row (VEC, Q a
+// multiple of four: all in the plan or none), or every kBlock-th.
 template <bool VEC>
-__device__ __forceinline__ void load4(const float* p, int j, int Q, float (&x)[kVec], float fill) {
+__device__ __forceinline__ int column(int c0, int v) {
+    return VEC ? c0 + int(threadIdx.x) * kVec + v : c0 + int(threadIdx.x) + v * kBlock;
+}
+template <bool VEC>
+__device__ __forceinline__ void load4(const float* p, int c0, int Q, float (&x)[kVec]) {
     if constexpr (VEC) {
-        if (j < Q) {
-            const float4 t = *reinterpret_cast<const float4*>(p + j);
-            x[0] = t.x;
-            x[1] = t.y;
-            x[2] = t.z;
-            x[3] = t.w;
-        } else {
-            x[0] = x[1] = x[2] = x[3] = fill;
-        }
+        const float4 t = *reinterpret_cast<const float4*>(p + column<VEC>(c0, 0));
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) x[i] = j + i * kBlock < Q ? p[j + i * kBlock] : fill;
+        for (int v = 0; v < kVec; ++v) {
+            const int c = column<VEC>(c0, v);
+            x[v] = c < Q ? p[c] : 0.0f;
+        }
     }
 }
 
-// First of a thread's columns in the tile from c0 on: four in a row, or every
-// kBlock-th.
-template <bool VEC>
-__device__ __forceinline__ int first_col(int c0) {
-    return c0 + (VEC ? int(threadIdx.x) * kVec : int(threadIdx.x));
-}
-
 // One workgroup per row.
-template <bool VEC>
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(kBlock) void plan_forward(const float* ratio, const float* plan, int P, int Q, Loss l,
                                                        float* loss) {
     __shared__ float sm[kWavesPerBlock];
@@ -123,23 +135,15 @@ __global__ __launch_bounds__(kBlock) void plan_forward(const float* ratio, const
     const float ri = ratio[i];
     const float* row = plan + int64_t(i) * Q;
     float sum = 0.0f;
+#pragma unroll 2
     for (int c0 = 0; c0 < Q; c0 += kCols) {
-        const int j = first_col<VEC>(c0);
-        float x[kVec], rj[kVec], slope;
-        load4<VEC>(row, j, Q, x, 0.0f);
-        if (VEC && P % kVec == 0) {
-            load4<true>(ratio + P, j, Q, rj, 0.0f);
-        } else {
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const int c = VEC ? j + v : j + v * kBlock;
-                rj[v] = c < Q ? ratio[P + c] : 0.0f;
-            }
-        }
+        if (column<VEC>(c0, 0) >= Q) break;
+        float x[kVec], slope;
+        load4<VEC>(row, c0, Q, x);
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-            const int c = VEC ? j + v : j + v * kBlock;
-            if (c < Q) sum = fmaf(x[v], loss_of<false>(l, ri - rj[v], slope), sum);
+            const int c = column<VEC>(c0, v);
+            if (VEC || c < Q) sum = fmaf(x[v], loss_of<TYPE, false>(l, ri - ratio[P + c], slope), sum);
         }
     }
     sum = block_reduce<kWavesPerBlock>(wave_sum(sum), sm, OpSum{});
@@ -160,42 +164,43 @@ struct PlanBwd {
 };
 
 // One tile: a strip of rows by kCols columns.
-template <bool VEC>
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(kBlock) void plan_backward(PlanBwd a) {
     __shared__ float sm[kMaxStrip][kWavesPerBlock];
     const int tile = blockIdx.x % unsigned(a.ncols), strip = blockIdx.x / unsigned(a.ncols);
-    const int i0 = strip * a.strip, rows = min(a.strip, a.P - i0);
-    const int j = first_col<VEC>(tile * kCols);
+    const int i0 = strip * a.strip, rows = min(a.strip, a.P - i0), c0 = tile * kCols;
+    const bool some = column<VEC>(c0, 0) < a.Q;
     float rj[kVec], col[kVec];
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-        const int c = VEC ? j + v : j + v * kBlock;
+        const int c = column<VEC>(c0, v);
         rj[v] = c < a.Q ? a.ratio[a.P + c] : 0.0f;
         col[v] = 0.0f;
     }
     for (int r = 0; r < rows; ++r) {
         const int i = i0 + r;
         const float ri = a.ratio[i], g = a.grad[a.grad_scalar ? 0 : i];
-        float x[kVec], f[kVec], slope, sum = 0.0f;
-        load4<VEC>(a.plan + int64_t(i) * a.Q, j, a.Q, x, 0.0f);
+        float sum = 0.0f;
+        if (some) {
+            float x[kVec], f[kVec], slope;
+            load4<VEC>(a.plan + int64_t(i) * a.Q, c0, a.Q, x);
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-            const int c = VEC ? j + v : j + v * kBlock;
-            if (c < a.Q) {
-                f[v] = g * loss_of<true>(a.l, ri - rj[v], slope);
+            for (int v = 0; v < kVec; ++v) {
+                if (!VEC && column<VEC>(c0, v) >= a.Q) continue;
+                f[v] = g * loss_of<TYPE, true>(a.l, ri - rj[v], slope);
                 const float pull = g * x[v] * slope;
                 sum += pull;
                 col[v] += pull;
             }
-        }
-        if (a.grad_plan) {
-            float* out = a.grad_plan + int64_t(i) * a.Q;
-            if constexpr (VEC) {
-                if (j < a.Q) *reinterpret_cast<float4*>(out + j) = make_float4(f[0], f[1], f[2], f[3]);
-            } else {
+            if (a.grad_plan) {
+                float* out = a.grad_plan + int64_t(i) * a.Q;
+                if constexpr (VEC) {
+                    *reinterpret_cast<float4*>(out + column<VEC>(c0, 0)) = make_float4(f[0], f[1], f[2], f[3]);
+                } else {
 #pragma unroll
-                for (int v = 0; v < kVec; ++v)
-                    if (j + v * kBlock < a.Q) out[j + v * kBlock] = f[v];
+                    for (int v = 0; v < kVec; ++v)
+                        if (column<VEC>(c0, v) < a.Q) out[column<VEC>(c0, v)] = f[v];
+                }
             }
         }
         sum = wave_sum(sum);
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void plan_backward(PlanBwd a) {
     float* cp = a.colpart + int64_t(strip) * a.Q;
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-        const int c = VEC ? j + v : j + v * kBlock;
+        const int c = column<VEC>(c0, v);
         if (c < a.Q) cp[c] = col[v];
     }
 }

@@ -60,20 +60,20 @@ extern "C" int dot_preference_forward(const dot_preference_fwd_args* a, dot_stre
     if (int rc = check_common(a->P, a->Q, has_plan, a->loss_type, a->beta, a->smoothing)) return rc;
     if (a->P == 0) return ok();
     if (!a->ratio || !a->loss) return fail(DOT_ERR_INVALID_ARG, "ratio and loss must be non-NULL");
-    const preference::Loss l{a->loss_type, a->beta, a->smoothing};
-    if (!has_plan) {
-        ProfScope prof("preference_pairs_forward", stream);
-        hipLaunchKernelGGL(preference::pairs_forward, dim3(blocks_of(a->P)), dim3(kBlock), 0, stream, a->ratio, a->P,
-                           l, a->loss);
-    } else {
-        ProfScope prof("preference_plan_forward", stream);
-        if (a->Q % preference::kVec == 0 && aligned16(a->plan) && aligned16(a->ratio))
-            hipLaunchKernelGGL((preference::plan_forward<true>), dim3(unsigned(a->P)), dim3(kBlock), 0, stream,
+    const preference::Loss l{a->beta, a->smoothing};
+    preference::dispatch_type(a->loss_type, a->smoothing, [&](auto type) {
+        constexpr int T = decltype(type)::value;
+        ProfScope prof(has_plan ? "preference_plan_forward" : "preference_pairs_forward", stream);
+        if (!has_plan)
+            hipLaunchKernelGGL((preference::pairs_forward<T>), dim3(blocks_of(a->P)), dim3(kBlock), 0, stream,
+                               a->ratio, a->P, l, a->loss);
+        else if (a->Q % preference::kVec == 0 && aligned16(a->plan))
+            hipLaunchKernelGGL((preference::plan_forward<T, true>), dim3(unsigned(a->P)), dim3(kBlock), 0, stream,
                                a->ratio, a->plan, a->P, a->Q, l, a->loss);
         else
-            hipLaunchKernelGGL((preference::plan_forward<false>), dim3(unsigned(a->P)), dim3(kBlock), 0, stream,
+            hipLaunchKernelGGL((preference::plan_forward<T, false>), dim3(unsigned(a->P)), dim3(kBlock), 0, stream,
                                a->ratio, a->plan, a->P, a->Q, l, a->loss);
-    }
+    });
     return check_launch("dot_preference_forward");
 }
 
@@ -90,11 +90,14 @@ extern "C" int dot_preference_backward(const dot_preference_bwd_args* a, dot_str
     if (a->P == 0 && a->Q == 0) return ok();
     if (!a->ratio || (a->P > 0 && !a->grad_loss) || !a->grad_ratio)
         return fail(DOT_ERR_INVALID_ARG, "ratio, grad_loss and grad_ratio must be non-NULL");
-    const preference::Loss l{a->loss_type, a->beta, a->smoothing};
+    const preference::Loss l{a->beta, a->smoothing};
     if (!has_plan) {
-        ProfScope prof("preference_pairs_backward", stream);
-        hipLaunchKernelGGL(preference::pairs_backward, dim3(blocks_of(a->P)), dim3(kBlock), 0, stream, a->ratio, a->P,
-                           l, a->grad_loss, a->grad_loss_scalar, a->grad_ratio);
+        preference::dispatch_type(a->loss_type, a->smoothing, [&](auto type) {
+            ProfScope prof("preference_pairs_backward", stream);
+            hipLaunchKernelGGL((preference::pairs_backward<decltype(type)::value>), dim3(blocks_of(a->P)),
+                               dim3(kBlock), 0, stream, a->ratio, a->P, l, a->grad_loss, a->grad_loss_scalar,
+                               a->grad_ratio);
+        });
         return check_launch("dot_preference_backward");
     }
     if (a->P == 0 || a->Q == 0) {  // an empty plan: no gradient reaches the ratios
@@ -119,13 +122,14 @@ extern "C" int dot_preference_backward(const dot_preference_bwd_args* a, dot_str
     x.colpart = L.colpart;
     x.rowpart = L.rowpart;
     const dim3 grid(unsigned(L.nstrips) * unsigned(L.ncols));
-    {
+    preference::dispatch_type(a->loss_type, a->smoothing, [&](auto type) {
+        constexpr int T = decltype(type)::value;
         ProfScope prof("preference_plan_backward", stream);
         if (a->Q % preference::kVec == 0 && aligned16(a->plan) && (!a->grad_plan || aligned16(a->grad_plan)))
-            hipLaunchKernelGGL((preference::plan_backward<true>), grid, dim3(kBlock), 0, stream, x);
+            hipLaunchKernelGGL((preference::plan_backward<T, true>), grid, dim3(kBlock), 0, stream, x);
         else
-            hipLaunchKernelGGL((preference::plan_backward<false>), grid, dim3(kBlock), 0, stream, x);
-    }
+            hipLaunchKernelGGL((preference::plan_backward<T, false>), grid, dim3(kBlock), 0, stream, x);
+    });
     {
         ProfScope prof("preference_plan_fold", stream);
         const int row_blocks = (a->P + preference::kFoldCols - 1) / preference::kFoldCols;
