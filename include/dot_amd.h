@@ -1,5 +1,6 @@
 /*
- * dot_amd — C ABI of the MI355X (gfx950) Sinkhorn and bidirectional-softmax engine.
+ * dot_amd — C ABI of the MI355X (gfx950) Sinkhorn and bidirectional-softmax engine,
+ * with the routing and preference operators beside it.
  *
  * Plain pointers and sizes only.  Every pointer argument is device memory
  * owned by the caller (fp32 unless stated); the library allocates nothing on
