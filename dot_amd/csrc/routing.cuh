@@ -328,33 +328,33 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
 // wave selects again by whole keys.  65536 rows of 256 fp32 scores, k = 8:
 // 52 us for the forward with the whole keys alone.
 template <class T, class S>
-__device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, const float* bias, bool plan, int gl,
-                                       int E, int k, Slot* stage) {
+__device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, const float* bias, bool biased, bool plan,
+                                       int gl, int E, int k, Slot* stage) {
     constexpr unsigned kMask = S::G * S::EL - 1;  // a power of two less one
     constexpr int kBits = __builtin_popcount(kMask);
-    // Ordered keys of a row, kTaken where an expert is not available.  (The bias
-    // has a place for every element; adding it, or 0, makes -0 a 0.)
-    auto keys = [&](const RawRow<T, S>& from, int (&key)[S::EL]) {
-        float x[S::EL];
+    // A row's scores with the bias (0 where there is none; -0 becomes 0), and
+    // whether an expert is available.
+    float x[S::EL];
+    bool open[S::EL];
+    auto load = [&](const RawRow<T, S>& from) {
         from.get(gl, E, x);
 #pragma unroll
+        for (int j = 0; j < S::EL; ++j) open[j] = x[j] > (plan ? 0.0f : kNegInf);
+#pragma unroll
         for (int j = 0; j < S::EL; ++j) {
-            const float t = x[j] + (bias ? bias[S::expert(gl, j)] : 0.0f);
-            const int o = ordered(t);
-            bool open = t > kNegInf;
-            if (plan) open = open & (x[j] > 0.0f);
-            key[j] = open ? o : kTaken;
+            x[j] += bias[S::expert(gl, j)];
+            open[j] = open[j] & (x[j] > kNegInf);
         }
     };
-    int key[S::EL];
+    load(raw);
     unsigned u[S::EL];
-    keys(raw, key);
 #pragma unroll
     for (int j = 0; j < S::EL; ++j) {
-        // the key's low bits give way to the expert (those of a 16-bit score are all alike); kTaken becomes 0
-        const unsigned upper = (unsigned(key[j]) ^ 0x80000000u) >> 1;
+        // the key's low bits give way to the expert (those of a 16-bit score are all alike)
+        const unsigned i = __builtin_bit_cast(unsigned, x[j]);
+        const unsigned upper = (i ^ (unsigned(int(i) >> 31) | 0x80000000u)) >> 1;
         const unsigned both = (upper & ~kMask) | (kMask - unsigned(S::expert(gl, j)));
-        u[j] = key[j] == kTaken ? 0u : both;
+        u[j] = open[j] ? both : 0u;
     }
     unsigned m = 0x80000000u;
     bool close = false;  // winners that agree in the key's upper bits
@@ -374,13 +374,16 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
         if (r0 + gl < k) stage[r0 + gl].e = mine ? int(kMask - (mine & kMask)) : -1;
     }
     wave_lds_fence();
-    const bool whole = sizeof(T) == 2 && !bias;
+    const bool whole = sizeof(T) == 2 && !biased;
     if (whole || !__any(close)) return;
 
     // Whole keys; the row is read again rather than kept over the rounds above.
     RawRow<T, S> again;
     again.load(row, gl, E, raw.live);
-    keys(again, key);
+    load(again);
+    int key[S::EL];
+#pragma unroll
+    for (int j = 0; j < S::EL; ++j) key[j] = open[j] ? ordered(x[j]) : kTaken;
     for (int r = 0; r < k; ++r) {
         int top = key[0];
 #pragma unroll
@@ -413,8 +416,8 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
     int* hist = reinterpret_cast<int*>(lds + kColRows * E);
     float* bias = lds + bias_at(kColRows, E);
     for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
-    if (SELECT && a.bias)
-        for (int e = threadIdx.x; e < S::G * S::EL; e += kThreads) bias[e] = e < E ? a.bias[e] + 0.0f : 0.0f;
+    if (SELECT)
+        for (int e = threadIdx.x; e < S::G * S::EL; e += kThreads) bias[e] = a.bias && e < E ? a.bias[e] + 0.0f : 0.0f;
     if (threadIdx.x == 0) ntokens = 0;
     __syncthreads();
 
@@ -459,7 +462,7 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
 
         if constexpr (SELECT) {
             const T* row = scores + int64_t(n) * a.sn;
-            select<T, S>(row, raw, a.bias ? bias : nullptr, a.scoring == DOT_SCORING_PLAN, gl, E, k, stage);
+            select<T, S>(row, raw, bias, a.bias != nullptr, a.scoring == DOT_SCORING_PLAN, gl, E, k, stage);
             // Each slot's expert and score.
             for (int r = gl; r < k; r += S::G) {
                 const int e = stage[r].e;
