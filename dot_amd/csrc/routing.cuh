@@ -359,6 +359,7 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
     unsigned m = 0x80000000u;
     bool close = false;  // winners that agree in the key's upper bits
     for (int r0 = 0; r0 <= k; r0 += S::G) {
+        const unsigned last = m;
         unsigned mine = 0;  // the winner of round r0 + gl
         const int rounds = min(k + 1 - r0, S::G);
         for (int r = 0; r < rounds; ++r) {
@@ -366,12 +367,13 @@ __device__ __forceinline__ void select(const T* row, const RawRow<T, S>& raw, co
 #pragma unroll
             for (int j = 1; j < S::EL; ++j) d = max(d, u[j] - m);
             d = group_reduce<S::G>(d, OpMaxUint{});
-            const unsigned next = m == 0u ? 0u : m + d;
-            close |= next != 0u && ((next ^ m) >> kBits) == 0u;
-            m = next;
+            m = m == 0u ? 0u : m + d;
             mine = r == gl ? m : mine;
         }
         if (r0 + gl < k) stage[r0 + gl].e = mine ? int(kMask - (mine & kMask)) : -1;
+        const unsigned beside = __shfl_up(mine, 1);
+        const unsigned before = gl == 0 ? last : beside;
+        close |= mine != 0u && ((mine ^ before) >> kBits) == 0u;
     }
     wave_lds_fence();
     const bool whole = sizeof(T) == 2 && !biased;
