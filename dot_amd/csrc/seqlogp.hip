@@ -18,16 +18,16 @@ int splits_of(int B, int S, int V, int dtype) {
     return int(std::min(want, most));
 }
 
-int check_shape(int dtype, int B, int S, int V, float tau, int reduction) {
+int check_shape(int dtype, int B, int S, int V, double tau, int reduction) {
     if (!known_dtype(dtype)) return fail(DOT_ERR_INVALID_ARG, "dtype must be DOT_F32, DOT_F16 or DOT_BF16");
     if (B < 0 || S < 0) return fail(DOT_ERR_INVALID_ARG, "B and S must be >= 0");
     if (V < 1) return fail(DOT_ERR_INVALID_ARG, "V must be >= 1");
     // a grid dimension holds less than 2^32 threads
     if (V > (1 << 30) || int64_t(B) * S > (1 << 23))
         return fail(DOT_ERR_UNSUPPORTED, "V must be at most 2^30 and B * S at most 2^23");
-    if (!(tau > 0.0f) || !std::isfinite(tau)) return fail(DOT_ERR_INVALID_ARG, "tau must be > 0");
+    if (!(tau > 0.0) || !std::isfinite(tau)) return fail(DOT_ERR_INVALID_ARG, "tau must be > 0");
     // log2(e) / tau and its rest are normal floats
-    if (tau < 1e-20f || tau > 1e20f) return fail(DOT_ERR_UNSUPPORTED, "tau must be in [1e-20, 1e20]");
+    if (tau < 1e-20 || tau > 1e20) return fail(DOT_ERR_UNSUPPORTED, "tau must be in [1e-20, 1e20]");
     if (reduction != DOT_REDUCE_NONE && reduction != DOT_REDUCE_SUM && reduction != DOT_REDUCE_MEAN)
         return fail(DOT_ERR_INVALID_ARG, "reduction must be a DOT_REDUCE_* value");
     return DOT_OK;
@@ -57,7 +57,7 @@ seqlogp::Rows rows_of(const A* a, bool training) {
     r.tokens = a->tokens;
     r.tokens64 = a->tokens_are_int64;
     r.mask = a->mask;
-    const double k = 1.4426950408889634074 / double(a->tau);
+    const double k = 1.4426950408889634074 / a->tau;
     r.k = float(k);
     if (double(r.k) >= k) r.k = std::nextafter(r.k, 0.0f);
     r.klo = float(k - double(r.k));
@@ -127,7 +127,7 @@ extern "C" int dot_seqlogp_backward(const dot_seqlogp_bwd_args* a, dot_stream_t 
         return fail(DOT_ERR_INVALID_ARG, "the gradient of a mean needs weight");
     const seqlogp::Rows r = rows_of(a, true);
     seqlogp::GradArgs g{};
-    g.inv_tau = 1.0f / a->tau;
+    g.inv_tau = float(1.0 / a->tau);
     g.reduction = a->reduction;
     g.stats = reinterpret_cast<const float2*>(a->row_stats);
     g.weight = a->weight;

@@ -223,7 +223,7 @@ void fill_rows(A& a, const Tensor& logits, const Tensor& tokens, const Tensor& m
     a.tokens = tokens.const_data_ptr();
     a.tokens_are_int64 = tokens.scalar_type() == at::kLong;
     a.mask = mask_ptr(mask);
-    a.tau = float(tau);
+    a.tau = tau;
     a.reduction = int(reduction);
 }
 

@@ -448,7 +448,7 @@ typedef struct {
     const void* ref;           /* fp32 (double with ref_is_f64) log-probabilities to subtract: [B,S]
                                   (ref_per_token) or [B], or NULL */
     int ref_is_f64, ref_per_token;
-    float tau;                 /* > 0 */
+    double tau;                /* > 0; a float's rounding would show in sums over long answers */
     int reduction;             /* DOT_REDUCE_* over the positions that are not left out */
     float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
     float* row_stats;          /* [B,S,2] out, for the backward: the row's max and
@@ -471,7 +471,7 @@ typedef struct {
     const void* tokens;
     int tokens_are_int64;
     const uint8_t* mask;
-    float tau;
+    double tau;
     int reduction;
     const float* row_stats;
     const float* weight;       /* with DOT_REDUCE_MEAN */

@@ -100,16 +100,19 @@ def test_references(ref_type, per_token, int_type):
     check(logits, tokens, ref=ref, reduction="mean", int_type=int_type)
 
 
-def test_long_sum_keeps_its_digits():
+@pytest.mark.parametrize("tau", [1.0, 1.3, 0.7])
+def test_long_sum_keeps_its_digits(tau):
     """The log ratio of a long answer to a reference given per position: a few units out of thousands."""
     rng = np.random.default_rng(2)
     logits, tokens = make(rng, 2, 4096, 300, torch.float32)
-    per, _, _ = oracle.sequence_logp(logits.numpy(), tokens, reduction="none")
+    per, _, _ = oracle.sequence_logp(logits.numpy(), tokens, tau=tau, reduction="none")
     ref = per + 1e-3 * rng.standard_normal(per.shape)
-    want, _, _ = oracle.sequence_logp(logits.numpy(), tokens, ref=ref)
-    got = call(logits.to(DEV), tokens, ref=ref).cpu().double().numpy()
+    want, _, _ = oracle.sequence_logp(logits.numpy(), tokens, ref=ref, tau=tau)
+    got = call(logits.to(DEV), tokens, ref=ref, tau=tau).cpu().double().numpy()
     assert (np.abs(got - want) <= 4096 * PER_POSITION).all()
-    assert np.abs(got - want).max() < 1e-3  # errors of single positions have both signs; sums in fp32 are off by 4e-3
+    # Errors of single positions have both signs: 1e-7 sqrt(4096) is 6e-6, and 5e-8 of bias 2e-4.  A temperature
+    # rounded to fp32 would give 4e-8 of x - E[x], 6e-4 here; sums in fp32 are off by 4e-3.
+    assert np.abs(got - want).max() < 3e-4
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])

@@ -231,7 +231,7 @@ def lib():
     return lib
 
 
-P, I, I64, F, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+P, I, I64, F, D, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 
 
 def struct(*fields):
@@ -248,7 +248,7 @@ RoutingBwd = struct(("scores", P), ("dtype", I), ("stride_b", I64), ("stride_n",
                     ("grad_scores", P))
 SeqFwd = struct(("logits", P), ("dtype", I), ("stride_b", I64), ("stride_s", I64), ("B", I), ("S", I), ("V", I),
                 ("tokens", P), ("tokens_are_int64", I), ("mask", P), ("ref", P), ("ref_is_f64", I),
-                ("ref_per_token", I), ("tau", F), ("reduction", I), ("out", P), ("row_stats", P), ("weight", P),
+                ("ref_per_token", I), ("tau", D), ("reduction", I), ("out", P), ("row_stats", P), ("weight", P),
                 ("workspace", P), ("workspace_bytes", Z))
 PrefFwd = struct(("ratio", P), ("plan", P), ("P", I), ("Q", I), ("loss_type", I), ("beta", F), ("smoothing", F),
                  ("loss", P))
@@ -292,6 +292,7 @@ def test_c_abi_refusals(lib):
     s = dict(logits=some, B=2, S=3, V=16, tokens=some, tau=1.0, reduction=1, out=some)
     f = "dot_seqlogp_forward"
     refused(lib, f, INVALID, "tau", SeqFwd(**{**s, "tau": 0.0}))
+    refused(lib, f, UNSUPPORTED, "tau", SeqFwd(**{**s, "tau": 1e-30}))
     refused(lib, f, INVALID, "V must", SeqFwd(**{**s, "V": 0}))
     refused(lib, f, UNSUPPORTED, "2^23", SeqFwd(**{**s, "B": 4096, "S": 4096}))
     refused(lib, f, INVALID, "reduction", SeqFwd(**{**s, "reduction": 5}))
