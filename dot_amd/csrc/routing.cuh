@@ -35,8 +35,10 @@ struct Shape {
 
 // f(Shape) of a group that holds E <= DOT_ROUTING_MAX_EXPERTS elements.  A round
 // of the selection costs a wave about 8 + 1.5 EL + log2(G) instructions for its
-// 64 / G rows, so the forward (PAIRS) takes two vectors per lane from 128 experts
-// on; the backward, bound by its loads, is faster with twice the lanes.
+// 64 / G rows, so a forward that selects (PAIRS) takes two vectors per lane from
+// 128 experts on: 65536 x 256 fp32, k = 8, 33.3 us, with twice the lanes 43.6.
+// Without a selection, and in the backward, twice the lanes are faster: 13.6 us
+// against 15.1, and 39.6 against 44.1.
 template <bool VEC, bool PAIRS, class F>
 void dispatch_shape(int E, F&& f) {
     if (E <= 8) f(Shape<1, 1, VEC>{});
@@ -52,7 +54,8 @@ void dispatch_shape(int E, F&& f) {
 }
 
 // Threads of a forward workgroup.  Few partial rows make `finish` short, so
-// workgroups are large where a lane's registers allow it (up to two vectors).
+// workgroups are large where a lane's registers allow it (up to two vectors; the
+// forward above takes 40.2 us with 512 workgroups of 256 threads).
 constexpr int fwd_block(int R) { return R <= 2 ? 512 : 256; }
 // Waves per SIMD that the registers have to leave room for: two workgroups per CU.
 constexpr int fwd_waves(int R) { return R <= 2 ? 4 : 1; }

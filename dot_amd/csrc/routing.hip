@@ -1,5 +1,5 @@
 // C ABI of the routing operators: argument checks and launches.
-#include <cmath>
+#include <algorithm>
 
 #include "host.hpp"
 #include "routing.cuh"
@@ -30,10 +30,10 @@ struct FwdLayout {
 };
 
 // About 512 workgroups, two per CU.
-FwdLayout fwd_layout(void* ws, int B, int N, int E) {
+FwdLayout fwd_layout(void* ws, int B, int N, int E, bool select) {
     Carver c(ws);
     FwdLayout L{};
-    const Lanes lanes = lanes_of<true>(E);
+    const Lanes lanes = select ? lanes_of<true>(E) : lanes_of<false>(E);
     L.lanes = lanes;
     L.threads = routing::fwd_block(lanes.r);
     L.rows = L.threads / lanes.g;
@@ -84,7 +84,7 @@ using namespace dot_amd;
 
 extern "C" size_t dot_routing_forward_workspace_bytes(int B, int N, int E) {
     if (B < 0 || N < 0 || E < 1) return 0;
-    return fwd_layout(nullptr, B, N, E).bytes;
+    return std::max(fwd_layout(nullptr, B, N, E, true).bytes, fwd_layout(nullptr, B, N, E, false).bytes);
 }
 
 extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t stream_) {
@@ -97,7 +97,7 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     if (!a->counts || !a->loss) return fail(DOT_ERR_INVALID_ARG, "counts and loss must be non-NULL");
     if (a->N > 0 && (!a->scores || (select && (!a->weights || !a->experts))))
         return fail(DOT_ERR_INVALID_ARG, "scores, weights and experts must be non-NULL");
-    const FwdLayout L = fwd_layout(a->workspace, a->B, a->N, a->E);
+    const FwdLayout L = fwd_layout(a->workspace, a->B, a->N, a->E, select);
     if (L.bytes > 0 && (!a->workspace || a->workspace_bytes < L.bytes))
         return fail(DOT_ERR_WORKSPACE, "workspace smaller than dot_routing_forward_workspace_bytes()");
     routing::FwdArgs x{};
@@ -127,15 +127,20 @@ extern "C" int dot_routing_forward(const dot_routing_fwd_args* a, dot_stream_t s
     x.loss = a->loss;
     const dim3 grid = batch_grid(unsigned(L.nchunks), a->B);
     const size_t lds = routing::fwd_lds_bytes(a->E, a->k, L.lanes.g, L.lanes.r, L.rows, select);
-    dispatch<true>(a->dtype, a->E, rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype), [&](auto t, auto s) {
+    const bool vec = rows_aligned(a->scores, a->stride_b, a->stride_n, a->E, a->dtype);
+    {
         ProfScope prof("routing_forward", stream);
         if (select)
-            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), true>), grid, dim3(L.threads), lds, stream,
-                               x);
+            dispatch<true>(a->dtype, a->E, vec, [&](auto t, auto s) {
+                hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), true>), grid, dim3(L.threads), lds,
+                                   stream, x);
+            });
         else
-            hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), false>), grid, dim3(L.threads), lds, stream,
-                               x);
-    });
+            dispatch<false>(a->dtype, a->E, vec, [&](auto t, auto s) {
+                hipLaunchKernelGGL((routing::forward<decltype(t), decltype(s), false>), grid, dim3(L.threads), lds,
+                                   stream, x);
+            });
+    }
     if (L.nchunks > 1) {
         ProfScope prof("routing_finish", stream);
         const routing::FinishArgs f{a->B, a->E, a->k, L.nchunks, L.psum, L.pcount, L.ptokens, L.dots, L.done,

@@ -9,7 +9,9 @@ namespace dot_amd {
 namespace {
 
 // Workgroups per row: rows alone fill the chip (2048 workgroups, eight per
-// CU); fewer rows are split, into spans of at least two packs per thread.
+// CU); fewer rows are split, into spans of at least two packs per thread.  Split
+// and whole, bf16: 1 x 131072 3.9 and 14.3 us, 7 x 32768 4.1 and 6.8, 64 x 131072
+// 7.8 and 15.5, 512 x 32768 10.5 and 10.2 (4 parts).
 int splits_of(int B, int S, int V, int dtype) {
     const int64_t rows = int64_t(B) * S;
     const int packs = V / (16 / dtype_bytes(dtype));
