@@ -468,46 +468,58 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
         if constexpr (SELECT) {
             const T* row = scores + int64_t(n) * a.sn;
             select<T, S>(row, raw, bias, a.bias != nullptr, a.scoring == DOT_SCORING_PLAN, gl, E, k, stage);
-            // Each slot's expert and score.
-            for (int r = gl; r < k; r += S::G) {
-                const int e = stage[r].e;
-                float s = 0.0f;
-                if (e >= 0) {
-                    s = to_float(row[e]);
-                    atomicAdd(&hist[e], 1);
-                }
-                stage[r].s = s;
-            }
-            // Weights: exp(s - top) or q(s), over the row's or the selected ones' sum.
             const bool soft = a.scoring == DOT_SCORING_SOFTMAX;
+            const int64_t at = (row0 + n) * k;
+            // The score of a slot's expert, which is counted.
+            auto score = [&](int e) {
+                if (e < 0) return kNegInf;
+                atomicAdd(&hist[e], 1);
+                return to_float(row[e]);
+            };
+            // A slot's mass: exp(s - top) or q(s); 0 for an empty one.
+            auto mass = [&](int e, float s) {
+                return e < 0 ? 0.0f : soft ? fast_exp(s - top) : mass_of(s, a.scoring);
+            };
+            // The largest selected score, from the lanes' largest.
+            auto largest = [&](float s) {
+                s = group_reduce<S::G>(s, OpMax{});
+                top = s == kNegInf ? 0.0f : s;
+            };
+            // Weights: masses over the row's sum, or over that of the selected ones (a
+            // division, so that a single expert's weight is 1 and its gradient 0; a
+            // row with NaN has no softmax weights).
             float scale = soft ? inv : 1.0f, over = 1.0f;
-            if (a.normalize) {
-                if (soft) {
-                    float m = kNegInf;
-                    for (int r = gl; r < k; r += S::G) {
-                        const Slot t = stage[r];
-                        if (t.e >= 0) m = fmaxf(m, t.s);
-                    }
-                    m = group_reduce<S::G>(m, OpMax{});
-                    top = m == kNegInf ? 0.0f : m;
+            auto normalizer = [&](float z) {
+                z = group_reduce<S::G>(z, OpSum{});
+                over = fabsf(z) < FLT_MIN ? __builtin_inff() : z;
+                scale = soft ? 1.0f + (inv - inv) : 1.0f;
+            };
+            if (k <= S::G) {  // a slot per lane
+                const int e = gl < k ? stage[gl].e : -1;
+                const float s = score(e);
+                if (a.normalize && soft) largest(s);
+                const float w = mass(e, s);
+                if (a.normalize) normalizer(w);
+                if (in && gl < k) {
+                    a.weights[at + gl] = e < 0 ? 0.0f : w * scale / over;
+                    a.experts[at + gl] = e;
                 }
-                float z = 0.0f;
+            } else {
+                float most = kNegInf, z = 0.0f;
+                for (int r = gl; r < k; r += S::G) {
+                    const float s = score(stage[r].e);
+                    stage[r].s = s;
+                    most = fmaxf(most, s);
+                }
+                if (a.normalize && soft) largest(most);
+                for (int r = gl; r < k; r += S::G) z += mass(stage[r].e, stage[r].s);
+                if (a.normalize) normalizer(z);
                 for (int r = gl; r < k; r += S::G) {
                     const Slot t = stage[r];
-                    if (t.e >= 0) z += soft ? fast_exp(t.s - top) : mass_of(t.s, a.scoring);
-                }
-                z = group_reduce<S::G>(z, OpSum{});
-                // a division, so that a single expert's weight is 1 and its gradient 0
-                over = fabsf(z) < FLT_MIN ? __builtin_inff() : z;
-                scale = soft ? 1.0f + (inv - inv) : 1.0f;  // a row with NaN has no weights
-            }
-            const int64_t at = (row0 + n) * k;
-            for (int r = gl; r < k; r += S::G) {
-                const Slot t = stage[r];
-                if (in) {
-                    const float w = soft ? fast_exp(t.s - top) : mass_of(t.s, a.scoring);
-                    a.weights[at + r] = t.e >= 0 ? w * scale / over : 0.0f;
-                    a.experts[at + r] = t.e;
+                    if (in) {
+                        a.weights[at + r] = t.e < 0 ? 0.0f : mass(t.e, t.s) * scale / over;
+                        a.experts[at + r] = t.e;
+                    }
                 }
             }
             wave_lds_fence();  // the next rows write the slots again

@@ -206,3 +206,39 @@ def test_training_step_in_a_graph():
         between = step(*data[(i + 2) % 3])
         assert all(torch.equal(a, b) for a, b in zip(outs, eager[i]))
         assert all(torch.equal(a, b) for a, b in zip(between, eager[(i + 2) % 3]))
+
+
+def test_two_streams_at_once_and_no_gradients():
+    """Calls of two streams in flight together, and calls that record nothing, give the same bits."""
+    gen = torch.Generator().manual_seed(3)
+    data = [(torch.randn(2, 5000, 48, generator=gen).to(DEV), torch.randn(3, 40, 4000, generator=gen).bfloat16().to(DEV))
+            for _ in range(2)]
+    tokens = torch.randint(0, 4000, (3, 40), generator=gen).to(DEV)
+    plan = torch.rand(40, 80, generator=gen).to(DEV)
+
+    def step(scores, logits):
+        r = dot_amd.topk_routing(scores, 4, normalize=True)
+        per = dot_amd.sequence_logp(logits, tokens, reduction="none")
+        loss = dot_amd.preference_loss(per.reshape(-1), plan=plan)
+        return [x.detach() for x in (r.weights, r.experts, r.counts, r.balance_loss, per, loss)]
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = step(*data[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+    leaves = [x.clone().requires_grad_() for x in data[0]]
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(want[0], step(*leaves)))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(want[0], step(*leaves)))
+    # a second backward through one graph, and an unused output
+    r = dot_amd.topk_routing(leaves[0], 4)
+    (a,) = torch.autograd.grad(r.balance_loss.sum(), leaves[0], retain_graph=True)
+    (b,) = torch.autograd.grad(r.balance_loss.sum(), leaves[0])
+    assert torch.equal(a, b) and not r.experts.requires_grad and not r.counts.requires_grad
