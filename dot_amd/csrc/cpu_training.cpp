@@ -386,8 +386,10 @@ Tensor preference_forward_cpu(Tensor ratio_, optional<Tensor> plan_, int64_t typ
         double sum = 0.0;
         if (!s.plan.defined()) sum = f(double(r[i]) - r[s.P + i]).first;
         else
-            for (int64_t j = 0; j < s.Q; ++j)
-                sum += s.plan.const_data_ptr<float>()[i * s.Q + j] * f(double(r[i]) - r[s.P + j]).first;
+            for (int64_t j = 0; j < s.Q; ++j) {
+                const double x = s.plan.const_data_ptr<float>()[i * s.Q + j];
+                if (x != 0.0) sum += x * f(double(r[i]) - r[s.P + j]).first;  // 0 leaves the pair out
+            }
         loss.data_ptr<float>()[i] = float(sum);
     }
     return loss;
@@ -406,10 +408,11 @@ std::vector<Tensor> preference_backward_cpu(Tensor ratio_, optional<Tensor> plan
         const double g = gl.const_data_ptr<float>()[i];
         for (int64_t j = s.plan.defined() ? 0 : i; j < (s.plan.defined() ? s.Q : i + 1); ++j) {
             const auto [v, slope] = f(double(r[i]) - r[s.P + j]);
-            const double pull = g * slope * (s.plan.defined() ? double(s.plan.const_data_ptr<float>()[i * s.Q + j]) : 1.0);
+            const double x = s.plan.defined() ? double(s.plan.const_data_ptr<float>()[i * s.Q + j]) : 1.0;
+            const double pull = x == 0.0 ? 0.0 : g * slope * x;
             acc[size_t(i)] += pull;
             acc[size_t(s.P + j)] -= pull;
-            if (grad_plan.numel()) grad_plan.data_ptr<float>()[i * s.Q + j] = float(g * v);
+            if (grad_plan.numel()) grad_plan.data_ptr<float>()[i * s.Q + j] = x == 0.0 && !(v < kInf) ? 0.0f : float(g * v);
         }
     }
     Tensor grad_ratio = at::empty_like(s.ratio);

@@ -6,7 +6,8 @@
 // once more, writes f as its gradient and adds up plan f' along rows and
 // columns: a workgroup takes a strip of rows of kCols columns, keeps the
 // column sums of its strip in registers and writes one partial row of them;
-// `fold` adds the partials in strip order.
+// `fold` adds the partials in strip order.  An entry of 0 leaves its pair out,
+// whatever their ratios.
 #pragma once
 
 #include <type_traits>
@@ -143,7 +144,9 @@ __global__ __launch_bounds__(kBlock) void plan_forward(const float* ratio, const
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
             const int c = column<VEC>(c0, v);
-            if (VEC || c < Q) sum = fmaf(x[v], loss_of<TYPE, false>(l, ri - ratio[P + c], slope), sum);
+            if (!VEC && c >= Q) continue;
+            const float f = loss_of<TYPE, false>(l, ri - ratio[P + c], slope);
+            sum = x[v] != 0.0f ? fmaf(x[v], f, sum) : sum;
         }
     }
     sum = block_reduce<kWavesPerBlock>(wave_sum(sum), sm, OpSum{});
@@ -182,13 +185,25 @@ __global__ __launch_bounds__(kBlock) void plan_backward(PlanBwd a) {
         const float ri = a.ratio[i], g = a.grad[a.grad_scalar ? 0 : i];
         float sum = 0.0f;
         if (some) {
-            float x[kVec], f[kVec], slope;
+            float x[kVec], f[kVec], slope[kVec], all = 1.0f;
             load4<VEC>(a.plan + int64_t(i) * a.Q, c0, a.Q, x);
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                if (!VEC && column<VEC>(c0, v) >= a.Q) continue;
-                f[v] = g * loss_of<TYPE, true>(a.l, ri - rj[v], slope);
-                const float pull = g * x[v] * slope;
+                f[v] = loss_of<TYPE, true>(a.l, ri - rj[v], slope[v]);
+                all *= x[v];
+            }
+            if (!(all > 0.0f)) {  // perhaps pairs that are left out
+#pragma unroll
+                for (int v = 0; v < kVec; ++v) {
+                    if (x[v] != 0.0f) continue;
+                    f[v] = f[v] < __builtin_inff() ? f[v] : 0.0f;
+                    slope[v] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) {
+                f[v] *= g;
+                const float pull = g * x[v] * slope[v];
                 sum += pull;
                 col[v] += pull;
             }

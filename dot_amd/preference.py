@@ -110,7 +110,9 @@ def preference_loss(
         log_ratio: (P + Q,) log ratios (:func:`sequence_logp`), first of the P preferred,
             then of the Q other answers; floating point, computed in fp32
         plan: Optional (P, Q) coupling of the two sets, such as the ``transport_plan``
-            of :func:`sinkhorn`; without it answer i is paired with answer P + i (P = Q)
+            of :func:`sinkhorn`; without it answer i is paired with answer P + i (P = Q).
+            An entry of 0 leaves its pair out, whatever their ratios (a padded answer
+            has a row or a column of 0); its own gradient is ``f`` where that is finite.
         beta: Scale (> 0)
         loss_type: ``"sigmoid"``, ``"hinge"`` or ``"square"``
         label_smoothing: In [0, 1), ``"sigmoid"`` only

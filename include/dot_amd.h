@@ -499,7 +499,8 @@ typedef struct {
 } dot_preference_fwd_args;
 
 /* f(d) = (1 - smoothing) log(1 + exp(-beta d)) + smoothing log(1 + exp(beta d)),
- * max(0, 1 - beta d), or (d - 1 / (2 beta))^2. */
+ * max(0, 1 - beta d), or (d - 1 / (2 beta))^2.  A plan entry of 0 leaves its pair
+ * out, whatever their ratios. */
 int dot_preference_forward(const dot_preference_fwd_args* args, dot_stream_t stream);
 
 typedef struct {
@@ -512,7 +513,7 @@ typedef struct {
     const float* grad_loss;    /* [P]; one value with grad_loss_scalar */
     int grad_loss_scalar;
     float* grad_ratio;         /* [P+Q] out */
-    float* grad_plan;          /* [P,Q] out, or NULL */
+    float* grad_plan;          /* [P,Q] out, or NULL; 0 where the entry is 0 and f not finite */
     void* workspace;
     size_t workspace_bytes;
 } dot_preference_bwd_args;

@@ -171,5 +171,7 @@ def preference(ratio, plan=None, beta=0.1, loss_type="sigmoid", smoothing=0.0, g
     if plan is None:
         return f, np.concatenate([g * slope, -g * slope]), None
     plan = np.asarray(plan, np.float64)
-    pull = plan * slope * g[:, None]
-    return (plan * f).sum(1), np.concatenate([pull.sum(1), -pull.sum(0)]), f * g[:, None]
+    out = plan == 0  # leaves the pair out
+    pull = plan * np.where(out, 0.0, slope) * g[:, None]
+    own = np.where(out & ~(f < np.inf), 0.0, f) * g[:, None]
+    return (plan * np.where(out, 0.0, f)).sum(1), np.concatenate([pull.sum(1), -pull.sum(0)]), own

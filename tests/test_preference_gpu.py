@@ -80,6 +80,29 @@ def test_far_ratios():
         assert torch.isnan(dot_amd.preference_loss(nan, loss_type=loss_type)).tolist() == [True, False]
 
 
+@pytest.mark.parametrize("loss_type,smoothing", LOSSES)
+@pytest.mark.parametrize("P,Q", [(7, 12), (40, 1030)])
+def test_pairs_left_out(P, Q, loss_type, smoothing):
+    """Answers without a share of the plan may hold anything."""
+    rng = np.random.default_rng(P)
+    ratio = rng.standard_normal(P + Q).astype(np.float32)
+    plan = rng.random((P, Q)).astype(np.float32) / P
+    clean = ratio.copy()
+    for at, value in ((1, np.nan), (3, np.inf), (5, -np.inf)):
+        ratio[at] = ratio[P + at] = value
+        clean[at] = clean[P + at] = 0.0
+        plan[at] = 0.0
+        plan[:, at] = 0.0
+    with np.errstate(invalid="ignore"):
+        loss, (g, gp) = check(ratio, plan, beta=0.3, loss_type=loss_type, smoothing=smoothing)
+    want, (gc, _) = check(clean, plan, beta=0.3, loss_type=loss_type, smoothing=smoothing)
+    assert torch.equal(loss, want) and torch.equal(g, gc)
+    assert torch.isfinite(gp).all() and (loss[[1, 3, 5]] == 0).all()
+    # weights of any size beside the ones left out
+    check(ratio, np.where(plan == 0, 0, 1e30 * plan).astype(np.float32), beta=0.3, loss_type=loss_type,
+          smoothing=smoothing)
+
+
 def test_types_and_layouts():
     rng = np.random.default_rng(1)
     ratio = torch.as_tensor(rng.standard_normal(20).astype(np.float32)).to(DEV)

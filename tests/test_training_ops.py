@@ -146,6 +146,14 @@ def test_cpu_preference(loss_type, smoothing):
         assert pl is None or rel_err(grads[1], gp) < TOL
 
 
+def test_cpu_pairs_left_out():
+    ratio = torch.tensor([1.0, float("nan"), 0.5, float("-inf")], requires_grad=True)
+    plan = torch.tensor([[0.5, 0.0], [0.0, 0.0]], requires_grad=True)
+    loss = dot_amd.preference_loss(ratio, plan=plan)
+    g, gp = torch.autograd.grad(loss.sum(), [ratio, plan])
+    assert torch.isfinite(loss).all() and loss[1] == 0 and torch.isfinite(g).all() and torch.isfinite(gp).all()
+
+
 def test_cpu_empty():
     r = dot_amd.topk_routing(torch.zeros(2, 0, 4), 2)
     assert r.weights.shape == (2, 0, 2) and (r.balance_loss == 0).all()
