@@ -3,8 +3,6 @@
 // a shift; writing rounds to nearest even (the hardware conversion of gfx950).
 #pragma once
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -47,7 +45,7 @@ struct Pack {
     T v[N];
 };
 
-// 16-byte load and store of a pack; the address is 16-byte aligned.
+// 16-byte load of a pack; the address is 16-byte aligned.
 template <class T>
 __device__ __forceinline__ Pack<T> load_pack(const T* p) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -59,12 +57,7 @@ __device__ __forceinline__ Pack<T> load_pack_stream(const T* p) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(Pack<T>, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
 }
-template <class T>
-__device__ __forceinline__ void store_pack(T* p, const Pack<T>& x) {
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<u4*>(p) = __builtin_bit_cast(u4, x);
-}
-// As store_pack, for outputs that nothing reads back soon.
+// 16-byte store of a pack that nothing reads back soon.
 template <class T>
 __device__ __forceinline__ void store_pack_stream(T* p, const Pack<T>& x) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
