@@ -765,26 +765,34 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
             for (int j = 0; j < S::EL; ++j) add[j] = spread[S::expert(gl, j)];
             wave_lds_fence();
         }
+        // The gradient takes the place of the shares.
         float ph = 0.0f;
-        const bool in_h = soft && !a.normalize;  // the weights are p itself
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) {
-            const float h = slope[j] + (in_h ? add[j] : 0.0f);
-            ph = fmaf(q[j] * inv, h, ph);
-        }
-        ph = group_reduce<S::G>(ph, OpSum{});
-        float g[S::EL];
+        for (int j = 0; j < S::EL; ++j) q[j] *= inv;
+        if (WEIGHTS && soft && !a.normalize) {  // the weights are p itself: add belongs to h
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) {
-            if (soft) {
-                const float h = slope[j] + (in_h ? add[j] : 0.0f);
-                g[j] = fmaf(q[j] * inv, h - ph, in_h ? 0.0f : add[j]);
-            } else {
-                g[j] = fmaf(slope[j] - ph, inv, add[j]) * x[j];
+            for (int j = 0; j < S::EL; ++j) {
+                add[j] += slope[j];
+                ph = fmaf(q[j], add[j], ph);
             }
-            g[j] = live ? g[j] : 0.0f;
+            ph = group_reduce<S::G>(ph, OpSum{});
+#pragma unroll
+            for (int j = 0; j < S::EL; ++j) q[j] *= add[j] - ph;
+        } else {
+#pragma unroll
+            for (int j = 0; j < S::EL; ++j) ph = fmaf(q[j], slope[j], ph);
+            ph = group_reduce<S::G>(ph, OpSum{});
+            if (soft) {
+#pragma unroll
+                for (int j = 0; j < S::EL; ++j) q[j] = fmaf(q[j], slope[j] - ph, add[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < S::EL; ++j) q[j] = fmaf(slope[j] - ph, inv, add[j]) * x[j];
+            }
         }
-        if (in) store_row<T, S>(static_cast<T*>(a.grad_scores) + at * E, gl, E, g);
+#pragma unroll
+        for (int j = 0; j < S::EL; ++j) q[j] = live ? q[j] : 0.0f;
+        if (in) store_row<T, S>(static_cast<T*>(a.grad_scores) + at * E, gl, E, q);
     }
 }
 
