@@ -151,7 +151,8 @@ def preference(ratio, plan=None, beta=0.1, loss_type="sigmoid", smoothing=0.0, g
     """-> (loss (P,), grad_ratio, grad_plan); gradients of sum(loss grad)."""
     r = np.asarray(ratio, np.float64)
     P = len(r) // 2 if plan is None else len(plan)
-    gap = r[:P] - r[P:] if plan is None else r[:P, None] - r[None, P:]
+    with np.errstate(invalid="ignore"):
+        gap = r[:P] - r[P:] if plan is None else r[:P, None] - r[None, P:]
     d = beta * gap
     if loss_type == "sigmoid":
         t = _exp(-np.abs(d))
