@@ -8,6 +8,7 @@
 // by the host's work, and a node that runs without the interpreter takes less
 // of it.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/core/dispatch/Dispatcher.h>
@@ -357,6 +358,13 @@ using torch::autograd::variable_list;
 bool records(const Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
 bool records(const optional<Tensor>& x) { return x.has_value() && records(*x); }
 
+// A tangent of forward-mode differentiation would be dropped below autograd, so
+// that the derivative came out as zero: an error instead.
+void check_no_tangent(const Tensor& x) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !x._fw_grad(0).defined(),
+                                "dot_amd operators have no forward-mode derivative");
+}
+
 // The gradient of an operator that has no second derivative: a backward
 // through it is an error, not a wrong result.
 Tensor once(const Tensor& grad) {
@@ -416,6 +424,7 @@ struct RoutingFunction : torch::autograd::Function<RoutingFunction> {
 
 std::vector<Tensor> routing_forward_autograd(Tensor scores, int64_t k, int64_t scoring, bool normalize,
                                              optional<Tensor> bias, optional<Tensor> mask, optional<Tensor> given) {
+    check_no_tangent(scores);
     if (!records(scores)) return call_routing(scores, k, scoring, normalize, bias, mask, given);
     return RoutingFunction::apply(scores, k, scoring, normalize, bias, mask, given);
 }
@@ -454,6 +463,7 @@ struct SequenceLogpFunction : torch::autograd::Function<SequenceLogpFunction> {
 
 std::vector<Tensor> sequence_logp_forward_autograd(Tensor logits, Tensor tokens, optional<Tensor> ref,
                                                    optional<Tensor> mask, double tau, int64_t reduction, bool keep) {
+    check_no_tangent(logits);
     if (!records(logits)) return call_sequence_logp(logits, tokens, ref, mask, tau, reduction, keep);
     return SequenceLogpFunction::apply(logits, tokens, ref, mask, tau, reduction);
 }
@@ -493,6 +503,8 @@ struct PreferenceFunction : torch::autograd::Function<PreferenceFunction> {
 };
 
 Tensor preference_forward_autograd(Tensor ratio, optional<Tensor> plan, int64_t type, double beta, double smoothing) {
+    check_no_tangent(ratio);
+    if (plan.has_value()) check_no_tangent(*plan);
     if (!records(ratio) && !records(plan)) return call_preference(ratio, plan, type, beta, smoothing);
     return PreferenceFunction::apply(ratio, plan, type, beta, smoothing);
 }
