@@ -14,6 +14,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -366,12 +367,17 @@ void check_no_tangent(const Tensor& x) {
 }
 
 // The gradient of an operator that has no second derivative: a backward
-// through it is an error, not a wrong result.
-Tensor once(const Tensor& grad) {
+// through it is an error, not a wrong result.  The error's node leads on to all
+// that the gradient is a function of (the inputs and the upstream gradients):
+// the engine runs only nodes on a way to what it is asked for.
+Tensor once(const Tensor& grad, const variable_list& of) {
     if (!at::GradMode::is_enabled() || !grad.defined()) return grad;
-    auto refuse = std::make_shared<torch::autograd::DelayedError>(
-        "dot_amd operators are differentiable once: no gradient flows through their backward", 1);
-    return (*refuse)({grad})[0];
+    auto refuse = std::make_shared<torch::autograd::Error>(
+        "dot_amd operators are differentiable once: no gradient flows through their backward",
+        torch::autograd::collect_next_edges(of));
+    Tensor out = grad.detach();
+    torch::autograd::set_history(out, refuse);
+    return out;
 }
 
 template <class F>
@@ -418,7 +424,7 @@ struct RoutingFunction : torch::autograd::Function<RoutingFunction> {
                         gw.defined() ? maybe(s[4]) : c10::nullopt, gw.defined() ? maybe(s[5]) : c10::nullopt,
                         maybe(gw));
         }
-        return {once(g), {}, {}, {}, {}, {}, {}};
+        return {once(g, {s[0], gl, gw}), {}, {}, {}, {}, {}, {}};
     }
 };
 
@@ -457,7 +463,7 @@ struct SequenceLogpFunction : torch::autograd::Function<SequenceLogpFunction> {
             g = op.call(s[0], s[1], maybe(s[2]), ctx->saved_data["tau"].toDouble(),
                         ctx->saved_data["reduction"].toInt(), s[3], grads[0]);
         }
-        return {once(g), {}, {}, {}, {}, {}};
+        return {once(g, {s[0], grads[0]}), {}, {}, {}, {}, {}};
     }
 };
 
@@ -498,7 +504,8 @@ struct PreferenceFunction : torch::autograd::Function<PreferenceFunction> {
             gr = g[0].to(s[0].scalar_type());
             if (want_plan) gp = g[1].to(s[1].scalar_type());
         }
-        return {once(gr), once(gp), {}, {}, {}};
+        const variable_list of{s[0], s[1], grads[0]};
+        return {once(gr, of), once(gp, of), {}, {}, {}};
     }
 };
 

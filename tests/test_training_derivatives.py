@@ -60,3 +60,43 @@ def test_constants_may_have_tangents(dev):
         assert fw.unpack_dual(r.weights).tangent is None and fw.unpack_dual(out).tangent is None
     assert torch.equal(r.weights, dot_amd.topk_routing(x, 2, bias=bias).weights)
     assert torch.equal(out, dot_amd.sequence_logp(x, tokens, ref_logp=ref))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("upstream", ["constant", "differentiable"])
+@pytest.mark.parametrize("name", NAMES)
+def test_second_order_is_refused(dev, upstream, name):
+    """A gradient that create_graph asks for can be used, but nothing flows through it unnoticed."""
+    f, x = operators(dev)[name]
+    x.requires_grad_()
+    out = f(x)
+    loss = out.sum() if upstream == "constant" else (out * out).sum()
+    (g,) = torch.autograd.grad(loss, x, create_graph=True)
+    assert g.requires_grad
+    (plain,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert not plain.requires_grad and torch.equal(g, plain)
+    for total in (g.sum(), loss + (g**2).sum()):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(total, x, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(loss, x, retain_graph=True)[0], plain)
+    up = torch.ones_like(out).requires_grad_()  # nor to the upstream gradient, in which g is linear
+    (g,) = torch.autograd.grad(out, x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(g.sum(), up)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_order_of_both_inputs_is_refused(dev):
+    gen = torch.Generator().manual_seed(2)
+    ratio = torch.randn(8, generator=gen).to(dev).requires_grad_()
+    plan = torch.rand(3, 5, generator=gen).to(dev).requires_grad_()
+    loss = dot_amd.preference_loss(ratio, plan=plan).sum()
+    for g in torch.autograd.grad(loss, [ratio, plan], create_graph=True):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum(), [ratio, plan], retain_graph=True, allow_unused=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.functional.hessian(lambda r: dot_amd.preference_loss(r).sum(), ratio.detach())
+    # leaves take the gradient of a graph that is kept
+    loss.backward(create_graph=True)
+    assert ratio.grad.requires_grad and plan.grad.requires_grad
+    ratio.grad = plan.grad = None
