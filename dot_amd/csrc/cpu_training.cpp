@@ -57,6 +57,16 @@ const bool* mask_ptr(const Tensor& m) { return m.defined() ? m.const_data_ptr<bo
 
 double logistic(double x) { return x >= 0 ? 1.0 / (1.0 + std::exp(-x)) : std::exp(x) / (1.0 + std::exp(x)); }
 
+// Masses whose sum is below the smallest normal fp32 count as none (the device
+// forms the reciprocal in fp32), and so does the logistic mass of a single score
+// (the device's exponential ends there); NaN stays NaN.
+bool none(double mass) { return std::fabs(mass) < double(std::numeric_limits<float>::min()); }
+
+double logistic_mass(double x) {
+    const double q = logistic(x);
+    return none(q) ? 0.0 : q;
+}
+
 // Masses of a row of E scores; returns their sum (softmax: q sums to 1, or to 0
 // where every score is -inf).
 double row_masses(const float* s, int64_t E, int64_t scoring, double* q) {
@@ -70,7 +80,7 @@ double row_masses(const float* s, int64_t E, int64_t scoring, double* q) {
         return sum == 0.0 ? 0.0 : sum / sum;
     }
     for (int64_t e = 0; e < E; ++e) {
-        q[e] = scoring == DOT_SCORING_SIGMOID ? logistic(s[e]) : double(s[e]) == -kInf ? 0.0 : double(s[e]);
+        q[e] = scoring == DOT_SCORING_SIGMOID ? logistic_mass(s[e]) : double(s[e]) == -kInf ? 0.0 : double(s[e]);
         sum += q[e];
     }
     return sum;
@@ -135,7 +145,7 @@ std::vector<Tensor> routing_forward_cpu(Tensor scores_, int64_t k, int64_t scori
                 }
                 for (int64_t i = 0; i < have; ++i) {
                     ep[r * k + i] = keys[size_t(i)].second;
-                    wp[r * k + i] = float(!normalize ? w[i] : z == 0.0 ? 0.0 : w[i] / z);
+                    wp[r * k + i] = float(!normalize ? w[i] : none(z) ? 0.0 : w[i] / z);
                 }
             }
         });
@@ -156,7 +166,7 @@ std::vector<Tensor> routing_forward_cpu(Tensor scores_, int64_t k, int64_t scori
                     if (e >= 0 && e < E) ++cp[b * E + e];
                 }
                 const double sum = row_masses(sp + r * E, E, scoring, q.data());
-                if (sum == 0.0) continue;
+                if (none(sum)) continue;
                 for (int64_t e = 0; e < E; ++e) share[size_t(e)] += q[size_t(e)] / sum;
             }
             double dot = 0.0;
@@ -223,19 +233,19 @@ Tensor routing_backward_cpu(Tensor scores_, int64_t k, int64_t scoring, bool nor
                 for (int64_t i = 0; i < k; ++i) {
                     if (ep[i] < 0 || ep[i] >= E) continue;
                     double v = dp[i];
-                    if (normalize) v = soft ? wp[i] * (v - dot) : mass == 0.0 ? 0.0 : (v - dot) / mass;
+                    if (normalize) v = soft ? wp[i] * (v - dot) : none(mass) ? 0.0 : (v - dot) / mass;
                     if (soft && !normalize) h[size_t(ep[i])] += v;
                     else add[size_t(ep[i])] = v;
                 }
             }
-            const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+            const double inv = none(sum) ? 0.0 : 1.0 / sum;
             double ph = 0.0;
             for (int64_t e = 0; e < E; ++e) ph += q[size_t(e)] * inv * h[size_t(e)];
             for (int64_t e = 0; e < E; ++e) {
                 double g = (h[size_t(e)] - ph) * (soft ? q[size_t(e)] : inv) + add[size_t(e)];
                 if (scoring == DOT_SCORING_SIGMOID) {
                     const double t = std::exp(-std::fabs(double(s[e])));
-                    g *= t / ((1.0 + t) * (1.0 + t));
+                    g *= none(t) ? 0.0 : t / ((1.0 + t) * (1.0 + t));
                 }
                 out[r * E + e] = float(g);
             }

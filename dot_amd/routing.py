@@ -98,7 +98,9 @@ def topk_routing(
     Experts are ordered by ``score + bias`` in fp32, equal ones by the lowest index.
     One is available where that is above -inf (and, with ``"plan"``, its mass above
     0); a token with fewer than ``k`` has empty slots.  Masses that sum to less than
-    the smallest normal fp32 count as none.  A NaN score is never
+    the smallest normal fp32 (1.2e-38) count as none, a token's own as well as those
+    of its experts that ``normalize`` divides by: their weights and shares are 0, and so
+    is the gradient through them.  A sigmoid mass below that is 0.  A NaN score is never
     selected; its token's softmax weights and the loss are NaN.
 
     Gradients reach ``scores`` from ``weights`` and ``balance_loss``.

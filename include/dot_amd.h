@@ -407,7 +407,9 @@ typedef struct {
  * order, equal keys by the lowest index; an expert is available where its key
  * is above -inf (and, with DOT_SCORING_PLAN, its score above 0).  Weights are
  * the masses q of the selected experts.  A masked token gets experts of -1 and
- * weights of 0. */
+ * weights of 0.  Masses that sum to less than the smallest normal fp32 (a token's,
+ * or those that normalize divides by) count as none: weights, shares and the
+ * gradient through them are 0. */
 size_t dot_routing_forward_workspace_bytes(int B, int N, int E);
 int dot_routing_forward(const dot_routing_fwd_args* args, dot_stream_t stream);
 

@@ -26,10 +26,16 @@ def _masses(s, scoring):
         return q, q.sum(-1, keepdims=True), None
     if scoring == "sigmoid":
         t = _exp(-np.abs(s))
+        t = np.where(t < np.finfo(np.float32).tiny, 0.0, t)  # counts as none, as such sums do
         q = np.where(s < 0, t, 1.0) / (1 + t)
         return q, q.sum(-1, keepdims=True), t / (1 + t) ** 2
     q = np.where(s == -np.inf, 0.0, s)
     return q, q.sum(-1, keepdims=True), np.ones_like(s)
+
+
+def _none(mass):
+    """Whether masses sum to less than the smallest normal fp32, and so count as none."""
+    return abs(mass) < np.finfo(np.float32).tiny
 
 
 def route(scores, k, scoring="softmax", normalize=False, bias=None, mask=None, given=None):
@@ -58,13 +64,13 @@ def route(scores, k, scoring="softmax", normalize=False, bias=None, mask=None, g
                     else:
                         w = q[took]
                     if normalize:
-                        w = w / w.sum() if w.sum() != 0 else 0.0 * w
+                        w = 0.0 * w if _none(w.sum()) else w / w.sum()
                     out["weights"][b, n, :len(took)] = w
                     out["experts"][b, n, :len(took)] = took
             else:
                 took = [e for e in given[b, n] if 0 <= e < E]
             np.add.at(out["counts"][b], np.asarray(took, dtype=np.int64), 1)
-            if total[0] != 0:
+            if not _none(total[0]):
                 share += q / total
         n_b = out["tokens"][b]
         if n_b:
@@ -93,16 +99,16 @@ def route_grad(scores, k, fwd, scoring="softmax", normalize=False, mask=None, gr
                 if normalize:
                     dw = dw - (w * dw).sum()
                     mass = q[at].sum()
-                    add[at] = w * dw if scoring == "softmax" else dw / mass if mass else 0.0
+                    add[at] = w * dw if scoring == "softmax" else 0.0 if _none(mass) else dw / mass
                 elif scoring == "softmax":
                     h[at] += dw
                 else:
                     add[at] = dw
-            p = q / total if total[0] != 0 else 0.0 * q
+            p = 0.0 * q if _none(total[0]) else q / total
             if scoring == "softmax":
                 out[b, n] = p * (h - (p * h).sum()) + add
             else:
-                back = (h - (p * h).sum()) / total if total[0] != 0 else 0.0
+                back = 0.0 if _none(total[0]) else (h - (p * h).sum()) / total
                 out[b, n] = slope * (back + add)
     return out
 
