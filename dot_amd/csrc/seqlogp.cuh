@@ -11,7 +11,10 @@
 // models is a small difference of large sums.  x - m is formed before the
 // scale, so rows at the type's lowest value give finite statistics.  The
 // backward reads the row again and writes dx_v = c (delta_va - p_v) with
-// p_v = 2^((x_v - m) k) / s.  Rows that are left out are not read.
+// p_v = 2^((x_v - m) k) / s.  Where the token a is likelier than not, 1 - p_a
+// is kept as the others' share of the sum, formed in 64 bits: as a difference it
+// would lose the digits that the forward keeps.  Rows that are left out are not
+// read.
 #pragma once
 
 #include "elem.cuh"
@@ -160,12 +163,19 @@ __device__ __forceinline__ Own own_of(const Rows& r, const JoinArgs& j, int64_t 
 }
 
 // The value of a position from the statistics of its row's other logits.  Those
-// of the whole row are kept for the backward.
+// of the whole row are kept for the backward: the largest logit m, and 1 / s; or,
+// where the token's share is above 1/2 (it is the largest then, its term is 1),
+// -(1 - p_a) = -(s - 1) / s, from which 1 / s = p_a follows.
 __device__ __forceinline__ double position(const Rows& r, const JoinArgs& j, int64_t at, const Own& own, MaxSum t) {
     const double kn = (double(r.k) + double(r.klo)) * 0.693147180559945309417;  // 1 / tau
+    const MaxSum others = t;
     t.join(own.x, 1.0, r);
     const float base = t.base();
-    if (j.stats) j.stats[at] = make_float2(base, float(1.0 / t.s));
+    if (j.stats) {
+        const double rest = others.s * double(__builtin_amdgcn_exp2f(scaled(r, others.m - base)));
+        const bool likely = own.x == base && t.s < 2.0;  // not NaN
+        j.stats[at] = make_float2(base, likely ? -float(rest / t.s) : float(1.0 / t.s));
+    }
     return (double(own.x) - double(base)) * kn - log(t.s) - own.ref;
 }
 
@@ -346,10 +356,12 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     const float2 st = g.stats[at];
     const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
     const float c = (g.reduction == DOT_REDUCE_MEAN ? up * g.weight[b] : up) * g.inv_tau;
-    const float scale = -c * st.y;
+    const bool likely = __builtin_bit_cast(int, st.y) < 0;  // -(1 - p_a), -0 among them
+    const float scale = -c * (likely ? 1.0f + st.y : st.y);
+    const float taken = likely ? c * -st.y : c, with = likely ? 0.0f : 1.0f;
     auto value = [&](float x, int v) {
         const float y = __builtin_amdgcn_exp2f(scaled(r, x - st.x)) * scale;
-        return v == tok ? c + y : y;
+        return v == tok ? fmaf(with, y, taken) : y;
     };
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     const Span sp = span_of(out, r.V, part, r.splits);

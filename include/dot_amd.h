@@ -454,7 +454,8 @@ typedef struct {
     int reduction;             /* DOT_REDUCE_* over the positions that are not left out */
     float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
     float* row_stats;          /* [B,S,2] out, for the backward: the row's max and
-                                  1 / sum exp((x - max) / tau); not written where left out */
+                                  1 / sum exp((x - max) / tau), or p - 1 where the token's probability p
+                                  is above 1/2; not written where left out */
     float* weight;             /* [B] out with DOT_REDUCE_MEAN, for the backward: 1 / positions */
     void* workspace;
     size_t workspace_bytes;

@@ -1,6 +1,7 @@
 """Digits of the routing, sequence log-probability and preference operators on the
 device, element by element against the float64 definition."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -8,12 +9,62 @@ import dot_amd
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
+DTYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 
 
 def half_step(dtype):
     """Relative, and absolute for results that are subnormal."""
     info = torch.finfo(dtype)
     return info.eps / 2, float(info.smallest_normal) * info.eps / 2
+
+
+def taken_rows(rng, V, dtype):
+    """(2, 12, V) logits: tokens from unlikely over even chances to nearly certain, and certain ones."""
+    x = torch.as_tensor(rng.standard_normal((2, 12, V)).astype(np.float32))
+    tokens = rng.integers(0, V, (2, 12))
+    rest = float(np.log(max(V - 1, 1)) + 0.5)  # about the log of the others' sum
+    for s in range(12):
+        at = torch.as_tensor(tokens[:, s])[:, None]
+        x[:, s].scatter_(1, at, rest + (-6.0, -1.0, -0.1, 0.0, 0.1, 1.0, 4.0, 8.0, 12.0, 16.0, 24.0, 0.0)[s])
+    others = torch.ones(2, V, dtype=torch.bool).scatter_(1, torch.as_tensor(tokens[:, 11])[:, None], False)
+    x[:, 11][others] = -float("inf")
+    x[:, 3, :] = 1.5  # the same chance for all
+    return x.to(dtype), tokens
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("V", [1, 2, 8, 100, 4099, 40000, 131072])
+def test_gradient_of_likely_tokens_keeps_its_digits(dtype, V):
+    """dx of the taken token is c (1 - p): others / total, where the sum of the others is good to 1e-6 of itself (each
+    term to 2^-22, partial sums to 2^-21) and 1 - p, the reciprocal, c and their product add 2^-24 each; a p of at most
+    1/2 is good to 2e-6 of itself.  dx of the others is c p.  A logit d tau below the largest is off by d 2^-24 for the
+    difference, as much for its product with log2(e) / tau, and 2^-22 for the exponential, c and their product; the sum
+    by 2^-20: d 2^-23 + 2^-22 + 2^-20 of itself.  Each to half a step of its type."""
+    print(f"[taken] {dtype} V={V}", flush=True)
+    rng = np.random.default_rng(V)
+    logits, tokens = taken_rows(rng, V, DTYPES[dtype])
+    half, tiny = half_step(DTYPES[dtype])
+    for tau, reduction in ((1.0, "none"), (0.7, "sum"), (1.3, "mean")):
+        x = logits.to(DEV).requires_grad_()
+        out = dot_amd.sequence_logp(x, torch.as_tensor(tokens).to(DEV), tau=tau, reduction=reduction)
+        up = rng.uniform(0.5, 2.0, tuple(out.shape)).astype(np.float32)
+        (g,) = torch.autograd.grad([out], [x], [torch.as_tensor(up).to(DEV)])
+        z = logits.double() / tau
+        at = torch.as_tensor(tokens)[..., None]
+        own = z.gather(2, at)
+        c = torch.as_tensor(up).double() / tau / (12 if reduction == "mean" else 1)
+        c = c[..., None] if reduction == "none" else c[:, None, None]
+        rest = torch.logsumexp(z.scatter(2, at, -float("inf")), -1, keepdim=True)
+        total = torch.logaddexp(own, rest)
+        want = -c * torch.exp(z - total)
+        want.scatter_(2, at, c * torch.exp(rest - total))
+        err = (g.detach().cpu().double() - want).abs()
+        taken = torch.zeros_like(z, dtype=torch.bool).scatter_(2, at, True)
+        d = z.amax(-1, keepdim=True) - torch.where(z == -float("inf"), z.amax(-1, keepdim=True), z)
+        relative = half + torch.where(taken, 3e-6, d * 2.0**-23 + 2.0**-22 + 2.0**-20)
+        over = err - relative * want.abs() - tiny - (2.0**-126 if dtype == "fp32" else 0)  # flushed exponentials
+        assert (over <= 0).all(), [(m & (over > 0)).sum() for m in (taken, ~taken)]
+        assert (g[:, 11] == 0).all()
 
 
 def test_gradient_of_large_logits():
