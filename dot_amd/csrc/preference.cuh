@@ -28,6 +28,7 @@ constexpr int kFoldCols = 64;            // of as many columns (or rows)
 
 struct Loss {
     float beta, smoothing;
+    double whole;  // beta with all its digits
 };
 
 // The loss types of the kernels: those of the C ABI, and the sigmoid loss
@@ -59,14 +60,23 @@ __device__ __forceinline__ float log1p_unit(float e) {
     return fmaf(z2 * w, s, z2);
 }
 
-// f(gap) and, with SLOPE, df / dgap.
+// 1 - beta d in 64 bits, each operation rounded as the definition has it.
+__device__ __forceinline__ double room_of(double beta, double gap) {
+#pragma clang fp contract(off)
+    return 1.0 - beta * gap;
+}
+
+// f(x - y) and, with SLOPE, its derivative.
 template <int TYPE, bool SLOPE>
-__device__ __forceinline__ float loss_of(const Loss& l, float gap, float& slope) {
+__device__ __forceinline__ float loss_of(const Loss& l, float x, float y, float& slope) {
+    const float gap = x - y;
     if constexpr (TYPE == DOT_PREFER_HINGE) {
-        const float room = fmaf(-l.beta, gap, 1.0f);
-        const bool shut = room <= 0.0f;  // not NaN
-        if (SLOPE) slope = shut ? 0.0f : room == room ? -l.beta : room;
-        return shut ? 0.0f : room;
+        // The slope jumps where the room is 0: a difference or a beta rounded to
+        // 32 bits would take a pair within 1e-7 of it to the other side.
+        const double room = room_of(l.whole, double(x) - double(y));
+        const bool shut = room <= 0.0;  // not NaN
+        if (SLOPE) slope = shut ? 0.0f : room == room ? -l.beta : float(room);
+        return shut ? 0.0f : float(room);
     } else if constexpr (TYPE == DOT_PREFER_SQUARE) {
         const float miss = gap - 0.5f / l.beta;
         if (SLOPE) slope = 2.0f * miss;
@@ -92,7 +102,7 @@ template <int TYPE>
 __global__ __launch_bounds__(kBlock) void pairs_forward(const float* ratio, int P, Loss l, float* loss) {
     const int i = int(blockIdx.x) * kBlock + int(threadIdx.x);
     float slope;
-    if (i < P) loss[i] = loss_of<TYPE, false>(l, ratio[i] - ratio[P + i], slope);
+    if (i < P) loss[i] = loss_of<TYPE, false>(l, ratio[i], ratio[P + i], slope);
 }
 
 template <int TYPE>
@@ -101,7 +111,7 @@ __global__ __launch_bounds__(kBlock) void pairs_backward(const float* ratio, int
     const int i = int(blockIdx.x) * kBlock + int(threadIdx.x);
     if (i >= P) return;
     float slope;
-    loss_of<TYPE, true>(l, ratio[i] - ratio[P + i], slope);
+    loss_of<TYPE, true>(l, ratio[i], ratio[P + i], slope);
     const float g = grad[grad_scalar ? 0 : i] * slope;
     grad_ratio[i] = g;
     grad_ratio[P + i] = -g;
@@ -145,7 +155,7 @@ __global__ __launch_bounds__(kBlock) void plan_forward(const float* ratio, const
         for (int v = 0; v < kVec; ++v) {
             const int c = column<VEC>(c0, v);
             if (!VEC && c >= Q) continue;
-            const float f = loss_of<TYPE, false>(l, ri - ratio[P + c], slope);
+            const float f = loss_of<TYPE, false>(l, ri, ratio[P + c], slope);
             sum = x[v] != 0.0f ? fmaf(x[v], f, sum) : sum;
         }
     }
@@ -189,7 +199,7 @@ __global__ __launch_bounds__(kBlock) void plan_backward(PlanBwd a) {
             load4<VEC>(a.plan + int64_t(i) * a.Q, c0, a.Q, x);
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                f[v] = loss_of<TYPE, true>(a.l, ri - rj[v], slope[v]);
+                f[v] = loss_of<TYPE, true>(a.l, ri, rj[v], slope[v]);
                 all *= x[v];
             }
             if (!(all > 0.0f)) {  // perhaps pairs that are left out

@@ -23,6 +23,10 @@ int check_common(int P, int Q, bool has_plan, int type, float beta, float smooth
     return DOT_OK;
 }
 
+preference::Loss loss_of_args(float beta, int beta_tail, float smoothing) {
+    return {beta, smoothing, double(beta) + std::ldexp(double(beta_tail), std::ilogb(beta) - 53)};
+}
+
 struct BwdLayout {
     int strip, nstrips, ncols;
     float* colpart;
@@ -60,7 +64,7 @@ extern "C" int dot_preference_forward(const dot_preference_fwd_args* a, dot_stre
     if (int rc = check_common(a->P, a->Q, has_plan, a->loss_type, a->beta, a->smoothing)) return rc;
     if (a->P == 0) return ok();
     if (!a->ratio || !a->loss) return fail(DOT_ERR_INVALID_ARG, "ratio and loss must be non-NULL");
-    const preference::Loss l{a->beta, a->smoothing};
+    const preference::Loss l = loss_of_args(a->beta, a->beta_tail, a->smoothing);
     preference::dispatch_type(a->loss_type, a->smoothing, [&](auto type) {
         constexpr int T = decltype(type)::value;
         ProfScope prof(has_plan ? "preference_plan_forward" : "preference_pairs_forward", stream);
@@ -90,7 +94,7 @@ extern "C" int dot_preference_backward(const dot_preference_bwd_args* a, dot_str
     if (a->P == 0 && a->Q == 0) return ok();
     if (!a->ratio || (a->P > 0 && !a->grad_loss) || !a->grad_ratio)
         return fail(DOT_ERR_INVALID_ARG, "ratio, grad_loss and grad_ratio must be non-NULL");
-    const preference::Loss l{a->beta, a->smoothing};
+    const preference::Loss l = loss_of_args(a->beta, a->beta_tail, a->smoothing);
     if (!has_plan) {
         preference::dispatch_type(a->loss_type, a->smoothing, [&](auto type) {
             ProfScope prof("preference_pairs_backward", stream);

@@ -18,6 +18,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -307,6 +308,9 @@ void fill_preference(A& a, const Tensor& ratio, const Tensor& plan, int64_t type
     a.Q = to_int(Q, "Q");
     a.loss_type = int(type);
     a.beta = float(beta);
+    // what is left is a whole number of at most 2^29 units
+    if (std::isnormal(a.beta))
+        a.beta_tail = int(std::ldexp(beta - double(a.beta), 53 - std::ilogb(a.beta)));
     a.smoothing = float(smoothing);
 }
 

@@ -498,6 +498,8 @@ typedef struct {
     int loss_type;             /* DOT_PREFER_* */
     float beta;                /* > 0 */
     float smoothing;           /* in [0, 1), DOT_PREFER_SIGMOID only */
+    int beta_tail;             /* digits of beta beyond a float's, in units of 2^(ilogb(beta) - 53), 0 for none:
+                                  whether a hinge is open is decided in 64 bits */
     float* loss;               /* [P] out: sum_j plan_ij f(ratio_i - ratio_{P+j}), or f of pair i */
 } dot_preference_fwd_args;
 
@@ -513,6 +515,7 @@ typedef struct {
     int loss_type;
     float beta;
     float smoothing;
+    int beta_tail;
     const float* grad_loss;    /* [P]; one value with grad_loss_scalar */
     int grad_loss_scalar;
     float* grad_ratio;         /* [P+Q] out */

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import dot_amd
+from oracle import training as oracle
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -93,3 +94,34 @@ def test_gradient_of_large_logits():
         assert ((g[b, s].double() - want).abs() <= (half + 5e-6) * want.abs() + tiny).all(), (b, s)
     g[mask] = 0
     assert not g.any()
+
+
+@pytest.mark.parametrize("coupled", [False, True])
+@pytest.mark.parametrize("beta", [0.1, 0.05, 0.3, 1 / 3, 1.7, 64.0])
+def test_hinge_at_its_kink(coupled, beta):
+    """Gaps within a few fp32 steps of 1 / beta, and at 1 / beta itself: the loss is 0 or not, and the slope -beta or 0,
+    as in 64 bits.  The loss is rounded once (sums of 33 positive ones 2e-6), the slope to fp32."""
+    steps = np.arange(-16, 17)
+    low = (np.array([0.0, 1e-8, -1e-8, 1.0, 3.0, -7.0, 1e-3, 100.0])).astype(np.float32)
+    if not coupled:
+        high = (low[:, None].astype(np.float64) + 1 / beta).astype(np.float32)
+        high = (high + np.spacing(high) * steps).astype(np.float32)
+        ratio = np.concatenate([high.ravel(), np.repeat(low, len(steps))])
+        plan = None
+    else:
+        mid = np.float32(1 / beta)
+        high = (mid + np.spacing(mid) * steps).astype(np.float32)
+        ratio = np.concatenate([high, low[:3]])
+        plan = np.ones((len(high), 3), np.float32) / 4
+    r = torch.as_tensor(ratio).to(DEV).requires_grad_()
+    pl = None if plan is None else torch.as_tensor(plan).to(DEV).requires_grad_()
+    loss = dot_amd.preference_loss(r, plan=pl, beta=beta, loss_type="hinge")
+    o, gr, gp = oracle.preference(ratio, plan, beta, "hinge")
+    if not coupled:
+        assert (np.abs(loss.detach().cpu().double().numpy() - o) <= 2.0**-24 * o).all()
+    grads = torch.autograd.grad(loss.sum(), [r] + ([] if pl is None else [pl]))
+    got = grads[0].cpu().double().numpy()
+    assert np.array_equal(got != 0, gr != 0) and (np.abs(got - gr) <= 2e-6 * np.abs(gr)).all()
+    if coupled:
+        assert (np.abs(loss.detach().cpu().double().numpy() - o) <= 2e-6 * o).all()
+        assert (np.abs(grads[1].cpu().double().numpy() - gp) <= 2.0**-24 * gp).all()
