@@ -218,28 +218,36 @@ __device__ __forceinline__ void store_row(T* row, int gl, int E, const float (&x
     }
 }
 
-// t = exp(-|x|) and u = 1 / (1 + t), from which the logistic function and its
-// slope t u^2 follow without cancellation; NaN stays NaN.
-__device__ __forceinline__ void logistic_parts(float x, float& t, float& u) {
-    t = fast_exp(-fabsf(x));
-    u = __builtin_amdgcn_rcpf(1.0f + t);
+// e^x of x <= 0.  FULL: to 1.25 ulp; otherwise the argument's product is rounded
+// once, (|x| + 2) 2^-23 of the result.  Weights and fp32 gradients are results of
+// single tokens and take the former (backward of 65536 x 256 fp32: 34.5 us with
+// the short one, 35.0; the forward's weights no difference).
+template <bool FULL>
+__device__ __forceinline__ float exp_of(float x) {
+    if constexpr (FULL) return exp_compensated_below(x);
+    else return fast_exp(x);
 }
 
-__device__ __forceinline__ float logistic(float x) {
-    float t, u;
-    logistic_parts(x, t, u);
-    return x < 0.0f ? t * u : u;
+// t = exp(-|x|) and u = 1 / (1 + t), from which the logistic function and its
+// slope t u^2 follow without cancellation; NaN stays NaN.
+template <bool FULL>
+__device__ __forceinline__ void logistic_parts(float x, float& t, float& u) {
+    t = exp_of<FULL>(-fabsf(x));
+    u = __builtin_amdgcn_rcpf(1.0f + t);
 }
 
 // The mass of one score where it needs no row statistics.
 __device__ __forceinline__ float mass_of(float x, int scoring) {
-    return scoring == DOT_SCORING_SIGMOID ? logistic(x) : x == kNegInf ? 0.0f : x;
+    if (scoring != DOT_SCORING_SIGMOID) return x == kNegInf ? 0.0f : x;
+    float t, u;
+    logistic_parts<true>(x, t, u);
+    return x < 0.0f ? t * u : u;
 }
 
 // Masses q of a row (softmax: exp(x - top), not yet divided), and 1 / sum q
 // (0 where the row has no mass: below the smallest normal float; NaN stays NaN).  SLOPE: x becomes dq/dx of the
 // masses that need no row statistics.
-template <class S, bool SLOPE = false>
+template <class S, bool FULL, bool SLOPE>
 __device__ __forceinline__ void row_masses(float (&x)[S::EL], int scoring, float (&q)[S::EL], float& top,
                                            float& inv) {
     float sum = 0.0f;
@@ -251,12 +259,12 @@ __device__ __forceinline__ void row_masses(float (&x)[S::EL], int scoring, float
         m = unordered(group_reduce<S::G>(ordered(m), OpMaxInt{}));
         top = m == kNegInf ? 0.0f : m;
 #pragma unroll
-        for (int j = 0; j < S::EL; ++j) q[j] = fast_exp(x[j] - top);
+        for (int j = 0; j < S::EL; ++j) q[j] = exp_of<FULL>(x[j] - top);
     } else if (scoring == DOT_SCORING_SIGMOID) {
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) {
             float t, u;
-            logistic_parts(x[j], t, u);
+            logistic_parts<FULL>(x[j], t, u);
             q[j] = x[j] < 0.0f ? t * u : u;
             if (SLOPE) x[j] = t * u * u;  // q (1 - q), exact where q is near 1
         }
@@ -461,7 +469,9 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
         live_rows += raw.live && gl == 0;
         float x[S::EL], q[S::EL], top, inv;
         raw.get(gl, E, x);
-        row_masses<S>(x, a.scoring, q, top, inv);
+        // The shares are summed over many tokens into one fp32: the short exponential
+        // (65536 x 256 fp32 without a selection 13.5 us, with the other 14.9).
+        row_masses<S, false, false>(x, a.scoring, q, top, inv);
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) acc[j] = fmaf(q[j], inv, acc[j]);
 
@@ -478,7 +488,7 @@ __global__ __launch_bounds__(fwd_block(S::R), fwd_waves(S::R)) void forward(FwdA
             };
             // A slot's mass: exp(s - top) or q(s); 0 for an empty one.
             auto mass = [&](int e, float s) {
-                return e < 0 ? 0.0f : soft ? fast_exp(s - top) : mass_of(s, a.scoring);
+                return e < 0 ? 0.0f : soft ? exp_of<true>(s - top) : mass_of(s, a.scoring);
             };
             // The largest selected score, from the lanes' largest.
             auto largest = [&](float s) {
@@ -725,7 +735,7 @@ __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
         const int64_t at = int64_t(b) * a.N + n;
         float x[S::EL], q[S::EL], top, inv;
         raw.get(gl, E, x);
-        row_masses<S, true>(x, a.scoring, q, top, inv);
+        row_masses<S, sizeof(T) == 4, true>(x, a.scoring, q, top, inv);  // 16 bits hold less than either
         float add[S::EL];
 #pragma unroll
         for (int j = 0; j < S::EL; ++j) add[j] = 0.0f;

@@ -95,6 +95,11 @@ __device__ __forceinline__ float exp_compensated(float x) {
     return fmaf(r, e * kLn2, r);
 }
 
+// exp_compensated of x <= 0, -inf (0) and NaN (NaN) among them.
+__device__ __forceinline__ float exp_compensated_below(float x) {
+    return exp_compensated(x < -100.0f ? -100.0f : x);
+}
+
 __device__ __forceinline__ float safe_exp(float x) {
     if (x < -88.0f) return 0.0f;
     return exp_compensated(fminf(x, 88.0f));

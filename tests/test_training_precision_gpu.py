@@ -96,6 +96,38 @@ def test_gradient_of_large_logits():
     assert not g.any()
 
 
+@pytest.mark.parametrize("scoring,normalize", [("sigmoid", True), ("sigmoid", False), ("softmax", True),
+                                               ("softmax", False)])
+@pytest.mark.parametrize("E,k", [(16, 8), (61, 16), (256, 8), (1024, 12)])
+def test_weights_far_below_one_keep_their_digits(scoring, normalize, E, k):
+    """Sigmoid scores near -20 and softmax scores down to -40 under the largest.  A mass is off by 1.25 ulp of its
+    exponential (1.5e-7) and, in a softmax, by d 2^-24 for the difference d to the largest score (of the row, or of the
+    selected).  Normalised: the sum of up to 16 such by as much as its terms and 4 roundings (2.4e-7), the quotient by
+    2^-24: 6e-7.  An unnormalised softmax weight is divided by the sum over the row, whose terms are off by
+    (d + 2) 2^-23: with sum p d <= log E <= 7 below 1.1e-6, with its roundings 1.5e-6 in all."""
+    rng = np.random.default_rng(E)
+    s = (-20.0 - 2.0 * rng.random((1, 200, E))).astype(np.float32)
+    if scoring == "softmax":
+        s = np.where(rng.random((1, 200, E)) < 2.0 / E, -rng.random((1, 200, E)), -40.0 * rng.random((1, 200, E)))
+        s = s.astype(np.float32)
+    x = torch.as_tensor(s).to(DEV).requires_grad_()
+    r = dot_amd.topk_routing(x, k, scoring=scoring, normalize=normalize)
+    o = oracle.route(s, k, scoring, normalize)
+    assert np.array_equal(r.experts.cpu().numpy(), o["experts"])
+    err = np.abs(r.weights.detach().cpu().double().numpy() / o["weights"] - 1)
+    if scoring == "softmax":
+        picked = np.take_along_axis(s, o["experts"], -1).astype(np.float64)
+        top = picked.max(-1, keepdims=True) if normalize else s.max(-1, keepdims=True)
+        # normalised, the sum's terms have that error too, weighed by their share: sum p d <= log 16
+        err -= (top - picked + (np.log(16) if normalize else 0)) * 2.0**-24
+    assert err.max() < (1.5e-6 if (scoring, normalize) == ("softmax", False) else 6e-7), err.max()
+    if scoring == "sigmoid" and not normalize:  # the slope t u^2 is t here, times the upstream gradient: 1.5e-7 + 2^-24
+        dw = rng.uniform(0.5, 2.0, o["weights"].shape).astype(np.float32)
+        (g,) = torch.autograd.grad([r.weights], [x], [torch.as_tensor(dw).to(DEV)])
+        og = oracle.route_grad(s, k, o, scoring, normalize, grad_weights=dw)
+        assert (np.abs(g.cpu().double().numpy() - og) <= 2.2e-7 * np.abs(og)).all()
+
+
 @pytest.mark.parametrize("coupled", [False, True])
 @pytest.mark.parametrize("beta", [0.1, 0.05, 0.3, 1 / 3, 1.7, 64.0])
 def test_hinge_at_its_kink(coupled, beta):
