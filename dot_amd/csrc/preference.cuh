@@ -84,6 +84,8 @@ __device__ __forceinline__ float loss_of(const Loss& l, float x, float y, float&
     } else {
         const float keep = TYPE == kPlain ? 1.0f : 1.0f - l.smoothing;
         const float d = l.beta * gap;
+        // d is rounded twice, to |d| 2^-23 of e: an exponential without the rounding of
+        // its own product (|d| 2^-23.5) would hardly be nearer.
         const float e = fast_exp(-fabsf(d));
         if (SLOPE) {
             const float u = __builtin_amdgcn_rcpf(1.0f + e), eu = e * u;

@@ -4,12 +4,13 @@
 // The forward reads each row once with a running maximum m and sum
 // s = sum_v 2^((x_v - m) k), k = log2(e) / tau, over the vocabulary without the
 // position's own token, which is added in 64 bits: next to a likely token's 1
-// the others' terms of 1e-7 each would lose their digits.  Terms are added
-// pairwise within a pack, and those sums in 64 bits.  A row may be split over several
-// workgroups, whose (m, s) the second kernel joins.  That kernel also forms
-// the position's value and the sequence's sum in 64 bits: the log ratio of two
-// models is a small difference of large sums.  x - m is formed before the
-// scale, so rows at the type's lowest value give finite statistics.  The
+// the others' terms of 1e-7 each would lose their digits.  The 4 or 8 terms of a
+// pack are added pairwise in 32 bits, at most 3 roundings (2e-7 of their sum, of
+// either sign from pack to pack), and the packs' sums in 64 bits.  A row may be
+// split over several workgroups, whose (m, s) the second kernel joins.  That
+// kernel also forms the position's value and the sequence's sum in 64 bits: the
+// log ratio of two models is a small difference of large sums.  x - m is formed
+// before the scale, so rows at the type's lowest value give finite statistics.  The
 // backward reads the row again and writes dx_v = c (delta_va - p_v) with
 // p_v = 2^((x_v - m) k) / s.  Where the token a is likelier than not, 1 - p_a
 // is kept as the others' share of the sum, formed in 64 bits: as a difference it
