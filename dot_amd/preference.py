@@ -24,6 +24,11 @@ from . import _ops
 _REDUCTION = {"none": 0, "sum": 1, "mean": 2}
 _LOSS = {"sigmoid": 0, "hinge": 1, "square": 2}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_F32 = torch.finfo(torch.float32)
+
+# What a call on a GPU takes at most.
+MAX_POSITIONS = 1 << 23
+MAX_ANSWERS = 1 << 22
 
 
 def sequence_logp(
@@ -53,7 +58,7 @@ def sequence_logp(
         mask: Optional bool, shaped as ``tokens``; positions that are False are left
             out (prompt, padding), and so are those whose token is outside [0, V).
             Their logits are not read and their gradient is 0.
-        tau: Temperature (> 0)
+        tau: Temperature (> 0; in [1e-20, 1e20] on a GPU)
         reduction: ``"sum"`` or ``"mean"`` over the positions of a sequence (0 for none),
             or ``"none"`` for each position (0 where left out)
 
@@ -74,6 +79,10 @@ def sequence_logp(
     tau = float(tau)
     if not 0.0 < tau < float("inf"):
         raise ValueError(f"tau must be > 0, got {tau}")
+    if logits.is_cuda and not 1e-20 <= tau <= 1e20:
+        raise ValueError(f"tau must be in [1e-20, 1e20] on a GPU, got {tau}")
+    if logits.is_cuda and tokens.numel() > MAX_POSITIONS:
+        raise ValueError(f"at most {MAX_POSITIONS} positions are supported on a GPU, got {tokens.numel()}")
     batched = logits.dim() == 3
     if ref_logp is not None:
         if not ref_logp.is_floating_point() or ref_logp.shape not in (tokens.shape, tokens.shape[:-1]):
@@ -108,12 +117,13 @@ def preference_loss(
 
     Args:
         log_ratio: (P + Q,) log ratios (:func:`sequence_logp`), first of the P preferred,
-            then of the Q other answers; floating point, computed in fp32
+            then of the Q other answers; floating point, computed in fp32.  P and Q are at
+            most 2^22 on a GPU.
         plan: Optional (P, Q) coupling of the two sets, such as the ``transport_plan``
             of :func:`sinkhorn`; without it answer i is paired with answer P + i (P = Q).
             An entry of 0 leaves its pair out, whatever their ratios (a padded answer
             has a row or a column of 0); its own gradient is ``f`` where that is finite.
-        beta: Scale (> 0)
+        beta: Scale (> 0; a normal fp32 number on a GPU)
         loss_type: ``"sigmoid"``, ``"hinge"`` or ``"square"``
         label_smoothing: In [0, 1), ``"sigmoid"`` only
 
@@ -134,6 +144,11 @@ def preference_loss(
     beta, label_smoothing = float(beta), float(label_smoothing)
     if not 0.0 < beta < float("inf"):
         raise ValueError(f"beta must be > 0, got {beta}")
+    if log_ratio.is_cuda and not _F32.tiny <= beta <= _F32.max:
+        raise ValueError(f"beta must be a normal fp32 number on a GPU, got {beta}")
+    answers = max(plan.shape) if plan is not None else log_ratio.size(0) // 2
+    if log_ratio.is_cuda and answers > MAX_ANSWERS:
+        raise ValueError(f"at most {MAX_ANSWERS} answers of a set are supported on a GPU, got {answers}")
     if not 0.0 <= label_smoothing < 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1), got {label_smoothing}")
     if label_smoothing and loss_type != "sigmoid":

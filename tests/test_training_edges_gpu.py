@@ -42,3 +42,27 @@ def test_masses_below_the_smallest_normal_count_as_none(scoring, normalize):
     q = dot_amd.balance_loss(x[:, none], torch.zeros(1, 3, 1, dtype=torch.int32, device=DEV), scoring=scoring)
     assert q.loss.tolist() == [0.0] and q.counts[0].tolist() == [3] + [0] * 7
     assert (torch.autograd.grad(q.loss.sum(), x)[0] == 0).all()
+
+
+def test_limits_of_the_device_are_refused_as_values():
+    """Before any launch, as other arguments are; on the CPU the same calls run."""
+    x, tokens = torch.zeros(1, 2, 4), torch.zeros(1, 2, dtype=torch.long)
+    for tau in (1e-21, 1e21):
+        assert torch.isfinite(dot_amd.sequence_logp(x, tokens, tau=tau)).all()
+        with pytest.raises(ValueError, match="tau"):
+            dot_amd.sequence_logp(x.to(DEV), tokens.to(DEV), tau=tau)
+    for tau in (1e-20, 1e20):
+        assert torch.isfinite(dot_amd.sequence_logp(x.to(DEV), tokens.to(DEV), tau=tau)).all()
+    few = torch.zeros(1, 1, 1, device=DEV).expand(1, 2**23 + 1, 1)
+    with pytest.raises(ValueError, match="positions"):
+        dot_amd.sequence_logp(few, torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(1, 2**23 + 1))
+    ratio = torch.zeros(4)
+    for beta in (1e-39, 1e39):
+        assert dot_amd.preference_loss(ratio, beta=beta).shape == (2,)
+        with pytest.raises(ValueError, match="beta"):
+            dot_amd.preference_loss(ratio.to(DEV), beta=beta)
+    many = torch.zeros(1, device=DEV)
+    with pytest.raises(ValueError, match="answers"):
+        dot_amd.preference_loss(many.expand(2**23 + 2))
+    with pytest.raises(ValueError, match="answers"):
+        dot_amd.preference_loss(many.expand(2**22 + 2), plan=many.expand(1, 2**22 + 1))
