@@ -90,8 +90,12 @@ def topk_routing(
         scoring: Mass of a score: ``"softmax"`` over the row, ``"sigmoid"``, or
             ``"plan"`` for rows of a transport plan (masses as they are)
         normalize: Weights of a token sum to 1
-        bias: Optional (E,) added to the scores for the selection only (a balancing
-            bias, a column potential); it gets no gradient
+        bias: Optional (E,) added to the scores themselves, whatever the scoring, for the
+            selection only (a column potential, -inf to close an expert); it gets no
+            gradient.  Routers that are balanced by a bias on the masses,
+            ``sigmoid(logit) + bias``, select by another order: form the masses first,
+            ``topk_routing(torch.sigmoid(logits.float()), k, scoring="plan", bias=bias)``,
+            which selects by ``mass + bias`` and has the same weights, loss and gradient
         mask: Optional bool (B, N); tokens that are False are left out: experts -1,
             weights 0, not counted, gradient 0.  Their scores are not read.
 

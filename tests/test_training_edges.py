@@ -1,4 +1,4 @@
-"""CPU: the routing, sequence log-probability and preference operators where their
+"""The routing, sequence log-probability and preference operators where their
 rules decide: rows of masses too small to count, and the rules that the device
 implementations share."""
 
@@ -10,6 +10,7 @@ import dot_amd
 from conftest import rel_err
 from oracle import training as oracle
 
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 TOL = 1e-6  # results in fp32 of sums in 64 bits
 
 
@@ -60,3 +61,36 @@ def test_masses_below_the_smallest_normal_count_as_none(scoring, normalize):
     q = dot_amd.balance_loss(x[:, none], torch.zeros(1, 3, 1, dtype=torch.int32), scoring=scoring)
     assert q.loss.tolist() == [0.0] and q.counts[0].tolist() == [3] + [0] * 7
     assert (torch.autograd.grad(q.loss.sum(), x)[0] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bias_on_the_masses(dev, normalize, dtype):
+    """A bias is added to the scores: to the logits with scoring="sigmoid", to sigmoid(logit) where the masses are
+    given.  Weights and gradients are those of the sigmoid router's definition in 64 bits; fp32 operations in a chain
+    of about ten (logistic function, shares, quotient, slope), 1e-5 of the largest value, and half a step of the type."""
+    gen = torch.Generator().manual_seed(3)
+    B, N, E, k = 2, 60, 64, 8
+    logits = torch.randn(B, N, E, generator=gen).to(dtype).to(dev).requires_grad_()
+    bias = (0.2 * torch.randn(E, generator=gen)).to(dev)
+    q = torch.sigmoid(logits.float())
+    r = dot_amd.topk_routing(q, k, scoring="plan", bias=bias, normalize=normalize)
+    order = torch.argsort(-(q.detach() + bias), dim=-1, stable=True)[..., :k]  # q + bias, equal ones by the lowest index
+    assert torch.equal(r.experts.long(), order)
+    raw = dot_amd.topk_routing(logits.detach(), k, scoring="sigmoid", bias=bias)
+    assert torch.equal(raw.experts.long(), torch.argsort(-(logits.detach().float() + bias), dim=-1, stable=True)[..., :k])
+    assert not torch.equal(raw.experts.long().sort(-1).values, order.sort(-1).values)
+
+    x = logits.detach().double().requires_grad_()
+    s = torch.sigmoid(x)
+    w = s.gather(-1, order)
+    w = w / w.sum(-1, keepdim=True) if normalize else w
+    counts = torch.stack([torch.bincount(t.reshape(-1), minlength=E) for t in order])
+    loss = E * (counts / (k * N) * (s / s.sum(-1, keepdim=True)).mean(1)).sum(-1)
+    assert torch.equal(r.counts.long(), counts)
+    assert rel_err(r.weights, w) < 1e-5 and rel_err(r.balance_loss, loss) < 1e-5
+    dw, dl = torch.randn(B, N, k, generator=gen).to(dev), torch.rand(B, generator=gen).to(dev)
+    (g,) = torch.autograd.grad([r.weights, r.balance_loss], [logits], [dw, dl])
+    (want,) = torch.autograd.grad([w, loss], [x], [dw.double(), dl.double()])
+    assert rel_err(g.float(), want) < 1e-5 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
