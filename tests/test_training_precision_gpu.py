@@ -157,3 +157,25 @@ def test_hinge_at_its_kink(coupled, beta):
     if coupled:
         assert (np.abs(loss.detach().cpu().double().numpy() - o) <= 2e-6 * o).all()
         assert (np.abs(grads[1].cpu().double().numpy() - gp) <= 2.0**-24 * gp).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,S", [(300, 2048), (32768, 500), (131072, 100)])
+@pytest.mark.parametrize("tau", [1.0, 0.7])
+def test_positions_less_their_reference(dtype, V, S, tau):
+    """The error of single positions, which a reference of the same value in fp64 lays bare.  A term p_v of the sum is
+    off by d_v 2^-24 for the difference to the largest logit, as much for its product and 2^-23 for the exponential;
+    it is rescaled for a new maximum, at 2^-23 a time, in its thread (say 5 times), its wave, its workgroup and for the
+    join; a pack adds 3 roundings: (2 sum_v p_v d_v + 2 + 16 + 3) 2^-24 of the sum, that is, of its logarithm."""
+    gen = torch.Generator(DEV).manual_seed(V)
+    x = (2 * torch.randn(2, S, V, device=DEV, generator=gen)).to(DTYPES[dtype])
+    tokens = torch.randint(0, V, (2, S), device=DEV, generator=gen)
+    taken = float(np.log(V)) - 3 + 10 * torch.rand(2, S, 1, device=DEV, generator=gen)
+    x.scatter_(2, tokens[..., None], taken.to(x.dtype))
+    for b in range(2):
+        z = x[b].double() / tau
+        want = torch.log_softmax(z, -1)
+        spread = (want.exp() * (z.amax(-1, keepdim=True) - z)).sum(-1)
+        ref = want.gather(1, tokens[b][:, None])[:, 0]
+        err = dot_amd.sequence_logp(x[b], tokens[b], ref_logp=ref, tau=tau, reduction="none").double().abs()
+        assert (err <= (2 * spread + 21) * 2.0**-24).all(), err.max()
