@@ -36,9 +36,9 @@ struct Shape {
 // f(Shape) of a group that holds E <= DOT_ROUTING_MAX_EXPERTS elements.  A round
 // of the selection costs a wave about 8 + 1.5 EL + log2(G) instructions for its
 // 64 / G rows, so a forward that selects (PAIRS) takes two vectors per lane from
-// 128 experts on: 65536 x 256 fp32, k = 8, 33.3 us, with twice the lanes 43.6.
-// Without a selection, and in the backward, twice the lanes are faster: 13.6 us
-// against 15.1, and 39.6 against 44.1.
+// 128 experts on: 65536 x 256 fp32, k = 8, 32.0 us, with twice the lanes 36.8.
+// Without a selection, and in the backward, twice the lanes are faster: 13.7 us
+// against 15.4, and 35.0 against 39.1.
 template <bool VEC, bool PAIRS, class F>
 void dispatch_shape(int E, F&& f) {
     if (E <= 8) f(Shape<1, 1, VEC>{});
@@ -55,7 +55,7 @@ void dispatch_shape(int E, F&& f) {
 
 // Threads of a forward workgroup.  Few partial rows make `finish` short, so
 // workgroups are large where a lane's registers allow it (up to two vectors; the
-// forward above takes 40.2 us with 512 workgroups of 256 threads).
+// forward above takes 38.3 us with 512 workgroups of 256 threads).
 constexpr int fwd_block(int R) { return R <= 2 ? 512 : 256; }
 // Waves per SIMD that the registers have to leave room for: two workgroups per CU.
 constexpr int fwd_waves(int R) { return R <= 2 ? 4 : 1; }
@@ -671,7 +671,10 @@ struct BwdArgs {
 // not normalised, the weights' gradient at the selected experts):
 //   softmax  ds = p (h - sum p h)  [+ w (dw - sum w dw) at the selected]
 //   others   ds = q' ((h - sum p h) / sum q + (dw or (dw - sum w dw) / Q at the selected))
-// The k values of a row go to their lanes through a zeroed row in LDS.
+// The k values of a row go to their lanes through a zeroed row in LDS.  A lane of
+// the widest shape (more than 2048 experts) holds 64 scores, shares, slopes and
+// additions: with WEIGHTS and rows of any alignment that takes all 256 registers,
+// and 57 (fp32) or 27 (16 bits) are spilled; no other instance spills.
 template <class T, class S, bool WEIGHTS>
 __global__ __launch_bounds__(kBlock) void backward(BwdArgs a) {
     extern __shared__ float lds[];

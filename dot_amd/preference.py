@@ -48,7 +48,8 @@ def sequence_logp(
     Args:
         logits: (B, S, V) or (S, V) in fp32, fp16 or bf16; position s predicts
             ``tokens[..., s]`` (shift them before the call).  A view such as
-            ``logits[:, :-1]`` is read in place.  At most 2^23 positions on a GPU.
+            ``logits[:, :-1]`` is read in place (one whose last dimension has a stride is
+            copied first).  At most 2^23 positions on a GPU.
         tokens: int32 or int64 (B, S) or (S,)
         ref_logp: Optional log-probabilities to subtract, a constant of the gradient:
             per position, shaped as ``tokens`` (``reduction="none"`` of the reference
