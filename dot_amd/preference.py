@@ -24,11 +24,11 @@ from . import _ops
 _REDUCTION = {"none": 0, "sum": 1, "mean": 2}
 _LOSS = {"sigmoid": 0, "hinge": 1, "square": 2}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
-_F32 = torch.finfo(torch.float32)
 
 # What a call on a GPU takes at most.
 MAX_POSITIONS = 1 << 23
 MAX_ANSWERS = 1 << 22
+_MIN_BETA, _MAX_BETA = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def sequence_logp(
@@ -80,10 +80,11 @@ def sequence_logp(
     tau = float(tau)
     if not 0.0 < tau < float("inf"):
         raise ValueError(f"tau must be > 0, got {tau}")
-    if logits.is_cuda and not 1e-20 <= tau <= 1e20:
-        raise ValueError(f"tau must be in [1e-20, 1e20] on a GPU, got {tau}")
-    if logits.is_cuda and tokens.numel() > MAX_POSITIONS:
-        raise ValueError(f"at most {MAX_POSITIONS} positions are supported on a GPU, got {tokens.numel()}")
+    if logits.is_cuda:
+        if not 1e-20 <= tau <= 1e20:
+            raise ValueError(f"tau must be in [1e-20, 1e20] on a GPU, got {tau}")
+        if tokens.numel() > MAX_POSITIONS:
+            raise ValueError(f"at most {MAX_POSITIONS} positions are supported on a GPU, got {tokens.numel()}")
     batched = logits.dim() == 3
     if ref_logp is not None:
         if not ref_logp.is_floating_point() or ref_logp.shape not in (tokens.shape, tokens.shape[:-1]):
@@ -145,11 +146,13 @@ def preference_loss(
     beta, label_smoothing = float(beta), float(label_smoothing)
     if not 0.0 < beta < float("inf"):
         raise ValueError(f"beta must be > 0, got {beta}")
-    if log_ratio.is_cuda and not _F32.tiny <= beta <= _F32.max:
-        raise ValueError(f"beta must be a normal fp32 number on a GPU, got {beta}")
-    answers = max(plan.shape) if plan is not None else log_ratio.size(0) // 2
-    if log_ratio.is_cuda and answers > MAX_ANSWERS:
-        raise ValueError(f"at most {MAX_ANSWERS} answers of a set are supported on a GPU, got {answers}")
+    if log_ratio.is_cuda:
+        if not _MIN_BETA <= beta <= _MAX_BETA:
+            raise ValueError(f"beta must be a normal fp32 number on a GPU, got {beta}")
+        if log_ratio.size(0) > MAX_ANSWERS:
+            answers = max(plan.shape) if plan is not None else log_ratio.size(0) // 2
+            if answers > MAX_ANSWERS:
+                raise ValueError(f"at most {MAX_ANSWERS} answers of a set are supported on a GPU, got {answers}")
     if not 0.0 <= label_smoothing < 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1), got {label_smoothing}")
     if label_smoothing and loss_type != "sigmoid":
