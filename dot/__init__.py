@@ -16,3 +16,5 @@ _sys.modules[__name__ + ".sinkhorn"] = _impl.sinkhorn
 _sys.modules[__name__ + ".bidirectional_softmax"] = _impl.bidirectional_softmax
 _sys.modules[__name__ + ".routing"] = _impl.routing
 _sys.modules[__name__ + ".preference"] = _impl.preference
+_sys.modules[__name__ + ".distillation"] = _impl.distillation
+_sys.modules[__name__ + ".beam"] = _impl.beam

@@ -16,6 +16,14 @@ preference loss over pairs or over a plan:
     ratio = dot_amd.sequence_logp(logits, tokens, ref_logp=ref)
     loss = dot_amd.preference_loss(ratio, plan=plan)
 
+and what makes and teaches the answers: distillation from a teacher's top
+log-probabilities, and the steps of a beam search:
+
+    teacher = dot_amd.top_logp(teacher_logits, k=64)      # logp, tokens
+    loss = dot_amd.distill_loss(logits, teacher.logp, teacher.tokens)
+    r = dot_amd.beam_step(logits, scores)                 # scores, beams, tokens
+    dot_amd.beam_reorder([tokens, *cache], r.beams)       # in place
+
 The operators are registered as ``torch.ops.dot.*`` (the reference's schemas)
 and run hand-written HIP kernels behind the C ABI in ``include/dot_amd.h``.
 ``import dot`` gives the same API under the reference's package name.
@@ -51,6 +59,18 @@ from .preference import (
     SequenceLogp,
     PreferenceLoss,
 )
+from .distillation import (
+    top_logp,
+    distill_loss,
+    TopLogpResult,
+    TopLogp,
+    DistillLoss,
+)
+from .beam import (
+    beam_step,
+    beam_reorder,
+    BeamResult,
+)
 
 __version__ = "0.1.0"
 
@@ -74,4 +94,12 @@ __all__ = [
     "preference_loss",
     "SequenceLogp",
     "PreferenceLoss",
+    "top_logp",
+    "distill_loss",
+    "TopLogpResult",
+    "TopLogp",
+    "DistillLoss",
+    "beam_step",
+    "beam_reorder",
+    "BeamResult",
 ]

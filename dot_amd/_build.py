@@ -31,9 +31,9 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = os.environ.get("DOT_AMD_ARCH", "gfx950")
 
 HIP_SOURCES = ["sinkhorn.hip", "tiled.hip", "bidi.hip", "preflight.hip", "methods.hip", "capi.hip", "noalloc.hip",
-               "routing.hip", "seqlogp.hip", "preference.hip"]
-TORCH_SOURCES = ["torch_ops.cpp", "torch_training.cpp"]  # HIP tensors, through the C ABI
-CPU_SOURCES = ["cpu_ops.cpp", "cpu_training.cpp"]
+               "routing.hip", "seqlogp.hip", "preference.hip", "toplist.hip", "distill.hip", "reorder.hip"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_training.cpp", "torch_generation.cpp"]  # HIP tensors, through the C ABI
+CPU_SOURCES = ["cpu_ops.cpp", "cpu_training.cpp", "cpu_generation.cpp"]
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-mcode-object-version=5",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,433 @@
+// Divergence of rows of logits from a teacher's few log-probabilities, and the
+// gradient of the logits.
+//
+// With a position's K tokens i_k of log-probability t_k, P_k = exp t_k, z = x / tau,
+// Q = softmax(z) and Q_r the sum of Q over the other tokens:
+//   forward  L = sum_k P_k (t_k - log Q_k) + P_r (log P_r - log Q_r)
+//   reverse  L = sum_k Q_k (log Q_k - t_k) + Q_r (log Q_r - log P_r)
+// P_r = 1 - sum_k P_k; with DOT_REST_NONE P is made to sum to 1 and P_r = 0.  The
+// gradient of a named token is a value of its own, that of any other token its share
+// w_j = Q_j / Q_r of one value for the row:
+//   tau dL/dx_j = Q_j - P_j,                     w_j (Q_r - P_r)
+//   tau dL/dx_j = Q_j (log Q_j - t_j - L),       w_j Q_r (log Q_r - log P_r - L)
+// So the row is read once for the others' maximum m and s = sum 2^((x - m) k) alone.
+// The named tokens are left out of it by a bit for each token of the span in LDS
+// (a byte for a pack: one read of LDS per 16 bytes of logits) and added in 64 bits:
+// next to a likely named token the others keep their digits, and differences of
+// probabilities near 1 theirs.  The others' own maximum keeps their shares from
+// vanishing where a named token is far likelier.  The backward writes
+// w_j = 2^((x_j - m) k) / s times the row's value, then the named tokens'.
+#pragma once
+
+#include "seqlogp.cuh"
+
+namespace dot_amd {
+namespace distill {
+
+using seqlogp::MaxSum;
+using seqlogp::Part;
+using seqlogp::Rows;
+using seqlogp::Span;
+
+constexpr int kMaxSpan = 1 << 18;  // tokens whose bits a workgroup holds (32 KB)
+constexpr int kPerLane = DOT_TOP_MAX / kWave;
+
+struct Teacher {
+    const void* tokens;  // [B,S,K]
+    int tokens64;
+    const float* logp;   // [B,S,K]
+    int K;
+};
+
+struct Value {
+    double v;
+    int live, pad;
+};
+
+struct Out {
+    int direction, rest, reduction;
+    float* out;       // [B,S] with DOT_REDUCE_NONE
+    Value* values;    // [B,S] otherwise
+    float2* stats;    // [B,S]: the others' maximum (NaN: left out) and the row's value / s
+    int32_t* at;      // [B,S,K]: the tokens that have a gradient of their own, or -1
+    float* own;       // [B,S,K]: that gradient
+};
+
+// The row of a position, which Rows has no token for.
+__device__ __forceinline__ bool masked(const Rows& r, int64_t at) { return r.mask && !r.mask[at]; }
+
+// The token of an entry, or -1 where it names none.
+__device__ __forceinline__ int named(const Rows& r, const Teacher& t, int64_t entry) {
+    const int64_t v = int_at(t.tokens, t.tokens64, entry);
+    return v >= 0 && v < r.V && !(t.logp[entry] == -__builtin_inff()) ? int(v) : -1;
+}
+
+__device__ __forceinline__ double wave_sum64(double x) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+__device__ __forceinline__ void leave_out(const Out& o, int64_t at) {
+    if (o.reduction == DOT_REDUCE_NONE) o.out[at] = 0.0f;
+    else o.values[at] = Value{0.0, 0, 0};
+    if (o.stats) o.stats[at] = make_float2(__builtin_nanf(""), 0.0f);
+}
+
+// The value of a position and what its gradient is made of, by one wave, from the
+// statistics of its other tokens.  `tok` holds the position's named tokens (-1 where
+// an entry names none, or one that an earlier entry names).
+template <class T>
+__device__ __forceinline__ void finish(const Rows& r, const Teacher& t, const Out& o, int64_t at,
+                                       const int (&tok)[kPerLane], const MaxSum& others) {
+    const int lane = int(threadIdx.x) % kWave;
+    const T* row = seqlogp::row_of<T>(r, at);
+    const double kn = (double(r.k) + double(r.klo)) * 0.693147180559945309417;  // 1 / tau
+    float x[kPerLane], top = others.m, most = -__builtin_inff();
+    double tl[kPerLane], p[kPerLane];
+    double mass = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        x[i] = -__builtin_inff();
+        tl[i] = p[i] = 0.0;
+        if (tok[i] < 0) continue;
+        x[i] = to_float(row[tok[i]]);
+        tl[i] = double(t.logp[at * t.K + i * kWave + lane]);
+        most = fmaxf(most, float(tl[i]));
+        top = fmaxf(top, x[i]);
+    }
+    const bool bucket = o.rest == DOT_REST_BUCKET, reverse = o.direction == DOT_DISTILL_REVERSE;
+    top = wave_max(top);
+    if (top == -__builtin_inff()) top = 0.0f;
+    // P made to sum to 1 keeps its digits however small it is
+    const double less = bucket ? 0.0 : double(wave_max(most));
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+        if (tok[i] >= 0) mass += p[i] = exp(tl[i] - less);
+    mass = wave_sum64(mass);
+    double z = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+        if (tok[i] >= 0) z += exp((double(x[i]) - double(top)) * kn);
+    const bool none = others.s == 0.0;  // no other token is possible
+    const double lr = none ? -__builtin_inf() : (double(others.m) - double(top)) * kn + log(others.s);
+    z = wave_sum64(z) + exp(lr);
+    const double lz = log(z), log_qr = lr - lz, qr = exp(log_qr);
+    double pr = 0.0;
+    if (bucket) {
+        pr = 1.0 - mass;
+        if (pr < 0.0) pr = 0.0;
+    }
+    if (!bucket) {
+        const double lm = log(mass) + less;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            p[i] /= mass;
+            tl[i] -= lm;
+        }
+    }
+    double value = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        if (tok[i] < 0) continue;
+        const double lq = (double(x[i]) - double(top)) * kn - lz;
+        if (!reverse) value += p[i] == 0.0 ? 0.0 : p[i] * (tl[i] - lq);
+        else value += lq == -__builtin_inf() ? 0.0 : exp(lq) * (lq - tl[i]);
+    }
+    value = wave_sum64(value);
+    const double log_pr = log(reverse ? fmax(pr, 0x1p-24) : pr);
+    double other;  // gradient of the others together
+    if (!reverse) {
+        // where no other token is possible, what rounding leaves of P_r is nothing
+        if (bucket && !(pr == 0.0 || (none && pr <= 0x1p-20))) value += pr * (log_pr - log_qr);
+        other = qr - pr;
+    } else {
+        if (!none) value += qr * (log_qr - log_pr);
+        other = none ? 0.0 : qr * (log_qr - log_pr - value);
+    }
+    if (lane == 0) {
+        if (o.reduction == DOT_REDUCE_NONE) o.out[at] = float(value);
+        else o.values[at] = Value{value, 1, 0};
+        if (o.stats) o.stats[at] = make_float2(others.base(), none ? 0.0f : float(other / others.s));
+    }
+    if (!o.stats) return;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int e = i * kWave + lane;
+        if (e >= t.K) break;
+        float g = 0.0f;
+        if (tok[i] >= 0) {
+            const double lq = (double(x[i]) - double(top)) * kn - lz, q = exp(lq);
+            if (!reverse) g = float(q - p[i]);
+            else g = lq == -__builtin_inf() ? 0.0f : float(q * (lq - tl[i] - value));
+        }
+        o.at[at * t.K + e] = tok[i];
+        o.own[at * t.K + e] = g;
+    }
+}
+
+// The position's named tokens, each where it is named first; whether there are any.
+// `list` holds DOT_TOP_MAX ints that this wave alone uses; `twice`: some may be named twice.
+__device__ __forceinline__ bool first_named(const Rows& r, const Teacher& t, int64_t at, int* list, bool twice,
+                                            int (&tok)[kPerLane]) {
+    const int lane = int(threadIdx.x) % kWave;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int e = i * kWave + lane;
+        tok[i] = e < t.K ? named(r, t, at * t.K + e) : -1;
+        list[e] = tok[i];
+        any |= tok[i] >= 0;
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < (twice ? t.K : 0); ++j) {
+        const int v = list[j];
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+            if (tok[i] == v && j < i * kWave + lane) tok[i] = -1;
+    }
+    return __ballot(any) != 0;
+}
+
+// The other tokens' statistics of every row, one for each split; an unsplit row is
+// finished at once.
+template <class T>
+__global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Part* parts) {
+    extern __shared__ uint32_t words[];
+    __shared__ float sm[kWavesPerBlock];
+    __shared__ double ss[kWavesPerBlock];
+    __shared__ int list[DOT_TOP_MAX];
+    __shared__ int any, twice;
+    constexpr int PN = Pack<T>::N;
+    const int64_t at = blockIdx.x / unsigned(r.splits);
+    const int part = int(blockIdx.x % unsigned(r.splits));
+    const bool whole = r.splits == 1;
+    if (masked(r, at)) {
+        if (whole && threadIdx.x == 0) leave_out(o, at);
+        return;
+    }
+    const T* row = seqlogp::row_of<T>(r, at);
+    const Span sp = seqlogp::span_of(row, r.V, part, r.splits);
+    const T* body = row + sp.head;
+    const int v0 = part == 0 ? 0 : sp.head + sp.p0 * PN;
+    const int v1 = part == r.splits - 1 ? r.V : sp.head + sp.p1 * PN;
+    const int first = sp.head + sp.p0 * PN - 32;  // token of bit 0
+    const int nwords = (v1 - first + 31) / 32;
+    for (int i = threadIdx.x; i < nwords; i += kBlock) words[i] = 0;
+    if (threadIdx.x == 0) any = twice = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < t.K; e += kBlock) {
+        const int v = named(r, t, at * t.K + e);
+        if (v < 0) continue;
+        any = 1;
+        if (v < v0 || v >= v1) continue;
+        const uint32_t bit = 1u << ((v - first) % 32);
+        if (atomicOr(&words[(v - first) / 32], bit) & bit) twice = 1;
+    }
+    __syncthreads();
+    if (!any) {
+        if (whole && threadIdx.x == 0) leave_out(o, at);
+        return;
+    }
+    auto bit = [&](int v) { return words[(v - first) / 32] >> ((v - first) % 32) & 1u; };
+    // the bits of a pack, from bit 0 on
+    auto bits = [&](int p) {
+        const uint32_t b = reinterpret_cast<const uint8_t*>(words)[(32 + (p - sp.p0) * PN) / 8];
+        return PN == 8 ? b : (p - sp.p0) % 2 ? b >> 4 : b & 15u;
+    };
+    MaxSum a;
+    auto packs = [&](auto stream) {
+        auto values = [&](const Pack<T>& x, int p, float* f) {
+#pragma unroll
+            for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
+            const uint32_t b = bits(p);
+            if (b) {
+#pragma unroll
+                for (int i = 0; i < PN; ++i)
+                    if (b >> i & 1u) f[i] = -__builtin_inff();
+            }
+        };
+        int p = sp.p0 + int(threadIdx.x);
+        constexpr int U = seqlogp::kUnroll;
+        for (; p + (U - 1) * kBlock < sp.p1; p += U * kBlock) {
+            Pack<T> x[U];
+            float f[U * PN];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                x[u] = seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p + u * kBlock) * PN);
+#pragma unroll
+            for (int u = 0; u < U; ++u) values(x[u], p + u * kBlock, f + u * PN);
+            a.template add<PN>(f, r);
+        }
+        for (; p < sp.p1; p += kBlock) {
+            float f[PN];
+            values(seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p) * PN), p, f);
+            a.template add<PN>(f, r);
+        }
+    };
+    if (at < r.cached) packs(std::true_type{});
+    else packs(std::false_type{});
+    auto one = [&](int v) {
+        const float f[1] = {bit(v) ? -__builtin_inff() : to_float(row[v])};
+        a.add<1>(f, r);
+    };
+    if (part == 0 && int(threadIdx.x) < sp.head) one(int(threadIdx.x));
+    if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) one(sp.tail + int(threadIdx.x));
+    const float m = wave_max(a.m);
+    a.raise(m, r);
+    const double s = wave_sum64(a.s);
+    if (threadIdx.x % kWave == 0) {
+        sm[threadIdx.x / kWave] = m;
+        ss[threadIdx.x / kWave] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x >= kWave) return;
+    MaxSum all;
+    for (int w = 0; w < kWavesPerBlock; ++w) all.join(sm[w], ss[w], r);
+    if (!whole) {
+        if (threadIdx.x == 0) parts[blockIdx.x] = Part{all.s, all.m};
+        return;
+    }
+    int tok[kPerLane];
+    first_named(r, t, at, list, twice, tok);
+    finish<T>(r, t, o, at, tok, all);
+}
+
+// Joins the parts of split rows, one wave a row.
+template <class T>
+__global__ __launch_bounds__(kBlock) void finish_rows(Rows r, Teacher t, Out o, const Part* parts) {
+    __shared__ int lists[kWavesPerBlock][DOT_TOP_MAX];
+    const int wave = int(threadIdx.x) / kWave;
+    const int64_t at = int64_t(blockIdx.x) * kWavesPerBlock + wave;
+    if (at >= int64_t(r.B) * r.S) return;
+    int tok[kPerLane];
+    if (masked(r, at) || !first_named(r, t, at, lists[wave], true, tok)) {
+        if (threadIdx.x % kWave == 0) leave_out(o, at);
+        return;
+    }
+    MaxSum all;
+    for (int i = 0; i < r.splits; ++i) {
+        const Part p = parts[at * r.splits + i];
+        all.join(p.m, p.s, r);
+    }
+    finish<T>(r, t, o, at, tok, all);
+}
+
+// The positions' values of each sequence, added up.
+__global__ __launch_bounds__(seqlogp::kJoinBlock) void sum(int B, int S, int reduction, const Value* values,
+                                                          float* out, float* weight) {
+    constexpr int waves = seqlogp::kJoinBlock / kWave;
+    __shared__ double wsum[waves];
+    __shared__ int wcount[waves];
+    const int b = batch_of_block();
+    if (b >= B) return;
+    double total = 0.0;
+    int count = 0;
+    for (int s = threadIdx.x; s < S; s += seqlogp::kJoinBlock) {
+        const Value v = values[int64_t(b) * S + s];
+        total += v.v;
+        count += v.live;
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        total += __shfl_xor(total, d);
+        count += __shfl_xor(count, d);
+    }
+    if (threadIdx.x % kWave == 0) {
+        wsum[threadIdx.x / kWave] = total;
+        wcount[threadIdx.x / kWave] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    total = 0.0;
+    count = 0;
+    for (int w = 0; w < waves; ++w) {
+        total += wsum[w];
+        count += wcount[w];
+    }
+    const double of = reduction == DOT_REDUCE_MEAN ? 1.0 / (count > 0 ? count : 1) : 1.0;
+    out[b] = float(total * of);
+    if (weight) weight[b] = float(of);
+}
+
+struct GradArgs {
+    int K;
+    float inv_tau;
+    int reduction;
+    const float2* stats;
+    const int32_t* at;
+    const float* own;
+    const float* weight;
+    const float* grad_out;
+    int grad_out_scalar;
+    void* grad;
+};
+
+// dx of one span of a row.
+template <class T>
+__global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
+    // last rows first: the forward has just read them
+    const int64_t at = int64_t(r.B) * r.S - 1 - blockIdx.x / unsigned(r.splits);
+    const int part = int(blockIdx.x % unsigned(r.splits));
+    constexpr int PN = Pack<T>::N;
+    T* out = static_cast<T*>(g.grad) + at * r.V;
+    const Span sp = seqlogp::span_of(out, r.V, part, r.splits);
+    const float2 st = g.stats[at];
+    if (st.x != st.x) {
+        const Pack<T> zero{};
+        for (int p = sp.p0 + int(threadIdx.x); p < sp.p1; p += kBlock)
+            store_pack_stream(out + sp.head + int64_t(p) * PN, zero);
+        if (part == 0 && int(threadIdx.x) < sp.head) out[threadIdx.x] = T{};
+        if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) out[sp.tail + threadIdx.x] = T{};
+        return;
+    }
+    const T* row = seqlogp::row_of<T>(r, at);
+    const int64_t b = at / r.S;
+    const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
+    const float c = (g.reduction == DOT_REDUCE_MEAN ? up * g.weight[b] : up) * g.inv_tau;
+    const float scale = c * st.y;
+    auto value = [&](float x) { return __builtin_amdgcn_exp2f(seqlogp::scaled(r, x - st.x)) * scale; };
+    const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+    auto pack_in = [&](int p, auto stream) {
+        const T* at_p = row + sp.head + int64_t(p) * PN;
+        if (together) return seqlogp::row_pack<decltype(stream)::value>(at_p);
+        Pack<T> x;
+#pragma unroll
+        for (int i = 0; i < PN; ++i) x.v[i] = at_p[i];
+        return x;
+    };
+    auto pack_out = [&](int p, const Pack<T>& x) {
+        Pack<T> y;
+#pragma unroll
+        for (int i = 0; i < PN; ++i) y.v[i] = from_float<T>(value(to_float(x.v[i])));
+        store_pack_stream(out + sp.head + int64_t(p) * PN, y);
+    };
+    auto packs = [&](auto stream) {
+        constexpr int U = seqlogp::kUnroll;
+        int p = sp.p0 + int(threadIdx.x);
+        for (; p + (U - 1) * kBlock < sp.p1; p += U * kBlock) {
+            Pack<T> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = pack_in(p + u * kBlock, stream);
+#pragma unroll
+            for (int u = 0; u < U; ++u) pack_out(p + u * kBlock, x[u]);
+        }
+        for (; p < sp.p1; p += kBlock) pack_out(p, pack_in(p, stream));
+    };
+    if (at < r.cached) packs(std::true_type{});
+    else packs(std::false_type{});
+    if (part == 0 && int(threadIdx.x) < sp.head) out[threadIdx.x] = from_float<T>(value(to_float(row[threadIdx.x])));
+    const int v = sp.tail + int(threadIdx.x);
+    if (part == r.splits - 1 && v < r.V) out[v] = from_float<T>(value(to_float(row[v])));
+    // the named tokens of the span, over what was just written there
+    __syncthreads();
+    const int v0 = part == 0 ? 0 : sp.head + sp.p0 * PN;
+    const int v1 = part == r.splits - 1 ? r.V : sp.head + sp.p1 * PN;
+    for (int e = threadIdx.x; e < g.K; e += kBlock) {
+        const int tok = g.at[at * g.K + e];
+        if (tok >= v0 && tok < v1) out[tok] = from_float<T>(c * g.own[at * g.K + e]);
+    }
+}
+
+}  // namespace distill
+}  // namespace dot_amd

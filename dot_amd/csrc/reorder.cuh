@@ -1,0 +1,107 @@
+// States of the chosen beams, in place.
+//
+// A thread holds one unit (16 bytes at most) of the same place in every beam: it
+// loads what the moving beams' parents have there, then stores it.  No place is read
+// by another thread than the one that writes it, so neither a second copy of the
+// states nor an order among the threads is needed, whatever the parents are.  Beams
+// that stay are not written, parents that no moving beam has are not read; a parent
+// of several is read from memory once.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "elem.cuh"
+#include "row.cuh"
+
+namespace dot_amd {
+namespace reorder {
+
+constexpr int kMaxStates = 32;  // of a launch: their descriptions travel with its arguments
+
+struct State {
+    char* data;
+    int64_t sb, sw, so, sp;
+    int64_t outer, positions;
+    uint32_t inner;  // units of a position
+    int first;       // first workgroup (of a batch element)
+};
+struct States {
+    State s[kMaxStates];
+    int count;
+    const void* beams;
+    int beams64;
+    const void* lengths;
+    int lengths64;
+    int B, W;
+};
+
+template <int BYTES>
+struct UnitOf;
+template <>
+struct UnitOf<1> {
+    using type = uint8_t;
+};
+template <>
+struct UnitOf<2> {
+    using type = uint16_t;
+};
+template <>
+struct UnitOf<4> {
+    using type = uint32_t;
+};
+template <>
+struct UnitOf<8> {
+    using type = uint64_t;
+};
+template <>
+struct UnitOf<16> {
+    typedef uint32_t type __attribute__((ext_vector_type(4)));
+};
+
+// MAX: the most beams that a thread has registers for.
+template <int BYTES, int MAX>
+__global__ __launch_bounds__(kBlock) void move(States a) {
+    using U = typename UnitOf<BYTES>::type;
+    __shared__ int parent[MAX];
+    const int b = batch_of_block();
+    if (b >= a.B) return;
+    int i = 0;
+    while (i + 1 < a.count && int(blockIdx.x) >= a.s[i + 1].first) ++i;
+    const State& s = a.s[i];
+    const int blocks = (i + 1 < a.count ? a.s[i + 1].first : int(gridDim.x)) - s.first;
+    bool moves = false;
+    for (int w = threadIdx.x; w < MAX; w += kBlock) {
+        const int64_t p = w < a.W ? int_at(a.beams, a.beams64, int64_t(b) * a.W + w) : -1;
+        parent[w] = p >= 0 && p < a.W && p != w ? int(p) : -1;
+        moves |= parent[w] >= 0;
+    }
+    if (!__syncthreads_or(moves)) return;
+    int64_t used = s.positions;
+    if (a.lengths) used = min(max(int_at(a.lengths, a.lengths64, b), int64_t(0)), used);
+    const uint64_t run = uint64_t(used) * s.inner, total = uint64_t(s.outer) * run;
+    char* base = s.data + int64_t(b) * s.sb;
+    const bool dense = s.sp == int64_t(s.inner) * BYTES;
+    for (uint64_t u = uint64_t(int(blockIdx.x) - s.first) * kBlock + threadIdx.x; u < total;
+         u += uint64_t(blocks) * kBlock) {
+        const uint64_t o = u / run, at = u - o * run;
+        int64_t off = int64_t(o) * s.so;
+        if (dense) {
+            off += int64_t(at) * BYTES;
+        } else {
+            const uint64_t p = at / s.inner;
+            off += int64_t(p) * s.sp + int64_t(at - p * s.inner) * BYTES;
+        }
+        U x[MAX];
+#pragma unroll
+        for (int w = 0; w < MAX; ++w)
+            if (parent[w] >= 0) x[w] = *reinterpret_cast<const U*>(base + off + int64_t(parent[w]) * s.sw);
+#pragma unroll
+        for (int w = 0; w < MAX; ++w)
+            if (parent[w] >= 0) *reinterpret_cast<U*>(base + off + int64_t(w) * s.sw) = x[w];
+    }
+}
+
+}  // namespace reorder
+}  // namespace dot_amd

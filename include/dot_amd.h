@@ -1,6 +1,6 @@
 /*
  * dot_amd — C ABI of the MI355X (gfx950) Sinkhorn and bidirectional-softmax engine,
- * with the routing and preference operators beside it.
+ * with the routing, preference, distillation and beam search operators beside it.
  *
  * Plain pointers and sizes only.  Every pointer argument is device memory
  * owned by the caller (fp32 unless stated); the library allocates nothing on
@@ -526,6 +526,145 @@ typedef struct {
 
 size_t dot_preference_backward_workspace_bytes(int P, int Q, int has_plan);
 int dot_preference_backward(const dot_preference_bwd_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Top log-probabilities (no counterpart in the reference)                 */
+/* ---------------------------------------------------------------------- */
+#define DOT_TOP_MAX 256 /* entries of a position, continuations of a beam step */
+
+typedef struct {
+    const void* logits;        /* element (b, s, v) at b * stride_b + s * stride_s + v */
+    int dtype;
+    int64_t stride_b, stride_s;
+    int B, S, V;               /* V <= 2^24, B * S <= 2^23 */
+    int k;                     /* 1 <= k <= min(V, DOT_TOP_MAX) */
+    const uint8_t* mask;       /* [B,S]: positions with 0 are left out, or NULL */
+    double tau;                /* > 0 */
+    float* logp;               /* [B,S,k] out: log-probabilities by descending logit, -inf in empty slots */
+    int32_t* tokens;           /* [B,S,k] out: their tokens, -1 in empty slots */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_top_logp_args;
+
+/* The k largest logits of each position, equal ones by the lowest token, as
+ * x / tau - log sum_v exp(x_v / tau).  Logits of -inf and NaN are not taken; a
+ * position with fewer than k others, or that is left out, has empty slots. */
+size_t dot_top_logp_workspace_bytes(int B, int S, int V, int dtype, int k);
+int dot_top_logp(const dot_top_logp_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Distillation from top log-probabilities (no counterpart in the reference) */
+/* ---------------------------------------------------------------------- */
+enum { DOT_DISTILL_FORWARD = 0, DOT_DISTILL_REVERSE = 1 };
+/* What the teacher's tokens leave of its mass: a class of its own, or nothing
+ * (the tokens' masses are made to sum to 1; DOT_DISTILL_FORWARD only). */
+enum { DOT_REST_BUCKET = 0, DOT_REST_NONE = 1 };
+
+typedef struct {
+    const void* logits;        /* element (b, s, v) at b * stride_b + s * stride_s + v */
+    int dtype;
+    int64_t stride_b, stride_s;
+    int B, S, V, K;            /* V <= 2^24, B * S <= 2^23, 1 <= K <= DOT_TOP_MAX */
+    const void* tokens;        /* [B,S,K] int32 (int64 with tokens_are_int64); an entry whose token is outside
+                                  [0, V), whose logp is -inf, or whose token an earlier entry names, names none */
+    int tokens_are_int64;
+    const float* logp;         /* [B,S,K] the teacher's log-probabilities of them */
+    const uint8_t* mask;       /* [B,S]: positions with 0 are left out, or NULL; so are those that name no token */
+    double tau;
+    int direction;             /* DOT_DISTILL_* */
+    int rest;                  /* DOT_REST_* */
+    int reduction;             /* DOT_REDUCE_* over the positions that are not left out */
+    float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
+    float* row_stats;          /* [B,S,2] out, for the backward, or NULL: the largest logit of the tokens that are
+                                  not named (NaN where left out), and the factor of their exponentials */
+    int32_t* own_tokens;       /* [B,S,K] out with row_stats: the named tokens, -1 elsewhere */
+    float* own_grad;           /* [B,S,K] out with row_stats: tau times their gradient */
+    float* weight;             /* [B] out with DOT_REDUCE_MEAN, for the backward: 1 / positions */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_distill_fwd_args;
+
+/* With P = exp(logp), P_r = max(0, 1 - sum P), Q = softmax(x / tau) and Q_r its sum
+ * over the tokens that are not named: sum P (log P - log Q) + P_r (log P_r - log Q_r),
+ * or sum Q (log Q - log P) + Q_r (log Q_r - log max(P_r, 2^-24)).  Where Q_r is 0, a
+ * P_r of at most 2^-20 counts as 0. */
+size_t dot_distill_forward_workspace_bytes(int B, int S, int V, int dtype, int reduction);
+int dot_distill_forward(const dot_distill_fwd_args* args, dot_stream_t stream);
+
+typedef struct {
+    const void* logits;
+    int dtype;
+    int64_t stride_b, stride_s;
+    int B, S, V, K;
+    double tau;
+    int reduction;
+    const uint8_t* mask;       /* not read: row_stats says what is left out */
+    const float* row_stats;
+    const int32_t* own_tokens;
+    const float* own_grad;
+    const float* weight;       /* with DOT_REDUCE_MEAN */
+    const float* grad_out;     /* [B], or [B,S] with DOT_REDUCE_NONE; one value with grad_out_scalar */
+    int grad_out_scalar;
+    void* grad_logits;         /* [B,S,V] out, contiguous, of type dtype; 0 where left out */
+} dot_distill_bwd_args;
+
+int dot_distill_backward(const dot_distill_bwd_args* args, dot_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Beam search (no counterpart in the reference)                           */
+/* ---------------------------------------------------------------------- */
+#define DOT_BEAM_MAX 128 /* beams of a batch element */
+
+typedef struct {
+    const void* logits;        /* element (b, w, v) at b * stride_b + w * stride_w + v */
+    int dtype;
+    int64_t stride_b, stride_w;
+    int B, W, V;               /* W <= DOT_BEAM_MAX, V <= 2^24, B * W <= 2^23 */
+    int n;                     /* continuations of a batch element, 1 <= n <= min(W * V, DOT_TOP_MAX) */
+    double tau;
+    const float* scores;       /* [B,W]: scores of the hypotheses; -inf closes a beam */
+    const uint8_t* finished;   /* [B,W]: a finished hypothesis goes on as it is, with token eos, or NULL */
+    int eos;                   /* token that finishes a hypothesis, or -1 */
+    float* out_scores;         /* [B,n] out, descending; -inf in empty slots */
+    int32_t* out_beams;        /* [B,n] out: the continued beam, -1 in empty slots */
+    int32_t* out_tokens;       /* [B,n] out: its next token, -1 in empty slots */
+    uint8_t* out_finished;     /* [B,n] out, or NULL */
+    void* workspace;
+    size_t workspace_bytes;
+} dot_beam_step_args;
+
+/* The n largest totals score_w + x_v / tau - log sum exp(x / tau) of each batch
+ * element, in 64 bits; equal ones by beam, then by descending logit, then by token.
+ * A NaN total is not taken.  Logits of closed and finished beams are not read. */
+size_t dot_beam_step_workspace_bytes(int B, int W, int V, int dtype, int n);
+int dot_beam_step(const dot_beam_step_args* args, dot_stream_t stream);
+
+/* One state of every beam.  Byte offset of byte i of position p of run o of beam w:
+ * b * stride_b + w * stride_w + o * stride_outer + p * stride_p + i, i < inner.
+ * Strides are >= 0; no two of these bytes may be the same. */
+typedef struct {
+    void* data;
+    int64_t stride_b, stride_w, stride_outer, stride_p; /* in bytes */
+    int64_t outer, positions, inner;
+} dot_beam_state;
+
+typedef struct {
+    const dot_beam_state* states; /* host array */
+    int count;
+    int B, W;                  /* W <= DOT_BEAM_MAX */
+    const void* beams;         /* [B,W] int32 (int64 with beams_are_int64): beam w becomes what beam beams[b, w] was;
+                                  outside [0, W): it stays as it is */
+    int beams_are_int64;
+    const void* lengths;       /* [B] int32 (int64 with lengths_are_int64): positions that are moved, the others
+                                  stay as they are; NULL: all */
+    int lengths_are_int64;
+} dot_beam_reorder_args;
+
+/* The beams' states are exchanged in place, all from what they were before the
+ * call.  No two states may share memory. */
+int dot_beam_reorder(const dot_beam_reorder_args* args, dot_stream_t stream);
+/* Its checks alone: a host function, data may be host memory. */
+int dot_beam_reorder_check(const dot_beam_reorder_args* args);
 
 /* ---------------------------------------------------------------------- */
 /* Diagnostics (no counterpart in the reference)                           */
