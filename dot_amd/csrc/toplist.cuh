@@ -70,9 +70,23 @@ __device__ __forceinline__ Pack<T> load_pack_any(const T* p) {
     return x;
 }
 
-__device__ __forceinline__ float minus_inf(float) { return -__builtin_inff(); }
-__device__ __forceinline__ F16 minus_inf(F16) { return F16{0xFC00}; }
-__device__ __forceinline__ BF16 minus_inf(BF16) { return BF16{0xFF80}; }
+// A pack as it is in registers: the compiler would otherwise keep the floats that one
+// pass made of it for the next, at twice the registers.
+template <class T>
+__device__ __forceinline__ void hold(Pack<T>& x) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    u4 raw = __builtin_bit_cast(u4, x);
+    asm volatile("" : "+v"(raw));
+    x = __builtin_bit_cast(Pack<T>, raw);
+}
+
+// A pack of -inf.
+template <class T>
+__device__ __forceinline__ Pack<T> nothing_pack() {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const uint32_t w = std::is_same_v<T, float> ? 0xFF800000u : std::is_same_v<T, F16> ? 0xFC00FC00u : 0xFF80FF80u;
+    return __builtin_bit_cast(Pack<T>, u4{w, w, w, w});
+}
 
 // Floats in an order of unsigned integers (of -0 and 0, which are equal, callers add 0 first).
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -120,16 +134,61 @@ struct TopOut {
     int32_t* token;   // [rows, n]
 };
 
+// A value that at least `r` of the wave's G * 64 values reach, and few more: the r-th
+// largest to within a quarter of r, by bisection with ballots.  Where fewer than r are
+// above -inf: the lowest finite value.
+template <int G>
+__device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
+    auto count = [&](float t) {
+        int c = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) c += __builtin_popcountll(__ballot(v[g] >= t));
+        return c;
+    };
+    float most = v[0], least = v[0];
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+        most = fmaxf(most, v[g]);
+        least = fminf(least, v[g]);
+    }
+    most = wave_max(most);
+    least = wave_reduce(least, [](float a, float b) { return fminf(a, b); });
+    const float lowest = -__FLT_MAX__;
+    if (!(least >= lowest)) {
+        least = lowest;
+        if (count(lowest) < r) return lowest;
+    }
+    uint32_t lo = order_of(least + 0.0f), hi = order_of(most + 0.0f) + 1;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const int c = count(value_of(mid));
+        if (c >= r) lo = mid;
+        else hi = mid;
+        if (c >= r && c <= r + r / 4) break;
+    }
+    return value_of(lo);
+}
+
 // One span of a row.  DIRECT: the row is one span, and its list the output.
+//
+// Each wave finds a value that its share of the n entries reaches, from the maxima of
+// its lanes (of parts of them for long lists); the lowest of the four values is reached
+// by n entries of the span at least, and by few more on logits in no particular order.
+// Those are collected, each wave in a place of its own, and ranked by counting.  Where
+// they are too many (ties, orders in which the largest lie in few lanes), the n-th
+// largest entry is found by bisection over all of them instead.
 template <class T, int P, bool DIRECT>
-__global__ __launch_bounds__(kBlock) void scan(Rows r, Lists lists, TopOut out) {
-    constexpr int PN = Pack<T>::N, NE = P * PN;
-    __shared__ uint64_t found[DOT_TOP_MAX];
+__global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut out) {
+    constexpr int PN = Pack<T>::N;
+    constexpr int G = P == 1 || P == 2 ? 2 : 4;   // values of a lane for lists of more than 128 entries
+    constexpr int ROOM = 512;                     // entries that a wave collects
+    constexpr int STRIDE = ROOM + 2;              // a quad reads the four places at once: other banks
+    __shared__ uint64_t found[kWavesPerBlock * STRIDE];
     __shared__ int counts[2][kWavesPerBlock];
-    __shared__ float wm[kWavesPerBlock];
+    __shared__ float wm[kWavesPerBlock], wt[kWavesPerBlock];
     __shared__ double ws[kWavesPerBlock];
-    __shared__ int places;
-    int turn = 0;
     const int row = batch_of_block(), part = int(blockIdx.x);
     if (row >= r.rows) return;
     if (!read_row(r, row)) {
@@ -140,107 +199,199 @@ __global__ __launch_bounds__(kBlock) void scan(Rows r, Lists lists, TopOut out) 
             }
         return;
     }
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     const T* x0 = row_of<T>(r, row);
     const int p0 = part * r.per, whole = r.V / PN;
     const int p1 = min(p0 + r.per, (r.V + PN - 1) / PN);
     Pack<T> x[P];
+    // packs past the span are the last whole one (a cache hit), then nothing
+    const int end = min(p1, whole);
+    if (end > p0) {
 #pragma unroll
-    for (int u = 0; u < P; ++u) {
-        const int p = p0 + u * kBlock + int(threadIdx.x);
-        if (p < min(p1, whole)) {
-            x[u] = load_pack_any(x0 + int64_t(p) * PN);
-        } else {
+        for (int u = 0; u < P; ++u)
+            x[u] = load_pack_any(x0 + int64_t(min(p0 + u * kBlock + int(threadIdx.x), end - 1)) * PN);
+    }
+    if (end - p0 < P * kBlock) {
 #pragma unroll
-            for (int i = 0; i < PN; ++i) {
-                const int v = p * PN + i;
-                x[u].v[i] = minus_inf(T{});
-                if (p < p1 && v < r.V) x[u].v[i] = x0[v];
-            }
+        for (int u = 0; u < P; ++u)
+            if (p0 + u * kBlock + int(threadIdx.x) >= end) x[u] = nothing_pack<T>();
+        if (p1 > whole) {  // the row's last elements
+            Pack<T> last = nothing_pack<T>();
+#pragma unroll
+            for (int i = 0; i < PN; ++i)
+                if (whole * PN + i < r.V) last.v[i] = x0[whole * PN + i];
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                if (p0 + u * kBlock + int(threadIdx.x) == whole) x[u] = last;
         }
     }
-    if (threadIdx.x == 0) places = 0;
+    float pm[P];  // the largest logit of each pack
     float m = -__builtin_inff();
 #pragma unroll
-    for (int e = 0; e < NE; ++e) m = fmaxf(m, to_float(x[e / PN].v[e % PN]));
-    m = wave_max(m);
-    if (threadIdx.x % kWave == 0) wm[threadIdx.x / kWave] = m;
-    __syncthreads();
-    m = wm[0];
-    for (int w = 1; w < kWavesPerBlock; ++w) m = fmaxf(m, wm[w]);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    double s = 0.0;
-#pragma unroll
     for (int u = 0; u < P; ++u) {
-        float e[PN];
+        pm[u] = to_float(x[u].v[0]);
 #pragma unroll
-        for (int i = 0; i < PN; ++i) e[i] = __builtin_amdgcn_exp2f((to_float(x[u].v[i]) - base) * r.k);
-        s += double(pairwise<PN>(e));
+        for (int i = 1; i < PN; ++i) pm[u] = fmaxf(pm[u], to_float(x[u].v[i]));
+        m = fmaxf(m, pm[u]);
+    }
+    const int share = (r.n + kWavesPerBlock - 1) / kWavesPerBlock;
+    float least;
+    if (r.n <= 128) {
+        const float v[1] = {m};
+        least = reached_by(v, share);
+    } else {
+        float v[G];
+        if constexpr (P == 1) {
+            v[0] = v[1] = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < PN; ++i) v[i % 2] = fmaxf(v[i % 2], to_float(x[0].v[i]));
+        } else {
+#pragma unroll
+            for (int u = 0; u < P; ++u) v[u % G] = u < G ? pm[u] : fmaxf(v[u % G], pm[u]);
+        }
+        least = reached_by(v, share);
+    }
+    m = wave_max(m);
+    if (lane == 0) {
+        wm[wave] = m;
+        wt[wave] = least;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    least = fminf(fminf(wt[0], wt[1]), fminf(wt[2], wt[3]));
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    // The span again from the caches, for what is rare.  All lanes of a wave go round
+    // together: `use` may hold ballots.
+    auto each = [&](auto use) {
+        for (int p = p0; p < p1; p += kBlock) {
+            const int mine = p + int(threadIdx.x);
+            Pack<T> y;
+            if (mine < end) y = load_pack_any(x0 + int64_t(mine) * PN);
+            for (int i = 0; i < PN; ++i) {
+                const int v = mine * PN + i;
+                float f = -__builtin_inff();
+                if (mine < end) f = to_float(y.v[i]);
+                else if (mine < p1 && v < r.V) f = to_float(x0[v]);
+                use(f, v);
+            }
+        }
+    };
+    // the sum; x k - m k in one rounding where m k has digits behind the point
+    double s = 0.0;
+    const float mk = base * r.k;
+    const bool near = fabsf(mk) < 65536.0f;
+#pragma unroll
+    for (int u = 0; u < P; ++u) hold(x[u]);
+    if (near) {
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+            float e[PN];
+#pragma unroll
+            for (int i = 0; i < PN; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(to_float(x[u].v[i]), r.k, -mk));
+            s += double(pairwise<PN>(e));
+        }
+    } else {
+        each([&](float f, int) { s += double(__builtin_amdgcn_exp2f((f - base) * r.k)); });
     }
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
-    if (threadIdx.x % kWave == 0) ws[threadIdx.x / kWave] = s;
+    if (lane == 0) ws[wave] = s;
 
-    // Entries of the span that `is` holds for.
-    auto count = [&](auto is) {
-        int c = 0;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-            const int v = (p0 + (e / PN) * kBlock + int(threadIdx.x)) * PN + e % PN;
-            c += __builtin_popcountll(__ballot(is(to_float(x[e / PN].v[e % PN]), v)));
-        }
-        return block_count(c, counts, turn);
+    // Entries of -inf and NaN are below `least`.  Each wave's go to a place of its own.
+    int found_here = 0;
+    auto put = [&](float f, int v, bool in) {
+        const uint64_t all = __ballot(in);
+        if (all == 0) return;
+        const int at = found_here + __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
+        if (in && at < ROOM) found[wave * STRIDE + at] = entry_of(f, v);
+        found_here += __builtin_popcountll(all);
     };
-    const float lowest = -__FLT_MAX__;
-    const int want = min(r.n, count([&](float f, int) { return f >= lowest; }));
-    float least = __builtin_inff();
-    int last = -1;
-    if (want > 0) {
-        // the want-th largest value
-        uint32_t lo = order_of(lowest), hi = order_of(m + 0.0f) + 1;
+#pragma unroll
+    for (int u = 0; u < P; ++u) hold(x[u]);
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        if (__ballot(pm[u] >= least) == 0) continue;
+#pragma unroll
+        for (int i = 0; i < PN; ++i) {
+            const float f = to_float(x[u].v[i]);
+            put(f, (p0 + u * kBlock + int(threadIdx.x)) * PN + i, f >= least);
+        }
+    }
+    if (lane == 0) counts[0][wave] = found_here;
+    __syncthreads();
+    int most = counts[0][0];
+    for (int w = 1; w < kWavesPerBlock; ++w) most = max(most, counts[0][w]);
+    if (most > ROOM) {
+        int turn = 1;
+        auto count = [&](auto is) {
+            int c = 0;
+            each([&](float f, int v) { c += __builtin_popcountll(__ballot(is(f, v))); });
+            return block_count(c, counts, turn);
+        };
+        // the want-th largest value, of those that `least` let through
+        const int want = min(r.n, count([&](float f, int) { return f >= least; }));
+        uint32_t lo = order_of(least + 0.0f), hi = order_of(m + 0.0f) + 1;
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
             const float t = value_of(mid);
             if (count([&](float f, int) { return f >= t; }) >= want) lo = mid;
             else hi = mid;
         }
-        least = value_of(lo);
+        const float value = value_of(lo);
         // and the last index of those equal to it
-        const int equal = want - count([&](float f, int) { return f > least; });
-        int below = p0 * PN - 1;
-        last = min(p1 * PN, r.V) - 1;
+        const int equal = want - count([&](float f, int) { return f > value; });
+        int below = p0 * PN - 1, last = min(p1 * PN, r.V) - 1;
         while (last - below > 1) {
             const int mid = below + (last - below) / 2;
-            if (count([&](float f, int v) { return f == least && v <= mid; }) >= equal) last = mid;
+            if (count([&](float f, int v) { return f == value && v <= mid; }) >= equal) last = mid;
             else below = mid;
         }
+        found_here = 0;
+        each([&](float f, int v) { put(f, v, f > value || (f == value && v <= last)); });
+        __syncthreads();
+        if (lane == 0) counts[0][wave] = found_here;
+        __syncthreads();
     }
+    int total = 0;
+    int from[kWavesPerBlock + 1];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-        const float f = to_float(x[e / PN].v[e % PN]);
-        const int v = (p0 + (e / PN) * kBlock + int(threadIdx.x)) * PN + e % PN;
-        if (f > least || (f == least && v <= last)) found[atomicAdd(&places, 1)] = entry_of(f, v);
+    for (int w = 0; w < kWavesPerBlock; ++w) {
+        from[w] = total;
+        total += counts[0][w];
     }
-    __syncthreads();
-    double total = 0.0;
-    for (int w = 0; w < kWavesPerBlock; ++w) total += ws[w];
     const int64_t list = DIRECT ? int64_t(row) : int64_t(row) * r.parts + part;
-    if (!DIRECT && threadIdx.x == 0) lists.parts[list] = Part{total, base};
-    const double shift = DIRECT ? log(total) : 0.0;
-    for (int c = threadIdx.x; c < r.n; c += kBlock) {
-        if (c < want) {
-            const uint64_t mine = found[c];
-            int rank = 0;
-            for (int j = 0; j < want; ++j) rank += found[j] > mine;
-            const float f = value_of(uint32_t(mine >> 32));
-            const int v = int(~uint32_t(mine));
-            if (DIRECT) {
-                out.logp[list * r.n + rank] = float(share_of(r, f, base) - shift);
-                out.token[list * r.n + rank] = v;
-            } else {
-                lists.value[list * r.n + rank] = f;
-                lists.token[list * r.n + rank] = v;
-            }
-        } else if (DIRECT) {
+    double z = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+    if (near) z *= exp2(double(mk) - double(base) * double(r.k));  // what the rounding of m k left
+    if (!DIRECT && threadIdx.x == 0) lists.parts[list] = Part{z, base};
+    const double shift = DIRECT ? log(z) : 0.0;
+    // a quad ranks an entry, each of its lanes among one wave's
+    const int quad = int(threadIdx.x) / 4, sub = int(threadIdx.x) % 4;
+    const int mine_of = counts[0][sub];
+    for (int c = quad; c < total; c += kBlock / 4) {
+        int w = 0;
+#pragma unroll
+        for (int i = 1; i < kWavesPerBlock; ++i) w += c >= from[i];
+        int start = from[0];
+#pragma unroll
+        for (int i = 1; i < kWavesPerBlock; ++i) start = w == i ? from[i] : start;
+        const uint64_t mine = found[w * STRIDE + c - start];
+        int rank = 0;
+        for (int j = 0; j < mine_of; ++j) rank += found[sub * STRIDE + j] > mine;
+        rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor1, 0xF, 0xF, false);
+        rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor2, 0xF, 0xF, false);
+        if (sub != 0 || rank >= r.n) continue;
+        const float f = value_of(uint32_t(mine >> 32));
+        const int v = int(~uint32_t(mine));
+        if (DIRECT) {
+            out.logp[list * r.n + rank] = float(share_of(r, f, base) - shift);
+            out.token[list * r.n + rank] = v;
+        } else {
+            lists.value[list * r.n + rank] = f;
+            lists.token[list * r.n + rank] = v;
+        }
+    }
+    for (int c = total + int(threadIdx.x); c < r.n; c += kBlock) {
+        if (DIRECT) {
             out.logp[list * r.n + c] = -__builtin_inff();
             out.token[list * r.n + c] = -1;
         } else {
