@@ -45,10 +45,13 @@ struct Part {
 };
 
 // What the scan leaves for the join: [rows, parts] statistics, [rows, parts, n] entries.
+struct Item {
+    float x;    // -inf: none
+    int token;
+};
 struct Lists {
     Part* parts;
-    float* value;
-    int32_t* token;
+    Item* items;
 };
 
 __device__ __forceinline__ bool read_row(const Rows& r, int row) {
@@ -139,25 +142,22 @@ struct TopOut {
 // above -inf: the lowest finite value.
 template <int G>
 __device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
+    const float lowest = -__FLT_MAX__;
     auto count = [&](float t) {
         int c = 0;
 #pragma unroll
         for (int g = 0; g < G; ++g) c += __builtin_popcountll(__ballot(v[g] >= t));
         return c;
     };
-    float most = v[0], least = v[0];
+    float most = v[0], least = __builtin_inff();
 #pragma unroll
-    for (int g = 1; g < G; ++g) {
+    for (int g = 0; g < G; ++g) {
         most = fmaxf(most, v[g]);
-        least = fminf(least, v[g]);
+        if (v[g] >= lowest) least = fminf(least, v[g]);
     }
     most = wave_max(most);
     least = wave_reduce(least, [](float a, float b) { return fminf(a, b); });
-    const float lowest = -__FLT_MAX__;
-    if (!(least >= lowest)) {
-        least = lowest;
-        if (count(lowest) < r) return lowest;
-    }
+    if (count(lowest) < r) return lowest;
     uint32_t lo = order_of(least + 0.0f), hi = order_of(most + 0.0f) + 1;
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
@@ -184,7 +184,8 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     constexpr int PN = Pack<T>::N;
     constexpr int G = P == 1 || P == 2 ? 2 : 4;   // values of a lane for lists of more than 128 entries
     constexpr int ROOM = 512;                     // entries that a wave collects
-    constexpr int STRIDE = ROOM + 2;              // a quad reads the four places at once: other banks
+    constexpr int STEP = 8;
+    constexpr int STRIDE = ROOM + STEP + 2;       // a quad reads the four places at once: other banks
     __shared__ uint64_t found[kWavesPerBlock * STRIDE];
     __shared__ int counts[2][kWavesPerBlock];
     __shared__ float wm[kWavesPerBlock], wt[kWavesPerBlock];
@@ -318,6 +319,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         }
     }
     if (lane == 0) counts[0][wave] = found_here;
+    if (lane < STEP) found[wave * STRIDE + min(found_here, ROOM) + lane] = 0;
     __syncthreads();
     int most = counts[0][0];
     for (int w = 1; w < kWavesPerBlock; ++w) most = max(most, counts[0][w]);
@@ -350,6 +352,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         each([&](float f, int v) { put(f, v, f > value || (f == value && v <= last)); });
         __syncthreads();
         if (lane == 0) counts[0][wave] = found_here;
+        if (lane < STEP) found[wave * STRIDE + found_here + lane] = 0;
         __syncthreads();
     }
     int total = 0;
@@ -364,7 +367,8 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     if (near) z *= exp2(double(mk) - double(base) * double(r.k));  // what the rounding of m k left
     if (!DIRECT && threadIdx.x == 0) lists.parts[list] = Part{z, base};
     const double shift = DIRECT ? log(z) : 0.0;
-    // a quad ranks an entry, each of its lanes among one wave's
+    // a quad ranks an entry, each of its lanes among one wave's (which end in zeros, below
+    // any entry, up to a whole step)
     const int quad = int(threadIdx.x) / 4, sub = int(threadIdx.x) % 4;
     const int mine_of = counts[0][sub];
     for (int c = quad; c < total; c += kBlock / 4) {
@@ -376,7 +380,13 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         for (int i = 1; i < kWavesPerBlock; ++i) start = w == i ? from[i] : start;
         const uint64_t mine = found[w * STRIDE + c - start];
         int rank = 0;
-        for (int j = 0; j < mine_of; ++j) rank += found[sub * STRIDE + j] > mine;
+        for (int j = 0; j < mine_of; j += STEP) {
+            uint64_t other[STEP];
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) other[i] = found[sub * STRIDE + j + i];
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) rank += other[i] > mine;
+        }
         rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor1, 0xF, 0xF, false);
         rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor2, 0xF, 0xF, false);
         if (sub != 0 || rank >= r.n) continue;
@@ -386,8 +396,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
             out.logp[list * r.n + rank] = float(share_of(r, f, base) - shift);
             out.token[list * r.n + rank] = v;
         } else {
-            lists.value[list * r.n + rank] = f;
-            lists.token[list * r.n + rank] = v;
+            lists.items[list * r.n + rank] = Item{f, v};
         }
     }
     for (int c = total + int(threadIdx.x); c < r.n; c += kBlock) {
@@ -395,8 +404,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
             out.logp[list * r.n + c] = -__builtin_inff();
             out.token[list * r.n + c] = -1;
         } else {
-            lists.value[list * r.n + c] = -__builtin_inff();
-            lists.token[list * r.n + c] = -1;
+            lists.items[list * r.n + c] = Item{-__builtin_inff(), -1};
         }
     }
 }
@@ -404,18 +412,30 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
 // ---------------------------------------------------------------------------
 // Lists in one
 // ---------------------------------------------------------------------------
-// An entry of a list under its 64-bit key; `id` is its place among the lists.
-// Larger keys first, equal ones by their place.
+// An entry of a list: its key, and what orders equal ones: the beam, then the logit,
+// then the place among the lists (which ascends with the token among equal logits).
+// Larger is better in both; no entry has a key of 0.
 struct Entry {
-    double key;
-    int id;
+    uint64_t key, tie;
 };
-__device__ __forceinline__ Entry nothing() { return Entry{-__builtin_inf(), 0x7FFFFFFF}; }
+constexpr int kPlaceBits = 25;  // beams * spans * entries: 2^7 * 2^10 * 2^8
+__device__ __forceinline__ uint64_t tie_of(int beam, float x, int place) {
+    return uint64_t(DOT_BEAM_MAX - 1 - beam) << (32 + kPlaceBits) | uint64_t(order_of(x)) << kPlaceBits |
+           uint64_t((1 << kPlaceBits) - 1 - place);
+}
+__device__ __forceinline__ int place_of(uint64_t tie) {
+    return (1 << kPlaceBits) - 1 - int(tie & ((1u << kPlaceBits) - 1));
+}
+__device__ __forceinline__ Entry nothing() { return Entry{0, 0}; }
 __device__ __forceinline__ bool before(const Entry& a, const Entry& b) {
-    return a.key > b.key || (a.key == b.key && a.id < b.id);
+    return a.key > b.key || (a.key == b.key && a.tie > b.tie);
+}
+__device__ __forceinline__ uint64_t shuffle(uint64_t x, int mask) {
+    const uint32_t lo = __shfl_xor(uint32_t(x), mask), hi = __shfl_xor(uint32_t(x >> 32), mask);
+    return uint64_t(hi) << 32 | lo;
 }
 __device__ __forceinline__ Entry shuffle(const Entry& a, int mask) {
-    return Entry{__shfl_xor(a.key, mask), __shfl_xor(a.id, mask)};
+    return Entry{shuffle(a.key, mask), shuffle(a.tie, mask)};
 }
 
 // A wave's 64 R best entries in order: entry r * 64 + lane in e[r].
@@ -462,64 +482,243 @@ struct JoinArgs {
     uint8_t* finished;     // or NULL
 };
 
-// The lists of `lists_of` spans (BEAM: of all spans of a batch element's beams) in one.
-template <int R, bool BEAM>
-__global__ void join(Rows r, Lists lists, JoinArgs a) {
-    extern __shared__ char shared[];
+// A 64-bit key in an order of unsigned integers, of which 0 is below any.
+__device__ __forceinline__ uint64_t order_of64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
+    return b ^ (uint64_t(int64_t(b) >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double value_of64(uint64_t o) {
+    return __builtin_bit_cast(double, o ^ (o >> 63 ? 0x8000000000000000ull : ~0ull));
+}
+
+// A float that a larger key never has a smaller one of.
+__device__ __forceinline__ float float_of(double key) { return float(key); }
+
+constexpr int kJoinRoom = 1024;  // entries that are ranked
+constexpr int kJoinPad = 64;     // behind them, of nothing: a whole step of 16 lanes
+
+// Sum and maximum over the 16 lanes of a row of the wave.
+__device__ __forceinline__ double dpp_sum16(double x) {
+    auto step = [&](auto ctrl) {
+        constexpr int C = decltype(ctrl)::value;
+        const uint64_t b = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(b), C, 0xF, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), C, 0xF, 0xF, false);
+        x += __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+    };
+    step(std::integral_constant<int, kDppQuadXor1>{});
+    step(std::integral_constant<int, kDppQuadXor2>{});
+    step(std::integral_constant<int, kDppRowHalfMirror>{});
+    step(std::integral_constant<int, kDppRowMirror>{});
+    return x;
+}
+__device__ __forceinline__ float dpp_max16(float x) {
+    x = fmaxf(x, dpp_move<kDppQuadXor1>(x));
+    x = fmaxf(x, dpp_move<kDppQuadXor2>(x));
+    x = fmaxf(x, dpp_move<kDppRowHalfMirror>(x));
+    return fmaxf(x, dpp_move<kDppRowMirror>(x));
+}
+
+// LDS of a join of `waves` waves over `beams` beams with lists of n <= 64 R entries:
+// what is ranked, or in its place what is merged; then the beams.
+__host__ __device__ inline size_t join_shared_entries(int R, int waves, int entries) {
+    const int room = (entries < kJoinRoom ? entries : kJoinRoom) + kJoinPad;
+    const size_t ranked = size_t(room) * sizeof(Entry) + size_t(room + room % 2) * sizeof(int);
+    const size_t merged = entries > kJoinRoom ? size_t(waves / 2) * R * kWave * sizeof(Entry) : 0;
+    return ranked > merged ? ranked : merged;
+}
+inline size_t join_shared(int R, int waves, int beams, int entries) {
+    return join_shared_entries(R, waves, entries) + size_t(beams) * (sizeof(double) + sizeof(float) + sizeof(int));
+}
+
+// The lists of a row's spans (BEAM: of all spans of a batch element's beams) in one.
+//
+// As in the scan: each wave finds a value that its share of the n entries reaches, those
+// above the lowest of these values are collected and ranked by counting, 4 or 16 lanes an
+// entry.  The values are keys rounded to floats, which keeps their order: at least n
+// entries reach the lowest value, so the n best do.  Where too many do (ties), each wave
+// keeps its best entries while it merges list after list, and the waves' are merged.
+// EACH entries of a thread stay in registers; with 0 they are read again.
+template <int R, bool BEAM, int EACH>
+__global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    __shared__ float wt[16];
+    __shared__ int places;
     constexpr int N = R * kWave;
     const int b = batch_of_block();
     const int beams = BEAM ? r.inner : 1;
     if (b >= r.rows / beams) return;
-    const int waves = int(blockDim.x) / kWave, wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
-    Entry* held = reinterpret_cast<Entry*>(shared);                           // [waves / 2][N]
-    double* shift = reinterpret_cast<double*>(held + max(waves / 2, 1) * N);  // [beams]: what a logit's share lacks
-    float* top = reinterpret_cast<float*>(shift + beams);                     // [beams]: the largest logit
-    int* kind = reinterpret_cast<int*>(top + beams);                          // [beams]: 0 no entries, 1 lists, 2 itself
+    const int threads = int(blockDim.x), waves = threads / kWave;
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
+    const int count = beams * r.parts, entries = count * r.n;
+    const int room = min(entries, kJoinRoom);
+    Entry* ranked = reinterpret_cast<Entry*>(shared);              // [room + kJoinPad]
+    int* tokens = reinterpret_cast<int*>(ranked + room + kJoinPad);
+    Entry* held = ranked;                                          // [waves / 2][N], in their place
+    double* shift = reinterpret_cast<double*>(shared + join_shared_entries(R, waves, entries));
+    float* top = reinterpret_cast<float*>(shift + beams);    // [beams]: the largest logit
+    int* kind = reinterpret_cast<int*>(top + beams);         // [beams]: 0 no entries, 1 lists, 2 itself
+    const Item* items = lists.items + int64_t(b) * entries;
     const double kn = double(r.k) * 0.693147180559945309417;
-    for (int w = threadIdx.x; w < beams; w += blockDim.x) {
+    // The lists are in order: neighbouring entries go to different waves and lanes, so
+    // that the lanes' maxima are as if there were no order.  97 is odd: `threads` places.
+    auto entry_at = [&](int i) { return i * threads + ((int(threadIdx.x) * 97 + i * 61) & (threads - 1)); };
+    // loads that depend on nothing are on their way first
+    Item x[EACH > 0 ? EACH : 1];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) x[i] = items[min(entry_at(i), entries - 1)];
+    if (threadIdx.x == 0) places = 0;
+    for (int i = threadIdx.x; i < room + kJoinPad; i += threads) ranked[i] = nothing();
+    // the sums of the beams' rows, 16 lanes a beam
+    for (int w = int(threadIdx.x) / 16; w < beams; w += threads / 16) {
         const int row = b * beams + w;
         const bool read = read_row(r, row);
         float m = -__builtin_inff();
         double s = 0.0;
-        if (read) {
-            bool any = false;
-            for (int p = 0; p < r.parts; ++p) {
-                const Part q = lists.parts[int64_t(row) * r.parts + p];
-                // a span of nothing but -inf has a sum of 0
-                if (q.s == 0.0) continue;
-                m = any ? fmaxf(m, q.m) : q.m;
-                any = true;
-            }
-            for (int p = 0; p < r.parts; ++p) {
-                const Part q = lists.parts[int64_t(row) * r.parts + p];
-                if (q.s != 0.0) s += q.s * exp((double(q.m) - double(m)) * kn);
-            }
+        for (int p = int(threadIdx.x) % 16; read && p < r.parts; p += 16) {
+            const Part q = lists.parts[int64_t(row) * r.parts + p];
+            if (q.s == 0.0) continue;  // nothing but -inf
+            const float to = fmaxf(m, q.m);
+            if (m > -__builtin_inff()) s *= exp((double(m) - double(to)) * kn);
+            s += q.m == to ? q.s : q.s * exp((double(q.m) - double(to)) * kn);
+            m = to;
         }
-        const float score = BEAM ? r.scores[row] : 0.0f;
-        top[w] = m;
-        shift[w] = (BEAM ? double(score) : 0.0) - log(s);
-        kind[w] = read ? 1 : BEAM && r.finished && r.finished[row] && score > -__builtin_inff() ? 2 : 0;
+        const float most = dpp_max16(m);
+        if (m != most) s = m > -__builtin_inff() ? s * exp((double(m) - double(most)) * kn) : s;
+        s = dpp_sum16(s);
+        if (threadIdx.x % 16 == 0) {
+            const float score = BEAM ? r.scores[row] : 0.0f;
+            top[w] = most;
+            shift[w] = (BEAM ? double(score) : 0.0) - log(s);  // what a logit's share lacks
+            kind[w] = read ? 1 : BEAM && r.finished && r.finished[row] && score > -__builtin_inff() ? 2 : 0;
+        }
     }
     __syncthreads();
+    // The key of entry `at` of list l, of beam w: -inf where there is none.
+    auto key_of = [&](int l, int w, int at, float f) {
+        if (!BEAM) return kind[0] == 1 && f > -__builtin_inff() ? double(f) : -__builtin_inf();
+        double key = -__builtin_inf();
+        if (kind[w] == 1 && f > -__builtin_inff()) {
+            const double total = shift[w] + share_of(r, f, top[w]);
+            if (total > key) key = total;  // not NaN
+        } else if (kind[w] == 2 && l == w * r.parts && at == 0) {
+            key = double(r.scores[b * beams + w]);
+        }
+        return key;
+    };
+    auto beam_of = [&](int l) { return BEAM ? l / r.parts : 0; };
+    auto tie_at = [&](int e, int w, float f) { return tie_of(w, kind[w] == 1 ? f : 0.0f, e); };
+    // use(e, w, key, item) for all entries, whole waves at once.
+    auto each = [&](auto use) {
+        if constexpr (EACH > 0) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                if (i * threads >= entries) break;
+                const int e = min(entry_at(i), entries - 1), l = e / r.n, w = beam_of(l);
+                use(e, w, entry_at(i) < entries ? key_of(l, w, e - l * r.n, x[i].x) : -__builtin_inf(), x[i]);
+            }
+        } else {
+            // A list at a time and wave, its entries in other lanes each time.
+            constexpr int U = 4 / R;
+            for (int l0 = wave; l0 < count; l0 += U * waves) {
+                Item y[U * R];
+#pragma unroll
+                for (int i = 0; i < U * R; ++i) {
+                    const int l = min(l0 + i / R * waves, count - 1), at = i % R * kWave + ((lane + 5 * (l / 16)) & 63);
+                    y[i] = items[int64_t(l) * r.n + min(at, r.n - 1)];
+                }
+#pragma unroll
+                for (int i = 0; i < U * R; ++i) {
+                    const int l = l0 + i / R * waves, at = i % R * kWave + ((lane + 5 * (l / 16)) & 63);
+                    if (l >= count) break;
+                    const int w = beam_of(l);
+                    use(l * r.n + at, w, at < r.n ? key_of(l, w, at, y[i].x) : -__builtin_inf(), y[i]);
+                }
+            }
+        }
+    };
+    float most[1] = {-__builtin_inff()};
+    each([&](int, int, double key, Item) { most[0] = fmaxf(most[0], float_of(key)); });
+    const float reached = reached_by(most, (r.n + waves - 1) / waves);
+    if (lane == 0) wt[wave] = reached;
+    __syncthreads();
+    float least = wt[0];
+    for (int w = 1; w < waves; ++w) least = fminf(least, wt[w]);
+    each([&](int e, int w, double key, Item y) {
+        // totals below the lowest float are entries too
+        const bool in = least == -__FLT_MAX__ ? key > -__builtin_inf() : float_of(key) >= least;
+        const uint64_t all = __ballot(in);
+        if (all == 0) return;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&places, int(__builtin_popcountll(all)));
+        at = __builtin_amdgcn_readfirstlane(at) +
+             __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
+        if (in && at < kJoinRoom) {
+            ranked[at] = Entry{order_of64(key), tie_at(e, w, y.x)};
+            tokens[at] = y.token;
+        }
+    });
+    __syncthreads();
+    const int found = places;
+    auto write = [&](int to_entry, double key, int id, int token) {
+        const int64_t to = int64_t(b) * r.n + to_entry;
+        if (id < 0) {
+            a.scores[to] = -__builtin_inff();
+            a.tokens[to] = -1;
+            if (BEAM) a.beams[to] = -1;
+            if (BEAM && a.finished) a.finished[to] = 0;
+            return;
+        }
+        const int w = BEAM ? id / r.n / r.parts : 0;
+        const bool itself = BEAM && kind[w] == 2;
+        if (itself) token = a.eos;
+        a.tokens[to] = token;
+        if (BEAM) {
+            a.scores[to] = float(key);
+            a.beams[to] = w;
+            if (a.finished) a.finished[to] = itself || token == a.eos;
+        } else {
+            a.scores[to] = float(share_of(r, float(key), top[0]) + shift[0]);
+        }
+    };
+    if (found <= kJoinRoom) {
+        const int lanes = found * 16 <= threads ? 16 : 4;
+        const int sub = int(threadIdx.x) % lanes;
+        for (int c = int(threadIdx.x) / lanes; c < found; c += threads / lanes) {
+            const Entry mine = ranked[c];
+            int rank = 0;
+            for (int j = sub; j < found; j += 4 * lanes) {
+                Entry other[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) other[i] = ranked[j + i * lanes];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    rank += int(other[i].key > mine.key) | (int(other[i].key == mine.key) & int(other[i].tie > mine.tie));
+            }
+            rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor1, 0xF, 0xF, false);
+            rank += __builtin_amdgcn_update_dpp(0, rank, kDppQuadXor2, 0xF, 0xF, false);
+            if (lanes == 16) {
+                rank += __builtin_amdgcn_update_dpp(0, rank, kDppRowHalfMirror, 0xF, 0xF, false);
+                rank += __builtin_amdgcn_update_dpp(0, rank, kDppRowMirror, 0xF, 0xF, false);
+            }
+            if (sub == 0 && rank < r.n) write(rank, value_of64(mine.key), place_of(mine.tie), tokens[c]);
+        }
+        for (int e = found + int(threadIdx.x); e < r.n; e += threads) write(e, 0.0, -1, -1);
+        return;
+    }
+    __syncthreads();  // `held` takes the place of the keys
     Best<R> best;
     best.clear();
-    const int count = beams * r.parts;
     for (int l = wave; l < count; l += waves) {
-        const int w = BEAM ? l / r.parts : 0;
-        if (kind[w] == 0 || (kind[w] == 2 && l != w * r.parts)) continue;
-        const int64_t list = int64_t(b) * count + l;
         Entry other[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int at = N - 1 - (i * kWave + lane);
             other[i] = nothing();
-            if (kind[w] == 2) {
-                if (at == 0) other[i] = Entry{double(r.scores[b * beams + w]), l * r.n};
-            } else if (at < r.n) {
-                const float f = lists.value[list * r.n + at];
-                const double key = BEAM ? shift[w] + share_of(r, f, top[w]) : double(f);
-                if (key > -__builtin_inf()) other[i] = Entry{key, l * r.n + at};
-            }
+            if (at >= r.n) continue;
+            const float f = items[l * r.n + at].x;
+            const double key = key_of(l, beam_of(l), at, f);
+            if (key > -__builtin_inf()) other[i] = Entry{order_of64(key), tie_at(l * r.n + at, beam_of(l), f)};
         }
         best.merge(other);
     }
@@ -541,26 +740,8 @@ __global__ void join(Rows r, Lists lists, JoinArgs a) {
     for (int i = 0; i < R; ++i) {
         const int e = i * kWave + lane;
         if (e >= r.n) continue;
-        const int64_t to = int64_t(b) * r.n + e;
-        const Entry x = best.e[i];
-        if (x.id == 0x7FFFFFFF) {
-            a.scores[to] = -__builtin_inff();
-            a.tokens[to] = -1;
-            if (BEAM) a.beams[to] = -1;
-            if (BEAM && a.finished) a.finished[to] = 0;
-            continue;
-        }
-        const int l = x.id / r.n, w = BEAM ? l / r.parts : 0;
-        const bool itself = BEAM && kind[w] == 2;
-        const int token = itself ? a.eos : lists.token[int64_t(b) * count * r.n + x.id];
-        a.tokens[to] = token;
-        if (BEAM) {
-            a.scores[to] = float(x.key);
-            a.beams[to] = w;
-            if (a.finished) a.finished[to] = itself || token == a.eos;
-        } else {
-            a.scores[to] = float(share_of(r, float(x.key), top[0]) + shift[0]);
-        }
+        const int id = best.e[i].key == 0 ? -1 : place_of(best.e[i].tie);
+        write(e, value_of64(best.e[i].key), id, id < 0 ? -1 : items[id].token);
     }
 }
 

@@ -43,8 +43,7 @@ toplist::Lists carve(void* workspace, size_t& bytes, int64_t rows, const Split& 
     Carver c(workspace);
     toplist::Lists l{};
     l.parts = c.take<toplist::Part>(size_t(rows) * sp.parts);
-    l.value = c.take<float>(size_t(rows) * sp.parts * n);
-    l.token = c.take<int32_t>(size_t(rows) * sp.parts * n);
+    l.items = c.take<toplist::Item>(size_t(rows) * sp.parts * n);
     bytes = c.used();
     return l;
 }
@@ -68,21 +67,26 @@ void scan(int dtype, const toplist::Rows& r, const toplist::Lists& l, const topl
     else launch_scan<16, DIRECT>(dtype, r, l, o, stream);
 }
 
+// A wave for each 256 entries of a join, four at least, sixteen at most: then up to
+// four entries of a thread stay in its registers.
 template <bool BEAM>
 void join(const toplist::Rows& r, const toplist::Lists& l, const toplist::JoinArgs& a, hipStream_t stream) {
     ProfScope prof("toplist_join", stream);
-    const int beams = BEAM ? r.inner : 1, count = beams * r.parts;
-    const int waves = count > 16 ? 16 : count > 2 ? 4 : 1;
-    auto go = [&](auto tag) {
-        constexpr int R = decltype(tag)::value;
-        const size_t shared = size_t(std::max(waves / 2, 1)) * R * kWave * sizeof(toplist::Entry) +
-                              size_t(beams) * (sizeof(double) + sizeof(float) + sizeof(int));
-        hipLaunchKernelGGL((toplist::join<R, BEAM>), batch_grid(1, r.rows / beams), dim3(unsigned(waves) * kWave),
-                           shared, stream, r, l, a);
+    const int beams = BEAM ? r.inner : 1, entries = beams * r.parts * r.n;
+    const int waves = entries <= 1024 ? 4 : 16;
+    auto go = [&](auto lists, auto each) {
+        constexpr int R = decltype(lists)::value, EACH = decltype(each)::value;
+        hipLaunchKernelGGL((toplist::join<R, BEAM, EACH>), batch_grid(1, r.rows / beams),
+                           dim3(unsigned(waves) * kWave), toplist::join_shared(R, waves, beams, entries), stream, r, l, a);
     };
-    if (r.n <= 64) go(std::integral_constant<int, 1>{});
-    else if (r.n <= 128) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 4>{});
+    using std::integral_constant;
+    auto with = [&](auto lists) {
+        if (entries <= 4 * waves * kWave) go(lists, integral_constant<int, 4>{});
+        else go(lists, integral_constant<int, 0>{});
+    };
+    if (r.n <= 64) with(integral_constant<int, 1>{});
+    else if (r.n <= 128) with(integral_constant<int, 2>{});
+    else with(integral_constant<int, 4>{});
 }
 
 void set_tau(toplist::Rows& r, double tau) {

@@ -88,6 +88,22 @@ def test_ties():
             r = check(logits, scores, k=k)
             _, beams, tokens, _ = oracle.beam_step(array(logits), scores, k)
             assert np.array_equal(r.beams.cpu().numpy(), beams) and np.array_equal(r.tokens.cpu().numpy(), tokens)
+    # totals of neighbouring logits that rounding makes equal, the larger logit behind the other in the row
+    for V in (600, 40000):
+        x = torch.full((1, 3, V), -5.0)
+        near = 1.0 + 2.0**-23 * torch.arange(40)
+        for w in range(3):
+            x[0, w, torch.arange(40) * (V // 40)] = near
+            x[0, w, V - 1] = 30.0
+        r = dot_amd.beam_step(x.to(DEV), torch.zeros(1, 3, device=DEV), k=100)
+        got = [(w, v) for w, v in zip(r.beams[0].tolist(), r.tokens[0].tolist())]
+        assert got[:3] == [(0, V - 1), (1, V - 1), (2, V - 1)]
+        rest = [(w, v) for s, w, v in sorted(((-float(s), w, i) for i, (s, (w, _)) in enumerate(zip(r.scores[0], got))))[3:]
+                for v in [got[v][1]]]
+        assert rest == got[3:]
+        for w in range(3):  # of one beam by logit, wherever the totals are equal
+            mine = [v for u, v in got[3:] if u == w]
+            assert mine == sorted(mine, reverse=True)
     # rows that lie at other offsets tie all the same
     V, W = 1001, 7
     flat = torch.zeros(W * (V + 3), dtype=torch.bfloat16, device=DEV)
