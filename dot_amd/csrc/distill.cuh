@@ -62,12 +62,6 @@ __device__ __forceinline__ int named(const Rows& r, const Teacher& t, int64_t en
     return v >= 0 && v < r.V && !(t.logp[entry] == -__builtin_inff()) ? int(v) : -1;
 }
 
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
-    return x;
-}
-
 __device__ __forceinline__ void leave_out(const Out& o, int64_t at) {
     if (o.reduction == DOT_REDUCE_NONE) o.out[at] = 0.0f;
     else o.values[at] = Value{0.0, 0, 0};

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     } own[kWavesPerBlock] __attribute__((aligned(16)));
     __shared__ int counts[2][kWavesPerBlock];
     __shared__ float wm[kWavesPerBlock], wt[kWavesPerBlock];
-    __shared__ double ws[kWavesPerBlock];
+    __shared__ double ws[kWavesPerBlock], wo[kWavesPerBlock];
     const int row = batch_of_block(), part = int(blockIdx.x);
     if (row >= r.rows) return;
     if (!read_row(r, row)) {
@@ -238,14 +238,35 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
                 if (p0 + u * kBlock + int(threadIdx.x) == whole) x[u] = last;
         }
     }
+    // Maxima and terms in one pass.  The terms are relative to the largest logit of the
+    // wave's first packs: it is near the largest of all, or the sum is formed again below.
+    // x k - m k takes one rounding where m k has digits behind the point.
     float pm[P];  // the largest logit of each pack
-    float m = -__builtin_inff();
+    float m = -__builtin_inff(), mk = 0.0f;
+    bool near = true;
+    double s = 0.0;
 #pragma unroll
     for (int u = 0; u < P; ++u) {
-        pm[u] = to_float(x[u].v[0]);
+        if (u > P / 2 && u * kBlock >= p1 - p0) {  // nothing but -inf
+            pm[u] = -__builtin_inff();
+            continue;
+        }
+        float f[PN];
 #pragma unroll
-        for (int i = 1; i < PN; ++i) pm[u] = fmaxf(pm[u], to_float(x[u].v[i]));
+        for (int i = 0; i < PN; ++i) f[i] = to_float(x[u].v[i]);
+        pm[u] = f[0];
+#pragma unroll
+        for (int i = 1; i < PN; ++i) pm[u] = fmaxf(pm[u], f[i]);
         m = fmaxf(m, pm[u]);
+        if (u == 0) {
+            const float first = wave_max(m);
+            mk = first == -__builtin_inff() ? 0.0f : first * r.k;
+            near = fabsf(mk) < 65536.0f;
+            if (!near) mk = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < PN; ++i) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i], r.k, -mk));
+        s += double(pairwise<PN>(f));
     }
     const int share = (r.n + kWavesPerBlock - 1) / kWavesPerBlock;
     float least;
@@ -264,15 +285,6 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         }
         least = reached_by(v, share);
     }
-    m = wave_max(m);
-    if (lane == 0) {
-        wm[wave] = m;
-        wt[wave] = least;
-    }
-    __syncthreads();
-    m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    least = fminf(fminf(wt[0], wt[1]), fminf(wt[2], wt[3]));
-    const float base = m == -__builtin_inff() ? 0.0f : m;
     // The span again from the caches, for what is rare.  All lanes of a wave go round
     // together: `use` may hold ballots.
     auto each = [&](auto use) {
@@ -289,27 +301,25 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
             }
         }
     };
-    // the sum; x k - m k in one rounding where m k has digits behind the point
-    double s = 0.0;
-    const float mk = base * r.k;
-    const bool near = fabsf(mk) < 65536.0f;
-#pragma unroll
-    for (int u = 0; u < P; ++u) hold(x[u]);
-    if (near) {
-#pragma unroll
-        for (int u = 0; u < P; ++u) {
-            if (u > P / 2 && u * kBlock >= p1 - p0) break;  // nothing but -inf
-            float e[PN];
-#pragma unroll
-            for (int i = 0; i < PN; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(to_float(x[u].v[i]), r.k, -mk));
-            s += double(pairwise<PN>(e));
-        }
-    } else {
-        each([&](float f, int) { s += double(__builtin_amdgcn_exp2f((f - base) * r.k)); });
+    m = wave_max(m);
+    // what the wave's terms are relative to, as a binary logarithm
+    double of = double(mk);
+    if (m > -__builtin_inff() && !(near && fabsf(m * r.k - mk) < 100.0f)) {
+        s = 0.0;
+        of = double(m) * double(r.k);
+        each([&](float f, int) { s += double(__builtin_amdgcn_exp2f((f - m) * r.k)); });
     }
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
-    if (lane == 0) ws[wave] = s;
+    s = wave_sum64(s);
+    if (lane == 0) {
+        wm[wave] = m;
+        wt[wave] = least;
+        ws[wave] = s;
+        wo[wave] = of;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    least = fminf(fminf(wt[0], wt[1]), fminf(wt[2], wt[3]));
+    const float base = m == -__builtin_inff() ? 0.0f : m;
 
     // Entries of -inf and NaN are below `least`.  Each wave's go to a place of its own:
     // first the packs that hold any, then, a lane an element, what is in them.
@@ -381,8 +391,11 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         __syncthreads();
     }
     const int64_t list = DIRECT ? int64_t(row) : int64_t(row) * r.parts + part;
-    double z = (ws[0] + ws[1]) + (ws[2] + ws[3]);
-    if (near) z *= exp2(double(mk) - double(base) * double(r.k));  // what the rounding of m k left
+    // the waves' sums relative to the largest logit, a lane of a quad a wave's
+    double z = ws[lane % 4];
+    if (z != 0.0) z *= exp2(wo[lane % 4] - double(base) * double(r.k));
+    z += dpp_move<kDppQuadXor1>(z);
+    z += dpp_move<kDppQuadXor2>(z);
     if (!DIRECT && threadIdx.x == 0) lists.parts[list] = Part{z, base};
     const double shift = DIRECT ? log(z) : 0.0;
     auto write = [&](int rank, uint64_t entry) {
@@ -550,22 +563,8 @@ __device__ __forceinline__ float float_of(double key) { return float(key); }
 constexpr int kJoinRoom = 1024;  // entries that are ranked
 constexpr int kJoinPad = 64;     // behind them, of nothing: a whole step of 16 lanes
 
-// Sum and maximum over the 16 lanes of a row of the wave.
-__device__ __forceinline__ double dpp_sum16(double x) {
-    auto step = [&](auto ctrl) {
-        constexpr int C = decltype(ctrl)::value;
-        const uint64_t b = __builtin_bit_cast(uint64_t, x);
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(b), C, 0xF, 0xF, false);
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), C, 0xF, 0xF, false);
-        x += __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
-    };
-    step(std::integral_constant<int, kDppQuadXor1>{});
-    step(std::integral_constant<int, kDppQuadXor2>{});
-    step(std::integral_constant<int, kDppRowHalfMirror>{});
-    step(std::integral_constant<int, kDppRowMirror>{});
-    return x;
-}
-__device__ __forceinline__ float dpp_max16(float x) {
+// The maximum over the 16 lanes of a row of the wave.
+__device__ __forceinline__ float row_max(float x) {
     x = fmaxf(x, dpp_move<kDppQuadXor1>(x));
     x = fmaxf(x, dpp_move<kDppQuadXor2>(x));
     x = fmaxf(x, dpp_move<kDppRowHalfMirror>(x));
@@ -636,9 +635,9 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
             s += q.m == to ? q.s : q.s * exp((double(q.m) - double(to)) * kn);
             m = to;
         }
-        const float most = dpp_max16(m);
+        const float most = row_max(m);
         if (m != most) s = m > -__builtin_inff() ? s * exp((double(m) - double(most)) * kn) : s;
-        s = dpp_sum16(s);
+        s = row_sum64(s);
         if (threadIdx.x % 16 == 0) {
             const float score = BEAM ? r.scores[row] : 0.0f;
             top[w] = most;

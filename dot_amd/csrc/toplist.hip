@@ -14,14 +14,18 @@ struct Split {
     int parts, per;
 };
 
-// Spans of a row: at most 16 packs a thread; fewer rows are split further, towards
-// 512 workgroups, down to one pack a thread.
-Split split_of(int64_t rows, int V, int dtype) {
+// Spans of a row: at most 16 packs a thread.  A row that is its own list (`alone`) and
+// fits a span stays whole: 8 x 32768 bf16 in one launch 8.8 us, in 64 spans and a join
+// 6.8 + 6.4.  Others are split towards 64 workgroups, down to one pack a thread; further
+// splitting makes the joins longer (256 x 131072 bf16 in 4 and 8 spans: 17.5 + 7.0 and
+// 18.2 + 8.6 us).
+Split split_of(int64_t rows, int V, int dtype, bool alone) {
     const int pn = 16 / dtype_bytes(dtype);
     const int packs = (V + pn - 1) / pn;
     const int least = (packs + kBlock * toplist::kMaxPacks - 1) / (kBlock * toplist::kMaxPacks);
+    if (alone && least == 1) return {1, packs};
     const int most = (packs + kBlock - 1) / kBlock;
-    const int64_t want = rows > 0 ? (512 + rows - 1) / rows : 1;
+    const int64_t want = rows > 0 ? (64 + rows - 1) / rows : 1;
     const int parts = int(std::min<int64_t>(std::max<int64_t>(want, least), most));
     const int per = (packs + parts - 1) / parts;
     return {(packs + per - 1) / per, per};
@@ -67,8 +71,8 @@ void scan(int dtype, const toplist::Rows& r, const toplist::Lists& l, const topl
     else launch_scan<16, DIRECT>(dtype, r, l, o, stream);
 }
 
-// A wave for each 256 entries of a join, four at least, sixteen at most: then up to
-// four entries of a thread stay in its registers.
+// Four waves for up to 1024 entries of a join, so that four of a thread stay in its
+// registers, sixteen for more.
 template <bool BEAM>
 void join(const toplist::Rows& r, const toplist::Lists& l, const toplist::JoinArgs& a, hipStream_t stream) {
     ProfScope prof("toplist_join", stream);
@@ -102,7 +106,7 @@ using namespace dot_amd;
 extern "C" size_t dot_top_logp_workspace_bytes(int B, int S, int V, int dtype, int k) {
     if (B < 0 || S < 0 || V < 1 || V > kMaxVocabulary || k < 1 || k > DOT_TOP_MAX || !known_dtype(dtype)) return 0;
     const int64_t rows = int64_t(B) * S;
-    const Split sp = split_of(rows, V, dtype);
+    const Split sp = split_of(rows, V, dtype, true);
     if (sp.parts == 1) return 0;
     size_t bytes = 0;
     carve(nullptr, bytes, rows, sp, k);
@@ -119,7 +123,7 @@ extern "C" int dot_top_logp(const dot_top_logp_args* a, dot_stream_t stream_) {
     if (rows == 0) return ok();
     if (!a->logits || !a->logp || !a->tokens)
         return fail(DOT_ERR_INVALID_ARG, "logits, logp and tokens must be non-NULL");
-    const Split sp = split_of(rows, a->V, a->dtype);
+    const Split sp = split_of(rows, a->V, a->dtype, true);
     toplist::Rows r{};
     r.logits = a->logits;
     r.so = a->stride_b;
@@ -154,7 +158,7 @@ extern "C" size_t dot_beam_step_workspace_bytes(int B, int W, int V, int dtype, 
         return 0;
     const int64_t rows = int64_t(B) * W;
     size_t bytes = 0;
-    carve(nullptr, bytes, rows, split_of(rows, V, dtype), n);
+    carve(nullptr, bytes, rows, split_of(rows, V, dtype, false), n);
     return bytes;
 }
 
@@ -171,7 +175,7 @@ extern "C" int dot_beam_step(const dot_beam_step_args* a, dot_stream_t stream_) 
     if (rows == 0) return ok();
     if (!a->logits || !a->scores || !a->out_scores || !a->out_beams || !a->out_tokens)
         return fail(DOT_ERR_INVALID_ARG, "logits, scores, out_scores, out_beams and out_tokens must be non-NULL");
-    const Split sp = split_of(rows, a->V, a->dtype);
+    const Split sp = split_of(rows, a->V, a->dtype, false);
     toplist::Rows r{};
     r.logits = a->logits;
     r.so = a->stride_b;

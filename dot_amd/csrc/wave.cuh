@@ -59,6 +59,31 @@ __device__ __forceinline__ float wave_reduce(float x, Op op) {
 __device__ __forceinline__ float wave_sum(float x) { return wave_reduce(x, OpSum{}); }
 __device__ __forceinline__ float wave_max(float x) { return wave_reduce(x, OpMax{}); }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double read_lane(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane(int(uint32_t(b)), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(int(uint32_t(b >> 32)), lane);
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+// Sums in 64 bits over the 16 lanes of a row, and over the wave (wave-uniform).
+__device__ __forceinline__ double row_sum64(double x) {
+    x += dpp_move<kDppQuadXor1>(x);
+    x += dpp_move<kDppQuadXor2>(x);
+    x += dpp_move<kDppRowHalfMirror>(x);
+    return x + dpp_move<kDppRowMirror>(x);
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+    x = row_sum64(x);
+    return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
+}
+
 // Workgroup all-reduce of one value per wave through LDS, combined in wave order.
 // `scratch` needs kMaxWaves floats; contains a barrier on entry and exit.
 template <int NWAVES, class Op>
