@@ -68,26 +68,30 @@ __device__ __forceinline__ void leave_out(const Out& o, int64_t at) {
     if (o.stats) o.stats[at] = make_float2(__builtin_nanf(""), 0.0f);
 }
 
-// The value of a position and what its gradient is made of, by one wave, from the
-// statistics of its other tokens.  `tok` holds the position's named tokens (-1 where
-// an entry names none, or one that an earlier entry names).
-template <class T>
-__device__ __forceinline__ void finish(const Rows& r, const Teacher& t, const Out& o, int64_t at,
-                                       const int (&tok)[kPerLane], const MaxSum& others) {
+// A position's entries as one wave holds them, entry i * 64 + lane in [i]: the token, -1
+// where the entry names none or one that an earlier entry names, its logit and its t.
+struct Entries {
+    int tok[kPerLane];
+    float x[kPerLane], t[kPerLane];
+};
+
+// The value of a position and what its gradient is made of, by one wave, from its
+// entries and the statistics of its other tokens.
+__device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64_t at, const Entries& in,
+                                       const MaxSum& others) {
     const int lane = int(threadIdx.x) % kWave;
-    const T* row = seqlogp::row_of<T>(r, at);
     const double kn = (double(r.k) + double(r.klo)) * 0.693147180559945309417;  // 1 / tau
-    float x[kPerLane], top = others.m, most = -__builtin_inff();
+    const int (&tok)[kPerLane] = in.tok;
+    const float (&x)[kPerLane] = in.x;
+    float top = others.m, most = -__builtin_inff();
     double tl[kPerLane], p[kPerLane];
     double mass = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-        x[i] = -__builtin_inff();
         tl[i] = p[i] = 0.0;
         if (tok[i] < 0) continue;
-        x[i] = to_float(row[tok[i]]);
-        tl[i] = double(t.logp[at * t.K + i * kWave + lane]);
-        most = fmaxf(most, float(tl[i]));
+        tl[i] = double(in.t[i]);
+        most = fmaxf(most, in.t[i]);
         top = fmaxf(top, x[i]);
     }
     const bool bucket = o.rest == DOT_REST_BUCKET, reverse = o.direction == DOT_DISTILL_REVERSE;
@@ -97,23 +101,23 @@ __device__ __forceinline__ void finish(const Rows& r, const Teacher& t, const Ou
     const double less = bucket ? 0.0 : double(wave_max(most));
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
-        if (tok[i] >= 0) mass += p[i] = exp(tl[i] - less);
+        if (tok[i] >= 0) mass += p[i] = short_exp(tl[i] - less);
     mass = wave_sum64(mass);
     double z = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
-        if (tok[i] >= 0) z += exp((double(x[i]) - double(top)) * kn);
+        if (tok[i] >= 0) z += short_exp((double(x[i]) - double(top)) * kn);
     const bool none = others.s == 0.0;  // no other token is possible
-    const double lr = none ? -__builtin_inf() : (double(others.m) - double(top)) * kn + log(others.s);
-    z = wave_sum64(z) + exp(lr);
-    const double lz = log(z), log_qr = lr - lz, qr = exp(log_qr);
+    const double lr = none ? -__builtin_inf() : (double(others.m) - double(top)) * kn + short_log(others.s);
+    z = wave_sum64(z) + short_exp(lr);
+    const double lz = short_log(z), log_qr = lr - lz, qr = short_exp(log_qr);
     double pr = 0.0;
     if (bucket) {
         pr = 1.0 - mass;
         if (pr < 0.0) pr = 0.0;
     }
     if (!bucket) {
-        const double lm = log(mass) + less;
+        const double lm = short_log(mass) + less;
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
             p[i] /= mass;
@@ -126,10 +130,10 @@ __device__ __forceinline__ void finish(const Rows& r, const Teacher& t, const Ou
         if (tok[i] < 0) continue;
         const double lq = (double(x[i]) - double(top)) * kn - lz;
         if (!reverse) value += p[i] == 0.0 ? 0.0 : p[i] * (tl[i] - lq);
-        else value += lq == -__builtin_inf() ? 0.0 : exp(lq) * (lq - tl[i]);
+        else value += lq == -__builtin_inf() ? 0.0 : short_exp(lq) * (lq - tl[i]);
     }
     value = wave_sum64(value);
-    const double log_pr = log(reverse ? fmax(pr, 0x1p-24) : pr);
+    const double log_pr = short_log(reverse ? fmax(pr, 0x1p-24) : pr);
     double other;  // gradient of the others together
     if (!reverse) {
         // where no other token is possible, what rounding leaves of P_r is nothing
@@ -148,51 +152,48 @@ __device__ __forceinline__ void finish(const Rows& r, const Teacher& t, const Ou
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
         const int e = i * kWave + lane;
-        if (e >= t.K) break;
+        if (e >= K) break;
         float g = 0.0f;
         if (tok[i] >= 0) {
-            const double lq = (double(x[i]) - double(top)) * kn - lz, q = exp(lq);
+            const double lq = (double(x[i]) - double(top)) * kn - lz, q = short_exp(lq);
             if (!reverse) g = float(q - p[i]);
             else g = lq == -__builtin_inf() ? 0.0f : float(q * (lq - tl[i] - value));
         }
-        o.at[at * t.K + e] = tok[i];
-        o.own[at * t.K + e] = g;
+        o.at[at * K + e] = tok[i];
+        o.own[at * K + e] = g;
     }
 }
 
-// The position's named tokens, each where it is named first; whether there are any.
-// `list` holds DOT_TOP_MAX ints that this wave alone uses; `twice`: some may be named twice.
-__device__ __forceinline__ bool first_named(const Rows& r, const Teacher& t, int64_t at, int* list, bool twice,
-                                            int (&tok)[kPerLane]) {
+// Leaves a token that several entries name to the first of them.  `list` holds the
+// entries' tokens, DOT_TOP_MAX of them.
+__device__ __forceinline__ void only_first(int K, const int* list, Entries& in) {
     const int lane = int(threadIdx.x) % kWave;
-    bool any = false;
+    for (int j = 0; j < K; j += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(list + j);
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        const int e = i * kWave + lane;
-        tok[i] = e < t.K ? named(r, t, at * t.K + e) : -1;
-        list[e] = tok[i];
-        any |= tok[i] >= 0;
+        for (int i = 0; i < kPerLane; ++i) {
+            if (i * kWave >= K) break;
+            const int e = i * kWave + lane;
+            if ((in.tok[i] == v.x && j < e) || (in.tok[i] == v.y && j + 1 < e) || (in.tok[i] == v.z && j + 2 < e) ||
+                (in.tok[i] == v.w && j + 3 < e))
+                in.tok[i] = -1;
+        }
     }
-    __builtin_amdgcn_wave_barrier();
-    for (int j = 0; j < (twice ? t.K : 0); ++j) {
-        const int v = list[j];
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i)
-            if (tok[i] == v && j < i * kWave + lane) tok[i] = -1;
-    }
-    return __ballot(any) != 0;
 }
 
 // The other tokens' statistics of every row, one for each split; an unsplit row is
-// finished at once.
+// finished at once.  The entries, a thread each, and the row's first packs are on their
+// way while the bits are made.
 template <class T>
 __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Part* parts) {
-    extern __shared__ uint32_t words[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t words[];
     __shared__ float sm[kWavesPerBlock];
     __shared__ double ss[kWavesPerBlock];
-    __shared__ int list[DOT_TOP_MAX];
-    __shared__ int any, twice;
-    constexpr int PN = Pack<T>::N;
+    __shared__ int list[DOT_TOP_MAX] __attribute__((aligned(16)));
+    __shared__ float list_x[DOT_TOP_MAX], list_t[DOT_TOP_MAX];
+    __shared__ int twice;
+    static_assert(DOT_TOP_MAX == kBlock, "a thread an entry");
+    constexpr int PN = Pack<T>::N, U = seqlogp::kUnroll;
     const int64_t at = blockIdx.x / unsigned(r.splits);
     const int part = int(blockIdx.x % unsigned(r.splits));
     const bool whole = r.splits == 1;
@@ -200,37 +201,51 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
         if (whole && threadIdx.x == 0) leave_out(o, at);
         return;
     }
+    const int e = int(threadIdx.x);
+    const int64_t entry = at * t.K + min(e, t.K - 1);
+    const int64_t named = int_at(t.tokens, t.tokens64, entry);
+    const float tl = t.logp[entry];
     const T* row = seqlogp::row_of<T>(r, at);
     const Span sp = seqlogp::span_of(row, r.V, part, r.splits);
     const T* body = row + sp.head;
+    const bool stream = at < r.cached, some = sp.p0 + e + (U - 1) * kBlock < sp.p1;
+    Pack<T> next[U];
+    if (some) {
+        const T* from = body + int64_t(sp.p0 + e) * PN;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            next[u] = stream ? load_pack_stream(from + u * kBlock * PN) : load_pack(from + u * kBlock * PN);
+    }
     const int v0 = part == 0 ? 0 : sp.head + sp.p0 * PN;
     const int v1 = part == r.splits - 1 ? r.V : sp.head + sp.p1 * PN;
     const int first = sp.head + sp.p0 * PN - 32;  // token of bit 0
     const int nwords = (v1 - first + 31) / 32;
     for (int i = threadIdx.x; i < nwords; i += kBlock) words[i] = 0;
-    if (threadIdx.x == 0) any = twice = 0;
-    __syncthreads();
-    for (int e = threadIdx.x; e < t.K; e += kBlock) {
-        const int v = named(r, t, at * t.K + e);
-        if (v < 0) continue;
-        any = 1;
-        if (v < v0 || v >= v1) continue;
-        const uint32_t bit = 1u << ((v - first) % 32);
-        if (atomicOr(&words[(v - first) / 32], bit) & bit) twice = 1;
-    }
-    __syncthreads();
-    if (!any) {
+    if (threadIdx.x == 0) twice = 0;
+    const int tok = e < t.K && named >= 0 && named < r.V && !(tl == -__builtin_inff()) ? int(named) : -1;
+    list[e] = tok;
+    // left out without an entry; the barrier is that of the zeros as well
+    if (!__syncthreads_or(tok >= 0)) {
         if (whole && threadIdx.x == 0) leave_out(o, at);
         return;
     }
+    float x = -__builtin_inff();
+    if (tok >= 0) {
+        if (whole) x = to_float(row[tok]);
+        if (tok >= v0 && tok < v1) {
+            const uint32_t bit = 1u << ((tok - first) % 32);
+            if (atomicOr(&words[(tok - first) / 32], bit) & bit) twice = 1;
+        }
+    }
+    MaxSum a;
     auto bit = [&](int v) { return words[(v - first) / 32] >> ((v - first) % 32) & 1u; };
     // the bits of a pack, from bit 0 on
     auto bits = [&](int p) {
         const uint32_t b = reinterpret_cast<const uint8_t*>(words)[(32 + (p - sp.p0) * PN) / 8];
         return PN == 8 ? b : (p - sp.p0) % 2 ? b >> 4 : b & 15u;
     };
-    MaxSum a;
     auto packs = [&](auto stream) {
+        auto pack = [&](int p) { return seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p) * PN); };
         auto values = [&](const Pack<T>& x, int p, float* f) {
 #pragma unroll
             for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
@@ -241,25 +256,30 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
                     if (b >> i & 1u) f[i] = -__builtin_inff();
             }
         };
-        int p = sp.p0 + int(threadIdx.x);
-        constexpr int U = seqlogp::kUnroll;
-        for (; p + (U - 1) * kBlock < sp.p1; p += U * kBlock) {
-            Pack<T> x[U];
-            float f[U * PN];
+        int p = sp.p0 + e;
+        if (some)
+            for (;; p += U * kBlock) {
+                float f[U * PN];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                x[u] = seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p + u * kBlock) * PN);
+                for (int u = 0; u < U; ++u) values(next[u], p + u * kBlock, f + u * PN);
+                const bool more = p + (2 * U - 1) * kBlock < sp.p1;
+                if (more)
 #pragma unroll
-            for (int u = 0; u < U; ++u) values(x[u], p + u * kBlock, f + u * PN);
-            a.template add<PN>(f, r);
-        }
+                    for (int u = 0; u < U; ++u) next[u] = pack(p + (U + u) * kBlock);
+                a.template add<PN>(f, r);
+                if (!more) {
+                    p += U * kBlock;
+                    break;
+                }
+            }
         for (; p < sp.p1; p += kBlock) {
             float f[PN];
-            values(seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p) * PN), p, f);
+            values(pack(p), p, f);
             a.template add<PN>(f, r);
         }
     };
-    if (at < r.cached) packs(std::true_type{});
+    __syncthreads();  // the bits are whole
+    if (stream) packs(std::true_type{});
     else packs(std::false_type{});
     auto one = [&](int v) {
         const float f[1] = {bit(v) ? -__builtin_inff() : to_float(row[v])};
@@ -270,6 +290,8 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
     const float m = wave_max(a.m);
     a.raise(m, r);
     const double s = wave_sum64(a.s);
+    list_x[e] = x;
+    list_t[e] = tl;
     if (threadIdx.x % kWave == 0) {
         sm[threadIdx.x / kWave] = m;
         ss[threadIdx.x / kWave] = s;
@@ -282,21 +304,40 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
         if (threadIdx.x == 0) parts[blockIdx.x] = Part{all.s, all.m};
         return;
     }
-    int tok[kPerLane];
-    first_named(r, t, at, list, twice, tok);
-    finish<T>(r, t, o, at, tok, all);
+    Entries in;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        in.tok[i] = list[i * kWave + e];
+        in.x[i] = list_x[i * kWave + e];
+        in.t[i] = list_t[i * kWave + e];
+    }
+    if (twice) only_first(t.K, list, in);
+    finish(r, t.K, o, at, in, all);
 }
 
 // Joins the parts of split rows, one wave a row.
 template <class T>
 __global__ __launch_bounds__(kBlock) void finish_rows(Rows r, Teacher t, Out o, const Part* parts) {
-    __shared__ int lists[kWavesPerBlock][DOT_TOP_MAX];
-    const int wave = int(threadIdx.x) / kWave;
+    __shared__ int lists[kWavesPerBlock][DOT_TOP_MAX] __attribute__((aligned(16)));
+    const int wave = int(threadIdx.x) / kWave, lane = int(threadIdx.x) % kWave;
     const int64_t at = int64_t(blockIdx.x) * kWavesPerBlock + wave;
     if (at >= int64_t(r.B) * r.S) return;
-    int tok[kPerLane];
-    if (masked(r, at) || !first_named(r, t, at, lists[wave], true, tok)) {
-        if (threadIdx.x % kWave == 0) leave_out(o, at);
+    Entries in;
+    bool any = false;
+    if (!masked(r, at)) {
+        const T* row = seqlogp::row_of<T>(r, at);
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int e = i * kWave + lane;
+            in.tok[i] = e < t.K ? named(r, t, at * t.K + e) : -1;
+            in.x[i] = in.tok[i] >= 0 ? to_float(row[in.tok[i]]) : 0.0f;
+            in.t[i] = in.tok[i] >= 0 ? t.logp[at * t.K + e] : 0.0f;
+            lists[wave][e] = in.tok[i];
+            any |= in.tok[i] >= 0;
+        }
+    }
+    if (__ballot(any) == 0) {
+        if (lane == 0) leave_out(o, at);
         return;
     }
     MaxSum all;
@@ -304,7 +345,8 @@ __global__ __launch_bounds__(kBlock) void finish_rows(Rows r, Teacher t, Out o, 
         const Part p = parts[at * r.splits + i];
         all.join(p.m, p.s, r);
     }
-    finish<T>(r, t, o, at, tok, all);
+    only_first(t.K, lists[wave], in);
+    finish(r, t.K, o, at, in, all);
 }
 
 // The positions' values of each sequence, added up.
@@ -396,31 +438,35 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
         for (int i = 0; i < PN; ++i) y.v[i] = from_float<T>(value(to_float(x.v[i])));
         store_pack_stream(out + sp.head + int64_t(p) * PN, y);
     };
+    // A named token's gradient is written over what the packs put there, soon enough to
+    // meet them in L2: behind all of the row 64 such stores cost 12 % of a row of 32768 bf16.
+    const int mine = int(threadIdx.x) < g.K ? g.at[at * g.K + threadIdx.x] : -1;
+    const T own = from_float<T>(mine >= 0 ? c * g.own[at * g.K + threadIdx.x] : 0.0f);
+    auto name = [&](int from, int to) {
+        __syncthreads();
+        if (mine >= from && mine < to) out[mine] = own;
+    };
     auto packs = [&](auto stream) {
         constexpr int U = seqlogp::kUnroll;
-        int p = sp.p0 + int(threadIdx.x);
-        for (; p + (U - 1) * kBlock < sp.p1; p += U * kBlock) {
+        int q = sp.p0;
+        for (; q + U * kBlock <= sp.p1; q += U * kBlock) {
+            const int p = q + int(threadIdx.x);
             Pack<T> x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) x[u] = pack_in(p + u * kBlock, stream);
 #pragma unroll
             for (int u = 0; u < U; ++u) pack_out(p + u * kBlock, x[u]);
+            name(sp.head + q * PN, sp.head + (q + U * kBlock) * PN);
         }
-        for (; p < sp.p1; p += kBlock) pack_out(p, pack_in(p, stream));
+        for (int p = q + int(threadIdx.x); p < sp.p1; p += kBlock) pack_out(p, pack_in(p, stream));
+        return sp.head + q * PN;
     };
-    if (at < r.cached) packs(std::true_type{});
-    else packs(std::false_type{});
+    const int behind = at < r.cached ? packs(std::true_type{}) : packs(std::false_type{});
     if (part == 0 && int(threadIdx.x) < sp.head) out[threadIdx.x] = from_float<T>(value(to_float(row[threadIdx.x])));
     const int v = sp.tail + int(threadIdx.x);
     if (part == r.splits - 1 && v < r.V) out[v] = from_float<T>(value(to_float(row[v])));
-    // the named tokens of the span, over what was just written there
-    __syncthreads();
-    const int v0 = part == 0 ? 0 : sp.head + sp.p0 * PN;
-    const int v1 = part == r.splits - 1 ? r.V : sp.head + sp.p1 * PN;
-    for (int e = threadIdx.x; e < g.K; e += kBlock) {
-        const int tok = g.at[at * g.K + e];
-        if (tok >= v0 && tok < v1) out[tok] = from_float<T>(c * g.own[at * g.K + e]);
-    }
+    name(behind, part == r.splits - 1 ? r.V : sp.head + sp.p1 * PN);
+    if (part == 0) name(0, sp.head);
 }
 
 }  // namespace distill

@@ -8,12 +8,12 @@
 namespace dot_amd {
 namespace {
 
-// Workgroups per row, as for the sequence log-probabilities, and at least as many as
-// keep the bits of a span in LDS.
-int splits_of(int B, int S, int V, int dtype) {
-    const int64_t rows = int64_t(B) * S;
+// Workgroups per row: rows alone fill the chip, fewer are split, into spans of at least two
+// packs per thread, and into as many as keep the bits of a span in LDS.
+int splits_of(int B, int S, int V, int dtype, bool backward) {
+    const int64_t rows = int64_t(B) * S, fill = backward ? 2048 : 512;
     const int packs = V / (16 / dtype_bytes(dtype));
-    const int64_t want = rows > 0 ? (2048 + rows - 1) / rows : 1;
+    const int64_t want = rows > 0 ? (fill + rows - 1) / rows : 1;
     const int64_t most = std::max(1, packs / (2 * kBlock));
     const int64_t least = (int64_t(V) + distill::kMaxSpan - 1) / distill::kMaxSpan;
     return int(std::max(std::min(want, most), least));
@@ -35,7 +35,7 @@ int check(const A* a) {
     if (a->K > DOT_TOP_MAX) return fail(DOT_ERR_UNSUPPORTED, "at most DOT_TOP_MAX tokens of a position are supported");
     // a grid dimension holds less than 2^32 threads
     if (a->V > (1 << 24) || int64_t(a->B) * a->S > (1 << 23) ||
-        int64_t(a->B) * a->S * splits_of(a->B, a->S, a->V, a->dtype) > (1 << 23))
+        int64_t(a->B) * a->S * splits_of(a->B, a->S, a->V, a->dtype, true) > (1 << 23))
         return fail(DOT_ERR_UNSUPPORTED, "V must be at most 2^24 and B * S (times V / 2^18) at most 2^23");
     if (!(a->tau > 0.0) || !std::isfinite(a->tau)) return fail(DOT_ERR_INVALID_ARG, "tau must be > 0");
     if (a->tau < 1e-20 || a->tau > 1e20) return fail(DOT_ERR_UNSUPPORTED, "tau must be in [1e-20, 1e20]");
@@ -45,7 +45,7 @@ int check(const A* a) {
 }
 
 template <class A>
-seqlogp::Rows rows_of(const A* a, bool training) {
+seqlogp::Rows rows_of(const A* a, bool training, bool backward) {
     seqlogp::Rows r{};
     r.logits = a->logits;
     r.sb = a->stride_b;
@@ -58,7 +58,7 @@ seqlogp::Rows rows_of(const A* a, bool training) {
     r.k = float(k);
     if (double(r.k) >= k) r.k = std::nextafter(r.k, 0.0f);
     r.klo = float(k - double(r.k));
-    r.splits = splits_of(a->B, a->S, a->V, a->dtype);
+    r.splits = splits_of(a->B, a->S, a->V, a->dtype, backward);
     // past the caches but for the rows that the backward begins with, as for the
     // sequence log-probabilities
     const int64_t rows = int64_t(a->B) * a->S, row_bytes = int64_t(a->V) * dtype_bytes(a->dtype);
@@ -84,7 +84,7 @@ Workspace carve(void* ws, int B, int S, int V, int dtype, int reduction) {
     Workspace w{};
     const size_t rows = size_t(B) * S;
     if (reduction != DOT_REDUCE_NONE) w.values = c.take<distill::Value>(rows);
-    const int splits = splits_of(B, S, V, dtype);
+    const int splits = splits_of(B, S, V, dtype, false);
     if (splits > 1) w.parts = c.take<seqlogp::Part>(rows * splits);
     w.bytes = c.used();
     return w;
@@ -116,7 +116,7 @@ extern "C" int dot_distill_forward(const dot_distill_fwd_args* a, dot_stream_t s
     const Workspace w = carve(a->workspace, a->B, a->S, a->V, a->dtype, a->reduction);
     if (w.bytes > 0 && (!a->workspace || a->workspace_bytes < w.bytes))
         return fail(DOT_ERR_WORKSPACE, "workspace smaller than dot_distill_forward_workspace_bytes()");
-    const seqlogp::Rows r = rows_of(a, a->row_stats != nullptr);
+    const seqlogp::Rows r = rows_of(a, a->row_stats != nullptr, false);
     const distill::Teacher t{a->tokens, a->tokens_are_int64, a->logp, a->K};
     distill::Out o{};
     o.direction = a->direction;
@@ -161,7 +161,7 @@ extern "C" int dot_distill_backward(const dot_distill_bwd_args* a, dot_stream_t 
                     "logits, row_stats, own_tokens, own_grad, grad_out and grad_logits must be non-NULL");
     if (a->reduction == DOT_REDUCE_MEAN && !a->weight)
         return fail(DOT_ERR_INVALID_ARG, "the gradient of a mean needs weight");
-    const seqlogp::Rows r = rows_of(a, true);
+    const seqlogp::Rows r = rows_of(a, true, true);
     distill::GradArgs g{};
     g.K = a->K;
     g.inv_tau = float(1.0 / a->tau);

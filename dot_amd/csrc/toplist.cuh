@@ -393,11 +393,11 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     const int64_t list = DIRECT ? int64_t(row) : int64_t(row) * r.parts + part;
     // the waves' sums relative to the largest logit, a lane of a quad a wave's
     double z = ws[lane % 4];
-    if (z != 0.0) z *= exp2(wo[lane % 4] - double(base) * double(r.k));
+    if (z != 0.0) z *= short_exp((wo[lane % 4] - double(base) * double(r.k)) * 0.693147180559945309417);
     z += dpp_move<kDppQuadXor1>(z);
     z += dpp_move<kDppQuadXor2>(z);
     if (!DIRECT && threadIdx.x == 0) lists.parts[list] = Part{z, base};
-    const double shift = DIRECT ? log(z) : 0.0;
+    const double shift = DIRECT ? short_log(z) : 0.0;
     auto write = [&](int rank, uint64_t entry) {
         const float f = value_of(uint32_t(entry >> 32));
         const int v = int(~uint32_t(entry));
@@ -631,17 +631,17 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
             const Part q = lists.parts[int64_t(row) * r.parts + p];
             if (q.s == 0.0) continue;  // nothing but -inf
             const float to = fmaxf(m, q.m);
-            if (m > -__builtin_inff()) s *= exp((double(m) - double(to)) * kn);
-            s += q.m == to ? q.s : q.s * exp((double(q.m) - double(to)) * kn);
+            if (m > -__builtin_inff()) s *= short_exp((double(m) - double(to)) * kn);
+            s += q.m == to ? q.s : q.s * short_exp((double(q.m) - double(to)) * kn);
             m = to;
         }
         const float most = row_max(m);
-        if (m != most) s = m > -__builtin_inff() ? s * exp((double(m) - double(most)) * kn) : s;
+        if (m != most) s = m > -__builtin_inff() ? s * short_exp((double(m) - double(most)) * kn) : s;
         s = row_sum64(s);
         if (threadIdx.x % 16 == 0) {
             const float score = BEAM ? r.scores[row] : 0.0f;
             top[w] = most;
-            shift[w] = (BEAM ? double(score) : 0.0) - log(s);  // what a logit's share lacks
+            shift[w] = (BEAM ? double(score) : 0.0) - short_log(s);  // what a logit's share lacks
             kind[w] = read ? 1 : BEAM && r.finished && r.finished[row] && score > -__builtin_inff() ? 2 : 0;
         }
     }

@@ -125,6 +125,35 @@ __device__ __forceinline__ float exp_compensated_below(float x) {
     return exp_compensated(x < -100.0f ? -100.0f : x);
 }
 
+// e^x of x <= 709 in 64 bits to 1e-11 of itself: 2^n e^f with f = x - n ln 2, |f| <= 0.347,
+// by the exponential series up to f^10 / 10! (the next term is below 3e-13).  14
+// instructions of 8 cycles a wave; the library's, to 1e-16, takes three times as many.
+__device__ __forceinline__ double short_exp(double x) {
+    if (x < -745.0) return 0.0;
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    constexpr double kHi = double(0.693147180559945309f), kLo = 0.693147180559945309417 - kHi;  // n kHi is exact
+    const double f = fma(-n, kLo, fma(-n, kHi, x));
+    double y = 1.0 / 3628800;
+    y = fma(y, f, 1.0 / 362880);
+    y = fma(y, f, 1.0 / 40320);
+    y = fma(y, f, 1.0 / 5040);
+    y = fma(y, f, 1.0 / 720);
+    y = fma(y, f, 1.0 / 120);
+    y = fma(y, f, 1.0 / 24);
+    y = fma(y, f, 1.0 / 6);
+    y = fma(y, f, 0.5);
+    y = fma(y, f, 1.0);
+    y = fma(y, f, 1.0);
+    return ldexp(y, int(n));
+}
+// log x of a normal float's range in 64 bits, off by 1e-11: l = logf(x) and what x e^-l is
+// beside 1, a 1e-6 at most, whose logarithm is d - d^2 / 2.
+__device__ __forceinline__ double short_log(double x) {
+    const double l = double(__logf(float(x)));
+    const double d = fma(x, short_exp(-l), -1.0);
+    return l + fma(-0.5 * d, d, d);
+}
+
 __device__ __forceinline__ float safe_exp(float x) {
     if (x < -88.0f) return 0.0f;
     return exp_compensated(fminf(x, 88.0f));
