@@ -24,7 +24,6 @@
 namespace dot_amd {
 namespace distill {
 
-using seqlogp::MaxSum;
 using seqlogp::Part;
 using seqlogp::Rows;
 using seqlogp::Span;
@@ -62,6 +61,23 @@ __device__ __forceinline__ int named(const Rows& r, const Teacher& t, int64_t en
     return v >= 0 && v < r.V && !(t.logp[entry] == -__builtin_inff()) ? int(v) : -1;
 }
 
+// s = sum 2^((x - m) k) of some logits, m one of them near the largest (-inf: of none but
+// -inf).  k is one float in the sums and everywhere else: a temperature that is off by
+// 3e-8 of itself moves a loss by that share of sum (Q - P) x / tau.
+struct Sum {
+    float m = -__builtin_inff();
+    double s = 0.0;
+    __device__ __forceinline__ void join(const Sum& b, double kn) {
+        if (b.m == -__builtin_inff() && b.s == 0.0) return;
+        const float to = fmaxf(m, b.m);
+        const double mine = s == 0.0 ? 0.0 : s * short_exp((double(m) - double(to)) * kn);
+        s = mine + b.s * short_exp((double(b.m) - double(to)) * kn);
+        m = to;
+    }
+};
+// 1 / tau
+__device__ __forceinline__ double inverse_tau(const Rows& r) { return double(r.k) * 0.693147180559945309417; }
+
 __device__ __forceinline__ void leave_out(const Out& o, int64_t at) {
     if (o.reduction == DOT_REDUCE_NONE) o.out[at] = 0.0f;
     else o.values[at] = Value{0.0, 0, 0};
@@ -78,9 +94,9 @@ struct Entries {
 // The value of a position and what its gradient is made of, by one wave, from its
 // entries and the statistics of its other tokens.
 __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64_t at, const Entries& in,
-                                       const MaxSum& others) {
+                                       const Sum& others) {
     const int lane = int(threadIdx.x) % kWave;
-    const double kn = (double(r.k) + double(r.klo)) * 0.693147180559945309417;  // 1 / tau
+    const double kn = inverse_tau(r);
     const int (&tok)[kPerLane] = in.tok;
     const float (&x)[kPerLane] = in.x;
     float top = others.m, most = -__builtin_inff();
@@ -103,14 +119,19 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
     for (int i = 0; i < kPerLane; ++i)
         if (tok[i] >= 0) mass += p[i] = short_exp(tl[i] - less);
     mass = wave_sum64(mass);
-    double z = 0.0;
+    double z = 0.0, q[kPerLane];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-        if (tok[i] >= 0) z += short_exp((double(x[i]) - double(top)) * kn);
+    for (int i = 0; i < kPerLane; ++i) {
+        q[i] = tok[i] >= 0 ? short_exp((double(x[i]) - double(top)) * kn) : 0.0;
+        z += q[i];
+    }
     const bool none = others.s == 0.0;  // no other token is possible
     const double lr = none ? -__builtin_inf() : (double(others.m) - double(top)) * kn + short_log(others.s);
-    z = wave_sum64(z) + short_exp(lr);
-    const double lz = short_log(z), log_qr = lr - lz, qr = short_exp(log_qr);
+    const double er = short_exp(lr);
+    z = wave_sum64(z) + er;
+    const double lz = short_log(z), log_qr = lr - lz, iz = 1.0 / z, qr = er * iz;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) q[i] *= iz;
     double pr = 0.0;
     if (bucket) {
         pr = 1.0 - mass;
@@ -130,7 +151,7 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
         if (tok[i] < 0) continue;
         const double lq = (double(x[i]) - double(top)) * kn - lz;
         if (!reverse) value += p[i] == 0.0 ? 0.0 : p[i] * (tl[i] - lq);
-        else value += lq == -__builtin_inf() ? 0.0 : short_exp(lq) * (lq - tl[i]);
+        else value += lq == -__builtin_inf() ? 0.0 : q[i] * (lq - tl[i]);
     }
     value = wave_sum64(value);
     const double log_pr = short_log(reverse ? fmax(pr, 0x1p-24) : pr);
@@ -146,7 +167,7 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
     if (lane == 0) {
         if (o.reduction == DOT_REDUCE_NONE) o.out[at] = float(value);
         else o.values[at] = Value{value, 1, 0};
-        if (o.stats) o.stats[at] = make_float2(others.base(), none ? 0.0f : float(other / others.s));
+        if (o.stats) o.stats[at] = make_float2(none ? 0.0f : others.m, none ? 0.0f : float(other / others.s));
     }
     if (!o.stats) return;
 #pragma unroll
@@ -155,9 +176,9 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
         if (e >= K) break;
         float g = 0.0f;
         if (tok[i] >= 0) {
-            const double lq = (double(x[i]) - double(top)) * kn - lz, q = short_exp(lq);
-            if (!reverse) g = float(q - p[i]);
-            else g = lq == -__builtin_inf() ? 0.0f : float(q * (lq - tl[i] - value));
+            const double lq = (double(x[i]) - double(top)) * kn - lz;
+            if (!reverse) g = float(q[i] - p[i]);
+            else g = lq == -__builtin_inf() ? 0.0f : float(q[i] * (lq - tl[i] - value));
         }
         o.at[at * K + e] = tok[i];
         o.own[at * K + e] = g;
@@ -208,9 +229,9 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
     const T* row = seqlogp::row_of<T>(r, at);
     const Span sp = seqlogp::span_of(row, r.V, part, r.splits);
     const T* body = row + sp.head;
-    const bool stream = at < r.cached, some = sp.p0 + e + (U - 1) * kBlock < sp.p1;
+    const bool stream = at < r.cached;
     Pack<T> next[U];
-    if (some) {
+    if (sp.p0 + U * kBlock <= sp.p1) {
         const T* from = body + int64_t(sp.p0 + e) * PN;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -237,69 +258,119 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
             if (atomicOr(&words[(tok - first) / 32], bit) & bit) twice = 1;
         }
     }
-    MaxSum a;
+    __syncthreads();  // the bits are whole
     auto bit = [&](int v) { return words[(v - first) / 32] >> ((v - first) % 32) & 1u; };
-    // the bits of a pack, from bit 0 on
-    auto bits = [&](int p) {
-        const uint32_t b = reinterpret_cast<const uint8_t*>(words)[(32 + (p - sp.p0) * PN) / 8];
-        return PN == 8 ? b : (p - sp.p0) % 2 ? b >> 4 : b & 15u;
-    };
-    auto packs = [&](auto stream) {
-        auto pack = [&](int p) { return seqlogp::row_pack<decltype(stream)::value>(body + int64_t(p) * PN); };
-        auto values = [&](const Pack<T>& x, int p, float* f) {
+    // A pack's logits, those of named tokens as -inf.
+    auto values = [&](const Pack<T>& x, int p, float* f) {
 #pragma unroll
-            for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
-            const uint32_t b = bits(p);
-            if (b) {
+        for (int i = 0; i < PN; ++i) f[i] = to_float(x.v[i]);
+        uint32_t b = reinterpret_cast<const uint8_t*>(words)[(32 + (p - sp.p0) * PN) / 8];
+        if (PN == 4) b = (p - sp.p0) % 2 ? b >> 4 : b & 15u;
+        if (b) {
 #pragma unroll
-                for (int i = 0; i < PN; ++i)
-                    if (b >> i & 1u) f[i] = -__builtin_inff();
-            }
-        };
-        int p = sp.p0 + e;
-        if (some)
-            for (;; p += U * kBlock) {
-                float f[U * PN];
-#pragma unroll
-                for (int u = 0; u < U; ++u) values(next[u], p + u * kBlock, f + u * PN);
-                const bool more = p + (2 * U - 1) * kBlock < sp.p1;
-                if (more)
-#pragma unroll
-                    for (int u = 0; u < U; ++u) next[u] = pack(p + (U + u) * kBlock);
-                a.template add<PN>(f, r);
-                if (!more) {
-                    p += U * kBlock;
-                    break;
-                }
-            }
-        for (; p < sp.p1; p += kBlock) {
-            float f[PN];
-            values(pack(p), p, f);
-            a.template add<PN>(f, r);
+            for (int i = 0; i < PN; ++i)
+                if (b >> i & 1u) f[i] = -__builtin_inff();
         }
     };
-    __syncthreads();  // the bits are whole
-    if (stream) packs(std::true_type{});
-    else packs(std::false_type{});
-    auto one = [&](int v) {
-        const float f[1] = {bit(v) ? -__builtin_inff() : to_float(row[v])};
-        a.add<1>(f, r);
+    // The unaligned logits before and behind, one a thread; then all a thread's logits,
+    // PN at a time, the first group from `next`.
+    const float none = -__builtin_inff();
+    const int tail = sp.tail + e;
+    const float before = part == 0 && e < sp.head && !bit(e) ? to_float(row[e]) : none;
+    const float behind = part == r.splits - 1 && tail < r.V && !bit(tail) ? to_float(row[tail]) : none;
+    const bool groups = sp.p0 + U * kBlock <= sp.p1;
+    auto each = [&](auto use, auto past) {
+        constexpr bool PAST = decltype(past)::value;
+        int q = sp.p0;
+        for (; q + U * kBlock <= sp.p1; q += U * kBlock) {
+            const bool more = q + 2 * U * kBlock <= sp.p1;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float f[PN];
+                values(next[u], q + u * kBlock + e, f);
+                if (more) next[u] = seqlogp::row_pack<PAST>(body + int64_t(q + (U + u) * kBlock + e) * PN);
+                use(f);
+            }
+        }
+        for (int p = q + e; p < sp.p1; p += kBlock) {
+            float f[PN];
+            values(seqlogp::row_pack<PAST>(body + int64_t(p) * PN), p, f);
+            use(f);
+        }
     };
-    if (part == 0 && int(threadIdx.x) < sp.head) one(int(threadIdx.x));
-    if (part == r.splits - 1 && sp.tail + int(threadIdx.x) < r.V) one(sp.tail + int(threadIdx.x));
-    const float m = wave_max(a.m);
-    a.raise(m, r);
-    const double s = wave_sum64(a.s);
+    // The terms are relative to the largest logit of the wave's first packs: none of them
+    // is larger than 1 by much, or the sum is formed again.
+    float m = fmaxf(before, behind);
+    if (groups) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[PN];
+            values(next[u], sp.p0 + u * kBlock + e, f);
+#pragma unroll
+            for (int i = 0; i < PN; ++i) m = fmaxf(m, f[i]);
+        }
+    } else if (sp.p0 + e < sp.p1) {
+        float f[PN];
+        values(load_pack(body + int64_t(sp.p0 + e) * PN), sp.p0 + e, f);
+#pragma unroll
+        for (int i = 0; i < PN; ++i) m = fmaxf(m, f[i]);
+    }
+    m = wave_max(m);
+    const float mk = m * r.k;
+    Sum a;
+    a.m = m;
+    // x k - m k in one rounding where m k has digits behind the point
+    const bool near = fabsf(mk) < 65536.0f;
+    if (near) {
+        auto term = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, r.k, -mk)); };
+        a.s = double(term(before)) + double(term(behind));
+        auto sum = [&](const float* f) {
+            float y[PN];
+#pragma unroll
+            for (int i = 0; i < PN; ++i) y[i] = term(f[i]);
+            a.s += double(seqlogp::pairwise<PN>(y));
+        };
+        if (stream) each(sum, std::true_type{});
+        else each(sum, std::false_type{});
+        a.s = wave_sum64(a.s);
+        a.s *= short_exp((double(mk) - double(m) * double(r.k)) * 0.693147180559945309417);  // what rounding m k left
+    }
+    if (!near || a.s > 0x1p60) {
+        // the largest logit of all, then the terms; from the caches
+        if (groups) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) next[u] = load_pack(body + int64_t(sp.p0 + u * kBlock + e) * PN);
+        }
+        m = fmaxf(before, behind);
+        each([&](const float* f) {
+            for (int i = 0; i < PN; ++i) m = fmaxf(m, f[i]);
+        }, std::false_type{});
+        m = a.m = wave_max(m);
+        const float base = m == none ? 0.0f : m;
+        auto term = [&](float x) { return double(__builtin_amdgcn_exp2f((x - base) * r.k)); };
+        a.s = term(before) + term(behind);
+        if (groups) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) next[u] = load_pack(body + int64_t(sp.p0 + u * kBlock + e) * PN);
+        }
+        each([&](const float* f) {
+            for (int i = 0; i < PN; ++i) a.s += term(f[i]);
+        }, std::false_type{});
+        a.s = wave_sum64(a.s);
+    }
     list_x[e] = x;
     list_t[e] = tl;
     if (threadIdx.x % kWave == 0) {
-        sm[threadIdx.x / kWave] = m;
-        ss[threadIdx.x / kWave] = s;
+        sm[threadIdx.x / kWave] = a.m;
+        ss[threadIdx.x / kWave] = a.s;
     }
     __syncthreads();
     if (threadIdx.x >= kWave) return;
-    MaxSum all;
-    for (int w = 0; w < kWavesPerBlock; ++w) all.join(sm[w], ss[w], r);
+    // the waves' sums, a lane of a quad each
+    Sum all{fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), ss[e % 4]};
+    if (all.s != 0.0) all.s *= short_exp((double(sm[e % 4]) - double(all.m)) * inverse_tau(r));
+    all.s += dpp_move<kDppQuadXor1>(all.s);
+    all.s += dpp_move<kDppQuadXor2>(all.s);
     if (!whole) {
         if (threadIdx.x == 0) parts[blockIdx.x] = Part{all.s, all.m};
         return;
@@ -340,10 +411,10 @@ __global__ __launch_bounds__(kBlock) void finish_rows(Rows r, Teacher t, Out o, 
         if (lane == 0) leave_out(o, at);
         return;
     }
-    MaxSum all;
+    Sum all;
     for (int i = 0; i < r.splits; ++i) {
         const Part p = parts[at * r.splits + i];
-        all.join(p.m, p.s, r);
+        all.join(Sum{p.m, p.s}, inverse_tau(r));
     }
     only_first(t.K, lists[wave], in);
     finish(r, t.K, o, at, in, all);
@@ -422,7 +493,7 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
     const float c = (g.reduction == DOT_REDUCE_MEAN ? up * g.weight[b] : up) * g.inv_tau;
     const float scale = c * st.y;
-    auto value = [&](float x) { return __builtin_amdgcn_exp2f(seqlogp::scaled(r, x - st.x)) * scale; };
+    auto value = [&](float x) { return __builtin_amdgcn_exp2f((x - st.x) * r.k) * scale; };
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     auto pack_in = [&](int p, auto stream) {
         const T* at_p = row + sp.head + int64_t(p) * PN;

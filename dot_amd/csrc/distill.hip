@@ -54,10 +54,7 @@ seqlogp::Rows rows_of(const A* a, bool training, bool backward) {
     r.S = a->S;
     r.V = a->V;
     r.mask = a->mask;
-    const double k = 1.4426950408889634074 / a->tau;
-    r.k = float(k);
-    if (double(r.k) >= k) r.k = std::nextafter(r.k, 0.0f);
-    r.klo = float(k - double(r.k));
+    r.k = float(1.4426950408889634074 / a->tau);
     r.splits = splits_of(a->B, a->S, a->V, a->dtype, backward);
     // past the caches but for the rows that the backward begins with, as for the
     // sequence log-probabilities
