@@ -6,6 +6,11 @@
 // states nor an order among the threads is needed, whatever the parents are.  Beams
 // that stay are not written, parents that no moving beam has are not read; a parent
 // of several is read from memory once.
+//
+// Bound by HBM.  16 caches of 8 x 4 x 8 x 1024 x 128 bf16, three quarters of the
+// positions in use, 0.98 GB: 205 us; with loads and stores that stay in the caches 213,
+// and with each workgroup striding through one state of its own 215 (226): neighbouring
+// workgroups at neighbouring places meet open pages of the memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -25,7 +30,6 @@ struct State {
     int64_t sb, sw, so, sp;
     int64_t outer, positions;
     uint32_t inner;  // units of a position
-    int first;       // first workgroup (of a batch element)
 };
 struct States {
     State s[kMaxStates];
@@ -60,6 +64,11 @@ struct UnitOf<16> {
     typedef uint32_t type __attribute__((ext_vector_type(4)));
 };
 
+// u / by, both at most `total`.
+__device__ __forceinline__ uint64_t quotient(uint64_t u, uint64_t by, uint64_t total) {
+    return total >> 32 ? u / by : uint64_t(uint32_t(u) / uint32_t(by));
+}
+
 // MAX: the most beams that a thread has registers for.
 template <int BYTES, int MAX>
 __global__ __launch_bounds__(kBlock) void move(States a) {
@@ -67,10 +76,6 @@ __global__ __launch_bounds__(kBlock) void move(States a) {
     __shared__ int parent[MAX];
     const int b = batch_of_block();
     if (b >= a.B) return;
-    int i = 0;
-    while (i + 1 < a.count && int(blockIdx.x) >= a.s[i + 1].first) ++i;
-    const State& s = a.s[i];
-    const int blocks = (i + 1 < a.count ? a.s[i + 1].first : int(gridDim.x)) - s.first;
     bool moves = false;
     for (int w = threadIdx.x; w < MAX; w += kBlock) {
         const int64_t p = w < a.W ? int_at(a.beams, a.beams64, int64_t(b) * a.W + w) : -1;
@@ -78,28 +83,38 @@ __global__ __launch_bounds__(kBlock) void move(States a) {
         moves |= parent[w] >= 0;
     }
     if (!__syncthreads_or(moves)) return;
-    int64_t used = s.positions;
-    if (a.lengths) used = min(max(int_at(a.lengths, a.lengths64, b), int64_t(0)), used);
-    const uint64_t run = uint64_t(used) * s.inner, total = uint64_t(s.outer) * run;
-    char* base = s.data + int64_t(b) * s.sb;
-    const bool dense = s.sp == int64_t(s.inner) * BYTES;
-    for (uint64_t u = uint64_t(int(blockIdx.x) - s.first) * kBlock + threadIdx.x; u < total;
-         u += uint64_t(blocks) * kBlock) {
-        const uint64_t o = u / run, at = u - o * run;
-        int64_t off = int64_t(o) * s.so;
-        if (dense) {
-            off += int64_t(at) * BYTES;
-        } else {
-            const uint64_t p = at / s.inner;
-            off += int64_t(p) * s.sp + int64_t(at - p * s.inner) * BYTES;
+    int64_t used = INT64_MAX;
+    if (a.lengths) used = max(int_at(a.lengths, a.lengths64, b), int64_t(0));
+    // The workgroups of a batch element go through its states side by side.
+    uint64_t chunk = blockIdx.x;
+    for (int i = 0; i < a.count; ++i) {
+        const State& s = a.s[i];
+        const uint64_t run = uint64_t(min(used, s.positions)) * s.inner, total = uint64_t(s.outer) * run;
+        const uint64_t chunks = (total + kBlock - 1) / kBlock;
+        char* base = s.data + int64_t(b) * s.sb;
+        const bool dense = s.sp == int64_t(s.inner) * BYTES;
+        for (; chunk < chunks; chunk += gridDim.x) {
+            const uint64_t u = chunk * kBlock + threadIdx.x;
+            if (u >= total) continue;
+            const uint64_t o = quotient(u, run, total), at = u - o * run;
+            int64_t off = int64_t(o) * s.so;
+            if (dense) {
+                off += int64_t(at) * BYTES;
+            } else {
+                const uint64_t p = quotient(at, s.inner, total);
+                off += int64_t(p) * s.sp + int64_t(at - p * s.inner) * BYTES;
+            }
+            U x[MAX];
+#pragma unroll
+            for (int w = 0; w < MAX; ++w)
+                if (parent[w] >= 0)
+                    x[w] = __builtin_nontemporal_load(reinterpret_cast<const U*>(base + off + int64_t(parent[w]) * s.sw));
+#pragma unroll
+            for (int w = 0; w < MAX; ++w)
+                if (parent[w] >= 0)
+                    __builtin_nontemporal_store(x[w], reinterpret_cast<U*>(base + off + int64_t(w) * s.sw));
         }
-        U x[MAX];
-#pragma unroll
-        for (int w = 0; w < MAX; ++w)
-            if (parent[w] >= 0) x[w] = *reinterpret_cast<const U*>(base + off + int64_t(parent[w]) * s.sw);
-#pragma unroll
-        for (int w = 0; w < MAX; ++w)
-            if (parent[w] >= 0) *reinterpret_cast<U*>(base + off + int64_t(w) * s.sw) = x[w];
+        chunk -= chunks;
     }
 }
 
