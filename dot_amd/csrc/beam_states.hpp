@@ -3,6 +3,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <c10/core/InferenceMode.h>
 
 #include <algorithm>
 #include <vector>
@@ -73,6 +74,8 @@ inline std::vector<dot_beam_state> beam_states(at::TensorList states, const at::
         TORCH_CHECK(t.layout() == at::kStrided && t.dim() >= 2 && t.size(0) == beams.size(0) &&
                         t.size(1) == beams.size(1) && t.device() == beams.device(),
                     "states must be dense tensors of shape [B, W, ...] on the device of beams");
+        TORCH_CHECK_VALUE(!t.is_inference() || c10::InferenceMode::is_enabled(),
+                          "states of inference mode cannot be reordered outside of it");
         TORCH_CHECK(!dim.has_value() || (d >= 2 && d < t.dim()), "dim must name a dimension behind the beams");
         out.push_back(beam_state(t, d));
     }

@@ -50,7 +50,11 @@ struct Lse {
         for (int64_t v = 0; v < V; ++v) sum += std::exp((double(x[v]) - top) / tau);
         log_sum = std::log(sum);
     }
-    double operator()(double x, double tau) const { return (x - top) / tau - log_sum; }
+    // The logits are scaled and their difference taken in fp32, in 64 bits where that ends.
+    double operator()(float x, double tau) const {
+        const float inv = 1.0f / float(tau), zx = x * inv, zm = float(top) * inv, d = zx - zm;
+        return (std::isnormal(inv) && std::isfinite(d) ? double(d) : (double(x) - top) / tau) - log_sum;
+    }
 };
 
 // The k first tokens of a row by descending logit, equal ones by the lowest token.

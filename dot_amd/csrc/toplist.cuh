@@ -128,7 +128,9 @@ __device__ __forceinline__ int block_count(int c, int (&sh)[2][kWavesPerBlock], 
 // its differences (rounded twice, 2^-24 of the logits each), so that what is next to
 // a border here is so there; in 64 bits where fp32 ends.
 __device__ __forceinline__ double share_of(const Rows& r, float x, float m) {
-    const float d = __fsub_rn(__fmul_rn(x, r.inv_tau), __fmul_rn(m, r.inv_tau));
+#pragma clang fp contract(off)
+    const float zx = x * r.inv_tau, zm = m * r.inv_tau;
+    const float d = zx - zm;
     return fabsf(d) < __builtin_inff() ? double(d) : (double(x) - double(m)) * double(r.inv_tau);
 }
 

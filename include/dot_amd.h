@@ -547,7 +547,8 @@ typedef struct {
 } dot_top_logp_args;
 
 /* The k largest logits of each position, equal ones by the lowest token, as
- * x / tau - log sum_v exp(x_v / tau).  Logits of -inf and NaN are not taken; a
+ * x / tau - log sum_v exp(x_v / tau), of which (x - max) / tau is formed in fp32
+ * (both logits scaled, then the difference) and the rest in 64 bits.  Logits of -inf and NaN are not taken; a
  * position with fewer than k others, or that is left out, has empty slots. */
 size_t dot_top_logp_workspace_bytes(int B, int S, int V, int dtype, int k);
 int dot_top_logp(const dot_top_logp_args* args, dot_stream_t stream);
@@ -575,8 +576,9 @@ typedef struct {
     int rest;                  /* DOT_REST_* */
     int reduction;             /* DOT_REDUCE_* over the positions that are not left out */
     float* out;                /* [B], or [B,S] with DOT_REDUCE_NONE (0 where left out) */
-    float* row_stats;          /* [B,S,2] out, for the backward, or NULL: the largest logit of the tokens that are
-                                  not named (NaN where left out), and the factor of their exponentials */
+    float* row_stats;          /* [B,S,2] out, for the backward, or NULL: a logit near the largest of the tokens that
+                                  are not named (NaN where left out), and the factor of their exponentials
+                                  relative to it */
     int32_t* own_tokens;       /* [B,S,K] out with row_stats: the named tokens, -1 elsewhere */
     float* own_grad;           /* [B,S,K] out with row_stats: tau times their gradient */
     float* weight;             /* [B] out with DOT_REDUCE_MEAN, for the backward: 1 / positions */
@@ -634,7 +636,8 @@ typedef struct {
 } dot_beam_step_args;
 
 /* The n largest totals score_w + x_v / tau - log sum exp(x / tau) of each batch
- * element, in 64 bits; equal ones by beam, then by descending logit, then by token.
+ * element, the log-probabilities as of dot_top_logp, added up and compared in 64
+ * bits; equal ones by beam, then by descending logit, then by token.
  * A NaN total is not taken.  Logits of closed and finished beams are not read. */
 size_t dot_beam_step_workspace_bytes(int B, int W, int V, int dtype, int n);
 int dot_beam_step(const dot_beam_step_args* args, dot_stream_t stream);

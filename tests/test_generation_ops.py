@@ -163,6 +163,30 @@ def test_cpu_beam_reorder(dtype):
     dot_amd.beam_reorder([], beams)
 
 
+@pytest.mark.parametrize("tau", [0.7, 1.0, 1.3])
+def test_cpu_logits_are_scaled_in_fp32(tau):
+    """As on the device: what beams are compared by."""
+    rng = np.random.default_rng(6)
+    x = np.full((300, 5), -np.inf, np.float32)
+    x[:, 0] = 100.0
+    x[:, 4] = 40 + 5 * rng.random(300)
+    inv = np.float32(1) / np.float32(tau)
+    r = dot_amd.top_logp(torch.as_tensor(x), 2, tau=tau)
+    assert np.array_equal(r.logp[:, 1].numpy(), x[:, 4] * inv - x[:, 0] * inv)
+    s = dot_amd.beam_step(torch.as_tensor(x[:, None]), torch.full((300, 1), -2.0), k=2, tau=tau)
+    want = (-2.0 + (x[:, 4] * inv - x[:, 0] * inv).astype(np.float64)).astype(np.float32)
+    assert np.array_equal(s.scores[:, 1].numpy(), want)
+
+
+def test_inference_states():
+    with torch.inference_mode():
+        t = torch.arange(8.0).view(1, 2, 4)
+        dot_amd.beam_reorder(t, torch.tensor([[1, 1]]))
+    assert t.tolist() == [[[4, 5, 6, 7], [4, 5, 6, 7]]]
+    with pytest.raises(ValueError, match="inference"):
+        dot_amd.beam_reorder(t, torch.tensor([[1, 0]]))
+
+
 def test_cpu_search_scores_and_losses():
     import test_beam_gpu
 

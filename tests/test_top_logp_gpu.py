@@ -131,6 +131,23 @@ def test_equal_rows_have_equal_bits_wherever_they_lie(dtype):
         assert (r.logp == r.logp[:1]).all() and (r.tokens == r.tokens[:1]).all()
 
 
+@pytest.mark.parametrize("V", [2, 40000])
+@pytest.mark.parametrize("tau", [0.7, 1.0, 1.3])
+def test_logits_are_scaled_in_fp32(tau, V):
+    """Each scaled logit and the difference from the largest one take a rounding of fp32, as in a program that scales
+    its logits so: beams are compared by what these differences are.  Next to a logit of 100 the others' terms are
+    below 2^-53 of its own, so that log-probabilities are the differences themselves."""
+    rng = np.random.default_rng(6)
+    x = np.full((300, V), -np.inf, np.float32)
+    x[:, 0] = 100.0
+    x[:, V - 1] = 40 + 5 * rng.random(300)
+    inv = np.float32(1) / np.float32(tau)
+    want = x[:, V - 1] * inv - x[:, 0] * inv
+    assert want.dtype == np.float32
+    r = dot_amd.top_logp(torch.as_tensor(x).to(DEV), 2, tau=tau)
+    assert (r.tokens[:, 1] == V - 1).all() and np.array_equal(r.logp[:, 1].cpu().numpy(), want)
+
+
 def test_empty():
     for B, S in ((0, 4), (3, 0), (0, 0)):
         r = dot_amd.top_logp(torch.zeros(B, S, 10, device=DEV), 3)
