@@ -184,7 +184,8 @@ __device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
 template <class T, int P, bool DIRECT>
 __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut out) {
     constexpr int PN = Pack<T>::N;
-    constexpr int G = P == 1 || P == 2 ? 2 : 4;   // values of a lane for lists of more than 128 entries
+    constexpr int LONG = 64;                      // entries of a list, above which
+    constexpr int G = P == 1 || P == 2 ? 2 : 4;   // a lane has so many values to find what is reached
     constexpr int ROOM = 512;                     // entries that a wave collects
     constexpr int STEP = 8;
     constexpr int HELD = 128;                     // packs that a wave looks into
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     }
     const int share = (r.n + kWavesPerBlock - 1) / kWavesPerBlock;
     float least;
-    if (r.n <= 128) {
+    if (r.n <= LONG) {
         const float v[1] = {m};
         least = reached_by(v, share);
     } else {
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     // wave orders its own by counting, then finds each one's place among the others' by
     // halving.  550 x 50021 fp32, n 20: 26.9 and 28.5 us, n 128: 49.9 and 38.8;
     // 2200 x 65536, n 64: 108 and 111.
-    if (r.n <= 64) {
+    if (r.n <= LONG) {
         for (int c = int(threadIdx.x) / 4; c < total; c += kBlock / 4) {
             int w = 0, at = c;
 #pragma unroll
@@ -618,9 +619,17 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     // that the lanes' maxima are as if there were no order.  97 is odd: `threads` places.
     auto entry_at = [&](int i) { return i * threads + ((int(threadIdx.x) * 97 + i * 61) & (threads - 1)); };
     // loads that depend on nothing are on their way first
-    Item x[EACH > 0 ? EACH : 1];
+    constexpr int U = 12;  // lists of a wave
+    Item x[EACH > 0 ? EACH : U];
+    const int first = __builtin_amdgcn_readfirstlane(wave);
+    if constexpr (EACH > 0) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) x[i] = items[min(entry_at(i), entries - 1)];
+        for (int i = 0; i < EACH; ++i) x[i] = items[min(entry_at(i), entries - 1)];
+    } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            x[i] = items[int64_t(min(first + i * waves, count - 1)) * r.n + min(lane, r.n - 1)];
+    }
     if (threadIdx.x == 0) places = 0;
     for (int i = threadIdx.x; i < room + kJoinPad; i += threads) ranked[i] = nothing();
     // the sums of the beams' rows, 16 lanes a beam
@@ -674,20 +683,22 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
             }
         } else {
             // A list at a time and wave, as far as its entries reach `least`.
-            for (int l0 = __builtin_amdgcn_readfirstlane(wave); l0 < count; l0 += 4 * waves) {
-                Item y[4];
+            for (int l0 = first; l0 < count; l0 += U * waves) {
+                if (l0 != first)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[i] = items[int64_t(min(l0 + i * waves, count - 1)) * r.n + min(lane, r.n - 1)];
+                    for (int i = 0; i < U; ++i)
+                        x[i] = items[int64_t(min(l0 + i * waves, count - 1)) * r.n + min(lane, r.n - 1)];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < U; ++i) {
                     const int l = l0 + i * waves;
                     if (l >= count) break;
                     const int w = beam_of(l);
-                    for (int at = lane; at - lane < r.n; at += kWave) {
-                        const Item z = at < kWave ? y[i] : items[int64_t(l) * r.n + min(at, r.n - 1)];
-                        const double key = at < r.n ? key_of(l, w, at, z.x) : -__builtin_inf();
-                        if (use(l * r.n + at, w, key, z) >> (kWave - 1) == 0) break;  // nor does any behind it
+                    const double key = lane < r.n ? key_of(l, w, lane, x[i].x) : -__builtin_inf();
+                    if (use(l * r.n + lane, w, key, x[i]) >> (kWave - 1) == 0) continue;  // nor does any behind it
+                    for (int at = kWave + lane; at - lane < r.n; at += kWave) {
+                        const Item z = items[int64_t(l) * r.n + min(at, r.n - 1)];
+                        const double more = at < r.n ? key_of(l, w, at, z.x) : -__builtin_inf();
+                        if (use(l * r.n + at, w, more, z) >> (kWave - 1) == 0) break;
                     }
                 }
             }
