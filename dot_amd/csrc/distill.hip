@@ -9,7 +9,9 @@ namespace dot_amd {
 namespace {
 
 // Workgroups per row: rows alone fill the chip, fewer are split, into spans of at least two
-// packs per thread, and into as many as keep the bits of a span in LDS.
+// packs per thread, and into as many as keep the bits of a span in LDS.  The forward is
+// split for fewer workgroups, since its parts are joined by a launch more (774 rows of
+// 50021 fp32 whole 25.5 us, in 3 parts 22.6 + 15.2).
 int splits_of(int B, int S, int V, int dtype, bool backward) {
     const int64_t rows = int64_t(B) * S, fill = backward ? 2048 : 512;
     const int packs = V / (16 / dtype_bytes(dtype));
