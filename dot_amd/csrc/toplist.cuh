@@ -19,6 +19,8 @@
 // the scan, 4.9 TB/s, the rate of a large copy, and 23 us in the join.
 #pragma once
 
+#include <type_traits>
+
 #include "elem.cuh"
 #include "row.cuh"
 #include "wave.cuh"
@@ -606,8 +608,8 @@ inline size_t join_shared(int R, int waves, int beams, int entries) {
 //
 // One workgroup a list, so bound by its latency: the sums of the spans, a bound, what
 // reaches it, the ranks.  4 beams, 8 entries and 16 spans each 4.9 us; 8 beams, 16
-// entries and 4 spans 7.4; 48 beams, 96 entries and 4 spans 18.6; 4096 rows of 4 spans
-// and 64 entries 22, 999 of 128 entries 12.4.
+// entries and 4 spans 6.9; 48 beams, 96 entries and 4 spans 18.3; 4096 rows of 4 spans
+// and 64 entries 20 to 24, 999 of 128 entries 12.
 template <int R, bool BEAM, int EACH>
 __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
@@ -685,58 +687,55 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     };
     auto beam_of = [&](int l) { return BEAM ? l / r.parts : 0; };
     auto tie_at = [&](int e, int w, float f) { return tie_of(w, kind[w] == 1 ? f : 0.0f, e); };
-    // use(e, w, key, item) for all entries, whole waves at once; it returns the lanes that
-    // are still of interest.
-    auto each = [&](auto use) {
-        if constexpr (EACH > 0) {
+    // Of K entries of each lane those that reach `least` go to the ranked ones, one atomic a
+    // wave; which of the K the last lane has among them, by bits.
+    float least = 0.0f;
+    auto collect = [&](auto many, const int* e, const int* w, const double* key, const Item* y) {
+        constexpr int K = decltype(many)::value;
+        uint64_t all[K];
+        int total = 0, last = 0;
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                if (i * threads >= entries) break;
-                const int e = min(entry_at(i), entries - 1), l = e / r.n, w = beam_of(l);
-                use(e, w, entry_at(i) < entries ? key_of(l, w, e - l * r.n, x[i].x) : -__builtin_inf(), x[i]);
-            }
-        } else {
-            // A list at a time and wave, as far as its entries reach `least`.  The code runs
-            // once and comes from memory, so it is short: U lists at a time, the next ones on
-            // their way, and one copy for what lies behind the first 64 entries (5 batch
-            // elements, 48 beams of 4 lists of 96: 18.6 us; twelve lists at once 19.7).
-#pragma unroll 1
-            for (int l0 = first; l0 < count; l0 += U * waves) {
-                Item next[U];
-#pragma unroll
-                for (int i = 0; i < U; ++i) next[i] = first_of(l0 + (U + i) * waves);
-                int more = 0;
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int l = l0 + i * waves;
-                    if (l >= count) break;
-                    const int w = beam_of(l);
-                    const double key = lane < r.n ? key_of(l, w, lane, x[i].x) : -__builtin_inf();
-                    more |= int(use(l * r.n + lane, w, key, x[i]) >> (kWave - 1)) << i;
-                }
-#pragma unroll 1
-                for (; more && r.n > kWave; more &= more - 1) {
-                    const int l = l0 + __builtin_ctz(more) * waves, w = beam_of(l);
-#pragma unroll 1
-                    for (int at = kWave + lane; at - lane < r.n; at += kWave) {
-                        const Item z = items[int64_t(l) * r.n + min(at, r.n - 1)];
-                        const double key = at < r.n ? key_of(l, w, at, z.x) : -__builtin_inf();
-                        if (use(l * r.n + at, w, key, z) >> (kWave - 1) == 0) break;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < U; ++i) x[i] = next[i];
-            }
+        for (int i = 0; i < K; ++i) {
+            // totals below the lowest float are entries too
+            all[i] = __ballot(least == -__FLT_MAX__ ? key[i] > -__builtin_inf() : float_of(key[i]) >= least);
+            total += __builtin_popcountll(all[i]);
+            last |= int(all[i] >> (kWave - 1)) << i;
         }
+        if (total == 0) return last;
+        int from = 0;
+        if (lane == 0) from = atomicAdd(&places, total);
+        from = __builtin_amdgcn_readfirstlane(from);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            if (all[i] == 0) continue;
+            const int at = from + __builtin_amdgcn_mbcnt_hi(uint32_t(all[i] >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo(uint32_t(all[i]), 0));
+            if ((all[i] >> lane & 1u) && at < kJoinRoom) {
+                ranked[at] = Entry{order_of64(key[i]), tie_at(e[i], w[i], y[i].x)};
+                tokens[at] = y[i].token;
+            }
+            from += __builtin_popcountll(all[i]);
+        }
+        return last;
     };
     // Keys that at least n entries reach the lowest of: each thread's largest, of all
     // entries or (EACH = 0) of the first few of each list, one a thread and 2 n at least.
+    constexpr int K = EACH > 0 ? EACH : U;
+    int e[K], w[K];
+    double key[K];
     float most[1] = {-__builtin_inff()};
     if constexpr (EACH > 0) {
-        each([&](int, int, double key, Item) {
-            most[0] = fmaxf(most[0], float_of(key));
-            return uint64_t(0);
-        });
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            e[i] = w[i] = 0;
+            key[i] = -__builtin_inf();
+            if (i * threads >= entries) continue;
+            e[i] = min(entry_at(i), entries - 1);
+            const int l = e[i] / r.n;
+            w[i] = beam_of(l);
+            if (entry_at(i) < entries) key[i] = key_of(l, w[i], e[i] - l * r.n, x[i].x);
+            most[0] = fmaxf(most[0], float_of(key[i]));
+        }
     } else {
         const int heads = min(r.n, (max(2 * r.n, threads) + count - 1) / count);
         for (int i = lane * waves + wave; i < count * heads; i += threads) {
@@ -747,23 +746,43 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     const float reached = reached_by(most, (r.n + waves - 1) / waves);
     if (lane == 0) wt[wave] = reached;
     __syncthreads();
-    float least = wt[0];
-    for (int w = 1; w < waves; ++w) least = fminf(least, wt[w]);
-    each([&](int e, int w, double key, Item y) {
-        // totals below the lowest float are entries too
-        const bool in = least == -__FLT_MAX__ ? key > -__builtin_inf() : float_of(key) >= least;
-        const uint64_t all = __ballot(in);
-        if (all == 0) return all;
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&places, int(__builtin_popcountll(all)));
-        at = __builtin_amdgcn_readfirstlane(at) +
-             __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
-        if (in && at < kJoinRoom) {
-            ranked[at] = Entry{order_of64(key), tie_at(e, w, y.x)};
-            tokens[at] = y.token;
+    least = wt[0];
+    for (int i = 1; i < waves; ++i) least = fminf(least, wt[i]);
+    if constexpr (EACH > 0) {
+        collect(std::integral_constant<int, K>{}, e, w, key, x);
+    } else {
+        // A list at a time and wave, as far as its entries reach `least`.  The code runs
+        // once and comes from memory, so it is short: U lists at a time, the next ones on
+        // their way, and one copy for what lies behind the first 64 entries (5 batch
+        // elements, 48 beams of 4 lists of 96: 18.3 us; twelve lists at once 1 us more).
+#pragma unroll 1
+        for (int l0 = first; l0 < count; l0 += U * waves) {
+            Item next[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) next[i] = first_of(l0 + (U + i) * waves);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int l = l0 + i * waves;
+                w[i] = beam_of(min(l, count - 1));
+                e[i] = l * r.n + lane;
+                key[i] = l < count && lane < r.n ? key_of(l, w[i], lane, x[i].x) : -__builtin_inf();
+            }
+            int more = collect(std::integral_constant<int, U>{}, e, w, key, x);
+#pragma unroll 1
+            for (; more && r.n > kWave; more &= more - 1) {
+                const int l = l0 + __builtin_ctz(more) * waves, wl = beam_of(l);
+#pragma unroll 1
+                for (int at = kWave + lane; at - lane < r.n; at += kWave) {
+                    const Item z = items[int64_t(l) * r.n + min(at, r.n - 1)];
+                    const double one = at < r.n ? key_of(l, wl, at, z.x) : -__builtin_inf();
+                    const int place = l * r.n + at;
+                    if (!collect(std::integral_constant<int, 1>{}, &place, &wl, &one, &z)) break;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) x[i] = next[i];
         }
-        return all;
-    });
+    }
     __syncthreads();
     const int found = places;
     auto write = [&](int to_entry, double key, int id, int token) {
