@@ -182,8 +182,9 @@ __device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
 // One span of a row.  DIRECT: the row is one span, and its list the output.
 //
 // Each wave finds a value that its share of the n entries reaches, from the maxima of
-// its lanes (of parts of them for long lists); the lowest of the four values is reached
-// by n entries of the span at least, and by few more on logits in no particular order.
+// its lanes (of parts of them where its share is above a quarter of its lanes); the
+// lowest of the four values is reached by n entries of the span at least, and by few more
+// on logits in no particular order.
 // Those are collected, each wave in a place of its own, and ranked by counting.  Where
 // they are too many (ties, orders in which the largest lie in few lanes), the n-th
 // largest entry is found by bisection over all of them instead.
@@ -195,11 +196,11 @@ __device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
 template <class T, int P, bool DIRECT>
 __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut out) {
     constexpr int PN = Pack<T>::N;
-    constexpr int LONG = 64;                      // entries of a list, above which
-    constexpr int G = P == 1 || P == 2 ? 2 : 4;   // a lane has so many values to find what is reached
-    constexpr int ROOM = 512;                     // entries that a wave collects
+    constexpr int LONG = 64;   // entries of a list above which the waves' are put in order first
+    constexpr int G = 4;       // values of a lane to find what is reached, where one is too few
+    constexpr int ROOM = 512;  // entries that a wave collects
     constexpr int STEP = 8;
-    constexpr int HELD = 128;                     // packs that a wave looks into
+    constexpr int HELD = 204;  // packs that a wave looks into: for 256 entries 128 are too few now and then
     __shared__ uint64_t found[kWavesPerBlock][ROOM + STEP];
     // a wave's packs, and when it is through with them its entries in order
     __shared__ union {
@@ -282,17 +283,36 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         for (int i = 0; i < PN; ++i) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i], r.k, -mk));
         s += double(pairwise<PN>(f));
     }
-    const int share = (r.n + kWavesPerBlock - 1) / kWavesPerBlock;
+    // The wave's share of the n entries, by what it has of the span's elements (16 rows of
+    // 2050 bf16 in 2 spans, 16 entries: 5.6 us, by equal shares 93, nearly all being ranked).
+    // A wave of a few packs beside full ones has none: the largest of so few is often small.
+    int np = p1 - p0, elements = min(p1 * PN, r.V) - p0 * PN;
+    if (np > kWave && np < kBlock && np % kWave > 0 && np % kWave < kWave / 4) {
+        np -= np % kWave;
+        elements = np * PN;
+    }
+    const int at_wave = __builtin_amdgcn_readfirstlane(wave);
+    const int has = np / kBlock * kWave + min(max(np % kBlock - at_wave * kWave, 0), kWave);
+    const int missing = (np - 1) % kBlock / kWave == at_wave ? np * PN - elements : 0;  // of the last pack
+    const int share = (r.n * (has * PN - missing) + elements - 1) / elements;
     float least;
-    if (r.n <= LONG) {
+    if (has == 0) {
+        least = __builtin_inff();
+    } else if (share * 4 <= min(has, kWave)) {
         const float v[1] = {m};
         least = reached_by(v, share);
     } else {
         float v[G];
-        if constexpr (P == 1) {
-            v[0] = v[1] = -__builtin_inff();
+        if constexpr (P <= 2) {
 #pragma unroll
-            for (int i = 0; i < PN; ++i) v[i % 2] = fmaxf(v[i % 2], to_float(x[0].v[i]));
+            for (int g = 0; g < G; ++g) v[g] = -__builtin_inff();
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+#pragma unroll
+                for (int i = 0; i < PN; ++i) {
+                    const int g = i % (G / P) * P + u;
+                    v[g] = fmaxf(v[g], to_float(x[u].v[i]));
+                }
         } else {
 #pragma unroll
             for (int u = 0; u < P; ++u) v[u % G] = u < G ? pm[u] : fmaxf(v[u % G], pm[u]);
@@ -743,48 +763,111 @@ __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
             most[0] = fmaxf(most[0], float_of(key_of(l, beam_of(l), at, items[int64_t(l) * r.n + at].x)));
         }
     }
-    const float reached = reached_by(most, (r.n + waves - 1) / waves);
+    // one value of a lane where that is half of them at most, or there are no others (256
+    // rows of 2 lists of 256: 19.5 us, of one value 41; 999 of 4 lists of 128: 13.1 and 12.0)
+    const int share = (r.n + waves - 1) / waves;
+    float reached;
+    if (EACH == 0 || share * 2 <= kWave) {
+        reached = reached_by(most, share);
+    } else {
+        float v[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) v[i] = float_of(key[i]);
+        reached = reached_by(v, share);
+    }
     if (lane == 0) wt[wave] = reached;
     __syncthreads();
     least = wt[0];
     for (int i = 1; i < waves; ++i) least = fminf(least, wt[i]);
-    if constexpr (EACH > 0) {
-        collect(std::integral_constant<int, K>{}, e, w, key, x);
-    } else {
-        // A list at a time and wave, as far as its entries reach `least`.  The code runs
-        // once and comes from memory, so it is short: U lists at a time, the next ones on
-        // their way, and one copy for what lies behind the first 64 entries (5 batch
-        // elements, 48 beams of 4 lists of 96: 18.3 us; twelve lists at once 1 us more).
+    int found;
+    for (int again = 0;; ++again) {
+        if constexpr (EACH > 0) {
+            collect(std::integral_constant<int, K>{}, e, w, key, x);
+        } else {
+            // A list at a time and wave, as far as its entries reach `least`.  The code runs
+            // once and comes from memory, so it is short: U lists at a time, the next ones on
+            // their way, and one copy for what lies behind the first 64 entries (5 batch
+            // elements, 48 beams of 4 lists of 96: 18.3 us; twelve lists at once 1 us more).
 #pragma unroll 1
-        for (int l0 = first; l0 < count; l0 += U * waves) {
-            Item next[U];
+            for (int l0 = first; l0 < count; l0 += U * waves) {
+                Item next[U];
 #pragma unroll
-            for (int i = 0; i < U; ++i) next[i] = first_of(l0 + (U + i) * waves);
+                for (int i = 0; i < U; ++i) next[i] = first_of(l0 + (U + i) * waves);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int l = l0 + i * waves;
-                w[i] = beam_of(min(l, count - 1));
-                e[i] = l * r.n + lane;
-                key[i] = l < count && lane < r.n ? key_of(l, w[i], lane, x[i].x) : -__builtin_inf();
-            }
-            int more = collect(std::integral_constant<int, U>{}, e, w, key, x);
-#pragma unroll 1
-            for (; more && r.n > kWave; more &= more - 1) {
-                const int l = l0 + __builtin_ctz(more) * waves, wl = beam_of(l);
-#pragma unroll 1
-                for (int at = kWave + lane; at - lane < r.n; at += kWave) {
-                    const Item z = items[int64_t(l) * r.n + min(at, r.n - 1)];
-                    const double one = at < r.n ? key_of(l, wl, at, z.x) : -__builtin_inf();
-                    const int place = l * r.n + at;
-                    if (!collect(std::integral_constant<int, 1>{}, &place, &wl, &one, &z)) break;
+                for (int i = 0; i < U; ++i) {
+                    const int l = l0 + i * waves;
+                    w[i] = beam_of(min(l, count - 1));
+                    e[i] = l * r.n + lane;
+                    key[i] = l < count && lane < r.n ? key_of(l, w[i], lane, x[i].x) : -__builtin_inf();
                 }
-            }
+                int more = collect(std::integral_constant<int, U>{}, e, w, key, x);
+#pragma unroll 1
+                for (; more && r.n > kWave; more &= more - 1) {
+                    const int l = l0 + __builtin_ctz(more) * waves, wl = beam_of(l);
+#pragma unroll 1
+                    for (int at = kWave + lane; at - lane < r.n; at += kWave) {
+                        const Item z = items[int64_t(l) * r.n + min(at, r.n - 1)];
+                        const double one = at < r.n ? key_of(l, wl, at, z.x) : -__builtin_inf();
+                        const int place = l * r.n + at;
+                        if (!collect(std::integral_constant<int, 1>{}, &place, &wl, &one, &z)) break;
+                    }
+                }
 #pragma unroll
-            for (int i = 0; i < U; ++i) x[i] = next[i];
+                for (int i = 0; i < U; ++i) x[i] = next[i];
+            }
+        }
+        __syncthreads();
+        found = places;
+        if (found <= kJoinRoom || again == 4) break;
+        // Too many: some beams are far better than others, and their lists go deeper than
+        // what the bound was taken from.  n of the entries that were collected, one of each
+        // of 1024 threads, give a better one (16 batch elements, 64 beams of 256 entries, 8 of
+        // them far ahead: 31 us, by the merging below 43).
+        const float one[1] = {float_of(value_of64(ranked[lane * waves + wave].key))};
+        const float better = reached_by(one, share);
+        __syncthreads();
+        for (int i = threadIdx.x; i < room; i += threads) ranked[i] = nothing();
+        if (lane == 0) wt[wave] = better;
+        if (threadIdx.x == 0) places = 0;
+        __syncthreads();
+        float bound = wt[0];
+        for (int i = 1; i < waves; ++i) bound = fminf(bound, wt[i]);
+        if (!(bound > least)) break;
+        least = bound;
+        if constexpr (EACH == 0) {
+#pragma unroll
+            for (int i = 0; i < U; ++i) x[i] = first_of(first + i * waves);
         }
     }
-    __syncthreads();
-    const int found = places;
+    // Ranking costs found^2: where there are many more than n, a bound of theirs, one of each
+    // thread, leaves fewer (16 batch elements, 64 beams of 2 lists of 128 entries, 585 found:
+    // 23.5 us, without this 64).
+    if (threads == kJoinRoom && found > 2 * r.n + kWave && found <= kJoinRoom) {
+        const int mine = lane * waves + wave;
+        const Entry y = ranked[mine];
+        const int token = tokens[mine];
+        const float one[1] = {mine < found ? float_of(value_of64(y.key)) : -__builtin_inff()};
+        const float better = reached_by(one, share);
+        __syncthreads();
+        ranked[mine] = nothing();
+        if (lane == 0) wt[wave] = better;
+        if (threadIdx.x == 0) places = 0;
+        __syncthreads();
+        float bound = wt[0];
+        for (int i = 1; i < waves; ++i) bound = fminf(bound, wt[i]);
+        const bool in = mine < found && (bound == -__FLT_MAX__ || one[0] >= bound);
+        const uint64_t all = __ballot(in);
+        int from = 0;
+        if (lane == 0 && all) from = atomicAdd(&places, int(__builtin_popcountll(all)));
+        from = __builtin_amdgcn_readfirstlane(from) +
+               __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
+        if (in) {
+            ranked[from] = y;
+            tokens[from] = token;
+        }
+        __syncthreads();
+        found = places;
+    }
     auto write = [&](int to_entry, double key, int id, int token) {
         const int64_t to = int64_t(b) * r.n + to_entry;
         if (id < 0) {

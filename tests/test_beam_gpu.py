@@ -433,3 +433,29 @@ def test_search_in_a_graph():
             search(model, B, W, 2, eos, V, D, DEV)
         for got, w in zip((tokens, scores, finished), want):
             assert torch.equal(got, w)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("W,k,ahead", [(64, 256, 8), (64, 128, 4), (64, 64, 9), (128, 256, 12), (128, 200, 6), (7, 256, 5)])
+def test_beams_that_are_far_ahead(dtype, W, k, ahead):
+    """All entries are from the depth of a few beams' lists; with 8 and 12 of 256 entries
+    each, more of them than a join ranks."""
+    print(f"[beam] {dtype} W={W} k={k} ahead={ahead}", flush=True)
+    rng = np.random.default_rng(W * k)
+    for V in (1501, 9000):
+        logits = logits_of(rng, (2, W, V), DTYPES[dtype])
+        scores = scores_of(rng, 2, W)
+        scores[0, :ahead] += 50.0
+        scores[1, rng.permutation(W)[:ahead]] += 50.0
+        check(logits, scores, k=k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [516, 520, 1032, 1040, 1096, 2050, 2056, 2064, 2120, 3080, 4104])
+def test_spans_that_do_not_fill_the_waves(dtype, V):
+    print(f"[beam] {dtype} V={V} waves", flush=True)
+    rng = np.random.default_rng(V)
+    for W in (1, 4, 16):
+        logits, scores = logits_of(rng, (1, W, V), DTYPES[dtype]), scores_of(rng, 1, W)
+        for k in sorted({1, W, 2 * W + 1, 70, 256}):
+            check(logits, scores, k=k)

@@ -193,3 +193,14 @@ def test_other_stream_and_graph():
         torch.cuda.synchronize()
         between = step(data[(i + 1) % 3])
         assert same(out, eager[i]) and same(between, eager[(i + 1) % 3])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [257, 264, 513, 520, 776, 1032, 1040, 1049, 1500, 2050, 2064, 3000, 4100, 8193])
+def test_rows_that_do_not_fill_the_waves(dtype, V):
+    """Waves with few packs or none take none or little of the entries that are looked for."""
+    print(f"[top] {dtype} V={V} waves", flush=True)
+    rng = np.random.default_rng(V)
+    logits = logits_of(rng, (1, 9, V), DTYPES[dtype])
+    for k in (1, 17, 64, 65, 130, 256):
+        check(logits, k)
