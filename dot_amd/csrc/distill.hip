@@ -11,7 +11,7 @@ namespace {
 // Workgroups per row: rows alone fill the chip, fewer are split, into spans of at least two
 // packs per thread, and into as many as keep the bits of a span in LDS.  The forward is
 // split for fewer workgroups, since its parts are joined by a launch more (774 rows of
-// 50021 fp32 whole 25.5 us, in 3 parts 22.6 + 15.2).
+// 50021 fp32 whole 23.2 us, in 3 parts 20.3 + 7.7).
 int splits_of(int B, int S, int V, int dtype, bool backward) {
     const int64_t rows = int64_t(B) * S, fill = backward ? 2048 : 512;
     const int packs = V / (16 / dtype_bytes(dtype));
@@ -75,7 +75,7 @@ using namespace dot_amd;
 namespace {
 struct Workspace {
     distill::Value* values;
-    seqlogp::Part* parts;
+    distill::Part* parts;
     size_t bytes;
 };
 Workspace carve(void* ws, int B, int S, int V, int dtype, int reduction) {
@@ -84,7 +84,7 @@ Workspace carve(void* ws, int B, int S, int V, int dtype, int reduction) {
     const size_t rows = size_t(B) * S;
     if (reduction != DOT_REDUCE_NONE) w.values = c.take<distill::Value>(rows);
     const int splits = splits_of(B, S, V, dtype, false);
-    if (splits > 1) w.parts = c.take<seqlogp::Part>(rows * splits);
+    if (splits > 1) w.parts = c.take<distill::Part>(rows * splits);
     w.bytes = c.used();
     return w;
 }
@@ -138,7 +138,7 @@ extern "C" int dot_distill_forward(const dot_distill_fwd_args* a, dot_stream_t s
                 ProfScope prof("distill_finish", stream);
                 const unsigned blocks = unsigned((rows + kWavesPerBlock - 1) / kWavesPerBlock);
                 hipLaunchKernelGGL((distill::finish_rows<T>), dim3(blocks), dim3(kBlock), 0, stream, r, t, o,
-                                   static_cast<const seqlogp::Part*>(w.parts));
+                                   static_cast<const distill::Part*>(w.parts));
             }
         });
     if (a->reduction != DOT_REDUCE_NONE) {
