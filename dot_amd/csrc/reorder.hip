@@ -70,6 +70,7 @@ void launch(const reorder::States& a, unsigned blocks, hipStream_t stream) {
     else if (a.W <= 16) hipLaunchKernelGGL((reorder::move<BYTES, 16>), grid, block, 0, stream, a);
     else if constexpr (BYTES <= 8) {
         if (a.W <= 32) hipLaunchKernelGGL((reorder::move<BYTES, 32>), grid, block, 0, stream, a);
+        else if (a.W <= 64) hipLaunchKernelGGL((reorder::move<BYTES, 64>), grid, block, 0, stream, a);
         else if constexpr (BYTES <= 4) hipLaunchKernelGGL((reorder::move<BYTES, 128>), grid, block, 0, stream, a);
     }
 }
@@ -130,7 +131,7 @@ static int reorder_states(const dot_beam_reorder_args* a, hipStream_t stream) {
     if (a->W == 1) return ok();
     // Launches of states of one unit.
     for (int unit = 16; unit >= 1; unit /= 2) {
-        const int most = a->W <= 16 ? 16 : a->W <= 32 ? 8 : 4;  // units of all beams in 64 or 128 registers
+        const int most = a->W <= 16 ? 16 : a->W <= 64 ? 8 : 4;  // units of all beams in 64 or 128 registers
         if (unit > most) continue;
         size_t i = 0;
         while (i < moved.size()) {

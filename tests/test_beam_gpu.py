@@ -459,3 +459,13 @@ def test_spans_that_do_not_fill_the_waves(dtype, V):
         logits, scores = logits_of(rng, (1, W, V), DTYPES[dtype]), scores_of(rng, 1, W)
         for k in sorted({1, W, 2 * W + 1, 70, 256}):
             check(logits, scores, k=k)
+
+
+@pytest.mark.parametrize("W", [48, 63, 64, 65])
+def test_parents_of_many_beams(W):
+    print(f"[reorder] W={W}", flush=True)
+    rng, gen = np.random.default_rng(W), torch.Generator(DEV).manual_seed(W)
+    beams = parents(rng, 2, W, "random")
+    check_reorder([state_of(gen, (2, W, 7, n), t) for t in TYPES for n in (1, 4, 40)], beams)
+    check_reorder([state_of(gen, (2, W, 3, 33, 16), torch.bfloat16)], beams,
+                  torch.as_tensor([33, 10], device=DEV), 3)
