@@ -628,8 +628,8 @@ inline size_t join_shared(int R, int waves, int beams, int entries) {
 //
 // One workgroup a list, so bound by its latency: the sums of the spans, a bound, what
 // reaches it, the ranks.  4 beams, 8 entries and 16 spans each 4.9 us; 8 beams, 16
-// entries and 4 spans 6.9; 48 beams, 96 entries and 4 spans 18.3; 4096 rows of 4 spans
-// and 64 entries 20 to 24, 999 of 128 entries 12.
+// entries and 4 spans 7; 48 beams, 96 entries and 4 spans 18.5; 4096 rows of 4 spans
+// and 64 entries 20 to 24, 999 of 128 entries 13.
 template <int R, bool BEAM, int EACH>
 __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
