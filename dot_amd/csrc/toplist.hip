@@ -72,7 +72,8 @@ void scan(int dtype, const toplist::Rows& r, const toplist::Lists& l, const topl
 }
 
 // Four waves for up to 1024 entries of a join, so that four of a thread stay in its
-// registers, sixteen for more.
+// registers, sixteen for more.  Eight for 257 to 512 entries: 999 rows of 4 lists of 128
+// 13.8 us instead of 12.5, 32 times 8 beams of 4 lists of 16 7.5 instead of 7.
 template <bool BEAM>
 void join(const toplist::Rows& r, const toplist::Lists& l, const toplist::JoinArgs& a, hipStream_t stream) {
     ProfScope prof("toplist_join", stream);
