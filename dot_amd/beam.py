@@ -137,15 +137,6 @@ def beam_reorder(
                              f"{tuple(lengths.shape)}")
     if dim is not None and (isinstance(dim, bool) or not isinstance(dim, int)):
         raise ValueError(f"dim must be an int, got {dim!r}")
-    grad = torch.is_grad_enabled()
-    for t in states:
-        if t.dim() < 2 or t.shape[:2] != beams.shape:
-            raise ValueError(f"states must have shape ({beams.size(0)}, {beams.size(1)}, ...), got {tuple(t.shape)}")
-        if t.device != beams.device:
-            raise ValueError(f"states must be on {beams.device}, got {t.device}")
-        if dim is not None and not 2 <= (dim + t.dim() if dim < 0 else dim) < t.dim():
-            raise ValueError(f"dim must name a dimension behind the beams of every state, got {dim} for {tuple(t.shape)}")
-        if grad and t.requires_grad:
-            raise ValueError("states that require a gradient cannot be reordered in place")
-    if states and beams.numel():
-        _ops.fused.beam_reorder(states, beams, lengths, None if lengths is None else dim)
+    # the states themselves are looked over by the operator: a step has those of all layers
+    if states:
+        _ops.fused.beam_reorder(states, beams, lengths, dim)

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/core/InferenceMode.h>
 
 #include <algorithm>
@@ -57,7 +58,8 @@ inline dot_beam_state beam_state(const at::Tensor& t, int64_t dim) {
     return s;
 }
 
-// Arguments that fit together, as both devices' implementations need them.
+// Arguments that fit together, as both devices' implementations need them: looked over
+// here, not in Python, for a step reorders the caches of all layers.
 inline std::vector<dot_beam_state> beam_states(at::TensorList states, const at::Tensor& beams,
                                                const c10::optional<at::Tensor>& lengths, c10::optional<int64_t> dim) {
     TORCH_CHECK(beams.dim() == 2 && (beams.scalar_type() == at::kInt || beams.scalar_type() == at::kLong),
@@ -69,14 +71,20 @@ inline std::vector<dot_beam_state> beam_states(at::TensorList states, const at::
                     "lengths must be int32 or int64 of shape [B], and come with dim");
     std::vector<dot_beam_state> out;
     out.reserve(states.size());
+    const bool records = at::GradMode::is_enabled();
     for (const at::Tensor& t : states) {
-        const int64_t d = !dim.has_value() ? -1 : *dim < 0 ? *dim + t.dim() : *dim;
-        TORCH_CHECK(t.layout() == at::kStrided && t.dim() >= 2 && t.size(0) == beams.size(0) &&
-                        t.size(1) == beams.size(1) && t.device() == beams.device(),
-                    "states must be dense tensors of shape [B, W, ...] on the device of beams");
+        TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.dim() >= 2 && t.size(0) == beams.size(0) &&
+                              t.size(1) == beams.size(1),
+                          "states must be dense and have shape (", beams.size(0), ", ", beams.size(1), ", ...), got ",
+                          t.sizes());
+        TORCH_CHECK_VALUE(t.device() == beams.device(), "states must be on ", beams.device(), ", got ", t.device());
+        const int64_t named = !dim.has_value() ? 2 : *dim < 0 ? *dim + t.dim() : *dim;
+        TORCH_CHECK_VALUE(!dim.has_value() || (named >= 2 && named < t.dim()),
+                          "dim must name a dimension behind the beams of every state, got ", *dim, " for ", t.sizes());
+        TORCH_CHECK_VALUE(!records || !t.requires_grad(), "states that require a gradient cannot be reordered in place");
         TORCH_CHECK_VALUE(!t.is_inference() || c10::InferenceMode::is_enabled(),
                           "states of inference mode cannot be reordered outside of it");
-        TORCH_CHECK(!dim.has_value() || (d >= 2 && d < t.dim()), "dim must name a dimension behind the beams");
+        const int64_t d = lengths.has_value() ? named : -1;  // the positions matter with lengths alone
         out.push_back(beam_state(t, d));
     }
     return out;

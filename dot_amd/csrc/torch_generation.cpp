@@ -164,7 +164,7 @@ std::vector<Tensor> beam_step_op(Tensor logits_, Tensor scores_, int64_t n, doub
 
 void beam_reorder_op(at::TensorList states, const Tensor& beams_, const optional<Tensor>& lengths_,
                      optional<int64_t> dim) {
-    TORCH_CHECK(beams_.device().is_cuda(), "beams must be a CUDA tensor");
+    TORCH_CHECK_VALUE(beams_.device().is_cuda(), "states must be on ", beams_.device(), ", as beams are");
     c10::OptionalDeviceGuard guard(beams_.device());
     const std::vector<dot_beam_state> s = beam_states(states, beams_, lengths_, dim);
     const Tensor beams = beams_.contiguous(), lengths = lengths_.has_value() ? lengths_->contiguous() : Tensor();
