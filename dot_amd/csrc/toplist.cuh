@@ -79,16 +79,6 @@ __device__ __forceinline__ Pack<T> load_pack_any(const T* p) {
     return x;
 }
 
-// A pack as it is in registers: the compiler would otherwise keep the floats that one
-// pass made of it for the next, at twice the registers.
-template <class T>
-__device__ __forceinline__ void hold(Pack<T>& x) {
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    u4 raw = __builtin_bit_cast(u4, x);
-    asm volatile("" : "+v"(raw));
-    x = __builtin_bit_cast(Pack<T>, raw);
-}
-
 // A pack of -inf.
 template <class T>
 __device__ __forceinline__ Pack<T> nothing_pack() {
