@@ -215,10 +215,12 @@ std::vector<Tensor> distill_forward_cpu(Tensor logits_, Tensor logp_, Tensor tok
                 if (!reverse) total += p == 0.0 ? 0.0 : p * (lp - lq);
                 else total += lq == -kInf ? 0.0 : std::exp(lq) * (lq - lp);
             }
-            double other;
+            double other, all = 1.0;  // all: the sum of the P that the forward loss has
             if (!reverse) {
-                if (bucket && !(pr == 0.0 || (none && pr <= std::ldexp(1.0, -20)))) total += pr * (std::log(pr) - log_qr);
-                other = qr - pr;
+                const bool left = bucket && !(pr == 0.0 || (none && pr <= std::ldexp(1.0, -20)));
+                if (left) total += pr * (std::log(pr) - log_qr);
+                else if (bucket) all = mass;
+                other = all * qr - (left ? pr : 0.0);
             } else {
                 const double log_pr = std::log(std::isnan(pr) ? pr : std::max(pr, std::ldexp(1.0, -24)));
                 if (!none) total += qr * (log_qr - log_pr);
@@ -233,7 +235,7 @@ std::vector<Tensor> distill_forward_cpu(Tensor logits_, Tensor logp_, Tensor tok
                 if (tok[size_t(e)] < 0) continue;
                 const double lp = double(t[e]) - scale, lq = (double(x[tok[size_t(e)]]) - top) / tau - lz;
                 const double q = std::exp(lq);
-                own[r * K + e] = float(!reverse ? q - std::exp(lp) : lq == -kInf ? 0.0 : q * (lq - lp - total));
+                own[r * K + e] = float(!reverse ? all * q - std::exp(lp) : lq == -kInf ? 0.0 : q * (lq - lp - total));
             }
         }
     });

@@ -5,10 +5,11 @@
 // Q = softmax(z) and Q_r the sum of Q over the other tokens:
 //   forward  L = sum_k P_k (t_k - log Q_k) + P_r (log P_r - log Q_r)
 //   reverse  L = sum_k Q_k (log Q_k - t_k) + Q_r (log Q_r - log P_r)
-// P_r = 1 - sum_k P_k; with DOT_REST_NONE P is made to sum to 1 and P_r = 0.  The
-// gradient of a named token is a value of its own, that of any other token its share
-// w_j = Q_j / Q_r of one value for the row:
-//   tau dL/dx_j = Q_j - P_j,                     w_j (Q_r - P_r)
+// P_r = 1 - sum_k P_k, 0 where that is negative; with DOT_REST_NONE P is made to sum to
+// 1 and P_r = 0.  The gradient of a named token is a value of its own, that of any other
+// token its share w_j = Q_j / Q_r of one value for the row; with M = sum_k P_k + P_r, which
+// is 1 but where P_r is 0 (log-probabilities kept in few bits):
+//   tau dL/dx_j = M Q_j - P_j,                   w_j (M Q_r - P_r)
 //   tau dL/dx_j = Q_j (log Q_j - t_j - L),       w_j Q_r (log Q_r - log P_r - L)
 // So the row is read once for s = sum 2^((x - m) k) of the others alone, m the largest
 // of the first of them, or of all where a term next to that one would be too large.
@@ -162,11 +163,14 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
     }
     value = wave_sum64(value);
     const double log_pr = short_log(reverse ? fmax(pr, 0x1p-24) : pr);
-    double other;  // gradient of the others together
+    double other;        // gradient of the others together
+    double total = 1.0;  // sum of the P that the forward loss has: the entries' alone where they leave no rest
     if (!reverse) {
         // where no other token is possible, what rounding leaves of P_r is nothing
-        if (bucket && !(pr == 0.0 || (none && pr <= 0x1p-20))) value += pr * (log_pr - log_qr);
-        other = qr - pr;
+        const bool left = bucket && !(pr == 0.0 || (none && pr <= 0x1p-20));
+        if (left) value += pr * (log_pr - log_qr);
+        else if (bucket) total = mass;
+        other = total * qr - (left ? pr : 0.0);
     } else {
         if (!none) value += qr * (log_qr - log_pr);
         other = none ? 0.0 : qr * (log_qr - log_pr - value);
@@ -184,7 +188,7 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
         float g = 0.0f;
         if (tok[i] >= 0) {
             const double lq = (double(x[i]) - double(top)) * kn - lz;
-            if (!reverse) g = float(q[i] - p[i]);
+            if (!reverse) g = float(total * q[i] - p[i]);
             else g = lq == -__builtin_inf() ? 0.0f : float(q[i] * (lq - tl[i] - value));
         }
         o.at[at * K + e] = tok[i];

@@ -82,10 +82,13 @@ def distill(logits, logp, tokens, mask=None, tau=1.0, direction="forward", rest=
                 pull = np.zeros(V)
                 if direction == "forward":
                     v = np.where(P == 0, 0.0, P * (lp - lq[at])).sum()
-                    if pr > 0 and not (lqr == -np.inf and pr <= 2.0**-20):
+                    if lqr == -np.inf and pr <= 2.0**-20:
+                        pr = 0.0
+                    if pr != 0:
                         v += pr * (np.log(pr) - lqr)
-                    other = qr - pr
-                    pull[at] = Q[at] - P
+                    total = P.sum() + pr  # the loss has no more than these
+                    other = total * qr - pr
+                    pull[at] = total * Q[at] - P
                 else:
                     lpr = np.log(max(pr, 2.0**-24))
                     v = np.where(Q[at] == 0, 0.0, Q[at] * (lq[at] - lp)).sum()

@@ -1,0 +1,75 @@
+"""Top log-probabilities, distillation and beam search where their rules decide; tolerances in generation_cases.py."""
+
+import numpy as np
+import pytest
+import torch
+
+import dot_amd
+from generation_cases import check_distill, logits_of, teacher_of
+from oracle import generation as oracle
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def distill(dev, logits, logp, tokens, **kw):
+    """check_distill of teacher tensors as they are given; -> (loss, gradient) on the CPU."""
+    tk = torch.as_tensor(tokens).to(dev)
+
+    def call(x, mask, **kw):
+        mask = None if mask is None else torch.as_tensor(mask).to(dev)
+        return dot_amd.distill_loss(x, logp.to(dev), tk, mask=mask, **kw)
+
+    out, g = check_distill(call, logits, logp.float().numpy(), tokens, x=logits.to(dev), **kw)
+    return out.cpu(), g.cpu().double()
+
+
+# ---------------------------------------------------------------------------
+# Teachers whose probabilities sum to more than 1
+# ---------------------------------------------------------------------------
+def test_gradient_of_masses_above_one_by_differences():
+    """The loss written out: there is no rest, and the probabilities that are named are taken as they are."""
+    rng = np.random.default_rng(0)
+    tau, p, at = 0.8, np.array([0.9, 0.6]), [1, 4]
+    logp = np.log(p).astype(np.float32)[None, None]
+    p = np.exp(logp[0, 0].astype(np.float64))
+    x = rng.standard_normal((1, 1, 6))
+
+    def loss(x):
+        z = x[0, 0] / tau
+        return (p * (np.log(p) - (z - np.log(np.exp(z).sum()))[at])).sum()
+
+    want = np.zeros(6)
+    for v in range(6):
+        d = np.zeros_like(x)
+        d[0, 0, v] = 1e-5
+        want[v] = (loss(x + d) - loss(x - d)) / 2e-5  # off by h^2 / 6 of a third derivative of order 1, and 1e-16 / h
+    value, parts = oracle.distill(x, logp, np.array([[at]]), tau=tau, reduction="sum")
+    g = oracle.distill_grad(x.shape, parts, np.ones(1), tau)[0, 0]
+    assert abs(value[0] - loss(x)) < 1e-12 and np.abs(g - want).max() < 1e-8
+    leaf = torch.as_tensor(x.astype(np.float32)).requires_grad_()
+    out = dot_amd.distill_loss(leaf, torch.as_tensor(logp), torch.as_tensor([[at]]), tau=tau, reduction="sum")
+    (g,) = torch.autograd.grad(out.sum(), leaf)
+    # the logits in fp32 move the gradient by 2^-24 of them, and it is rounded once
+    assert np.abs(g[0, 0].numpy() - want).max() < 1e-6
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kept", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V,k", [(6, 2), (300, 40), (4000, 64), (70000, 64), (300000, 200)])
+def test_masses_above_one(dev, kept, V, k):
+    """Log-probabilities kept in 16 bits, and ones that are too large by 0.05: the gradient sums to 0 over a row."""
+    print(f"[edges] mass {dev} {kept} V={V} k={k}", flush=True)
+    rng = np.random.default_rng(V)
+    logits = logits_of(rng, (2, 6, V), torch.float32)
+    logp, tokens = teacher_of(rng, logits, k, tau=0.7, noise=0.3)
+    logp = torch.as_tensor(logp)
+    logp[0] = torch.where(logp[0] > -1, logp[0] + 0.05, logp[0]).clamp(max=-1e-3)
+    logp = logp.to(kept)
+    mass = logp.double().exp().sum(-1)
+    assert (mass > 1.001).any() and mass.max() < 2
+    for reduction in ("mean", "none"):
+        _, g = distill(dev, logits, logp, tokens, tau=0.7, reduction=reduction)
+        # each entry to the bound above, of which the row's have 3 SUM M / tau and 1e-5 of themselves
+        assert (g.sum(-1).abs() <= (9e-6 * 2 + 2e-5) * g.abs().sum(-1) + 2e-5).all()
+    distill(dev, logits, logp, tokens, tau=0.7, direction="reverse")
+    distill(dev, logits, logp, tokens, tau=0.7, rest="none")
