@@ -217,7 +217,7 @@ std::vector<Tensor> distill_forward_cpu(Tensor logits_, Tensor logp_, Tensor tok
             }
             double other, all = 1.0;  // all: the sum of the P that the forward loss has
             if (!reverse) {
-                const bool left = bucket && !(pr == 0.0 || (none && pr <= std::ldexp(1.0, -20)));
+                const bool left = bucket && !(pr == 0.0 || (none && pr <= DOT_REST_ROUNDING));
                 if (left) total += pr * (std::log(pr) - log_qr);
                 else if (bucket) all = mass;
                 other = all * qr - (left ? pr : 0.0);

@@ -167,7 +167,7 @@ __device__ __forceinline__ void finish(const Rows& r, int K, const Out& o, int64
     double total = 1.0;  // sum of the P that the forward loss has: the entries' alone where they leave no rest
     if (!reverse) {
         // where no other token is possible, what rounding leaves of P_r is nothing
-        const bool left = bucket && !(pr == 0.0 || (none && pr <= 0x1p-20));
+        const bool left = bucket && !(pr == 0.0 || (none && pr <= DOT_REST_ROUNDING));
         if (left) value += pr * (log_pr - log_qr);
         else if (bucket) total = mass;
         other = total * qr - (left ? pr : 0.0);

@@ -131,7 +131,9 @@ def distill_loss(
             GPU V is at most 2^24, and there are at most 2^23 positions.
         teacher_logp: (B, S, K) or (S, K) floating point log-probabilities at the same
             temperature (``top_logp(..., tau=tau).logp``), computed in fp32; constants of the
-            gradient.  K is at most 256.
+            gradient.  K is at most 256.  Ones kept in 16 bits are taken as they are, and what
+            their rounding leaves of 1 is rest (up to 2^-11 of the list's entropy in fp16, 2^-8
+            in bf16): where the list is all that the student allows, use ``rest="none"``.
         teacher_tokens: int32 or int64, shaped as ``teacher_logp``.  An entry whose token is
             outside [0, V) or whose log-probability is -inf names no token, nor does one whose
             token an earlier entry names.
@@ -147,9 +149,10 @@ def distill_loss(
 
     Returns:
         fp32 (B,), 0-dim for unbatched logits, or (B, S) for ``"none"``.  Where the student
-        has no probability for what the teacher has, the divergence is +inf (a rest of the
-        teacher of at most 2^-20 is not held against a student that has none); its gradient
-        stays finite.
+        has no probability for what the teacher has, the divergence is +inf; its gradient
+        stays finite.  A rest of the teacher of at most 2^-12 is not held against a student
+        that has none: the log-probabilities of :func:`top_logp` leave as much by their
+        rounding, 2^-23 times the largest scaled logit.
     """
     if reduction not in _REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTION)}, got {reduction!r}")

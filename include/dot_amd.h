@@ -560,6 +560,9 @@ enum { DOT_DISTILL_FORWARD = 0, DOT_DISTILL_REVERSE = 1 };
 /* What the teacher's tokens leave of its mass: a class of its own, or nothing
  * (the tokens' masses are made to sum to 1; DOT_DISTILL_FORWARD only). */
 enum { DOT_REST_BUCKET = 0, DOT_REST_NONE = 1 };
+/* A rest that the log-probabilities' rounding may have made: dot_top_logp's are off by
+ * 2^-23 |x / tau| together, half of this at scaled logits of 2^10. */
+#define DOT_REST_ROUNDING 0x1p-12
 
 typedef struct {
     const void* logits;        /* element (b, s, v) at b * stride_b + s * stride_s + v */
@@ -589,7 +592,7 @@ typedef struct {
 /* With P = exp(logp), P_r = max(0, 1 - sum P), Q = softmax(x / tau) and Q_r its sum
  * over the tokens that are not named: sum P (log P - log Q) + P_r (log P_r - log Q_r),
  * or sum Q (log Q - log P) + Q_r (log Q_r - log max(P_r, 2^-24)).  Where Q_r is 0, a
- * P_r of at most 2^-20 counts as 0. */
+ * P_r of at most DOT_REST_ROUNDING counts as 0. */
 size_t dot_distill_forward_workspace_bytes(int B, int S, int V, int dtype, int reduction);
 int dot_distill_forward(const dot_distill_fwd_args* args, dot_stream_t stream);
 

@@ -82,7 +82,7 @@ def distill(logits, logp, tokens, mask=None, tau=1.0, direction="forward", rest=
                 pull = np.zeros(V)
                 if direction == "forward":
                     v = np.where(P == 0, 0.0, P * (lp - lq[at])).sum()
-                    if lqr == -np.inf and pr <= 2.0**-20:
+                    if lqr == -np.inf and pr <= 2.0**-12:
                         pr = 0.0
                     if pr != 0:
                         v += pr * (np.log(pr) - lqr)

@@ -73,3 +73,29 @@ def test_masses_above_one(dev, kept, V, k):
         assert (g.sum(-1).abs() <= (9e-6 * 2 + 2e-5) * g.abs().sum(-1) + 2e-5).all()
     distill(dev, logits, logp, tokens, tau=0.7, direction="reverse")
     distill(dev, logits, logp, tokens, tau=0.7, rest="none")
+
+
+# ---------------------------------------------------------------------------
+# What rounding leaves of a teacher's rest
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("offset", [0.0, 50.0, 500.0, -1000.0])
+@pytest.mark.parametrize("tau", [0.9, 1.3])
+def test_rest_of_a_list_of_a_whole_vocabulary(dev, offset, tau):
+    """top_logp rounds scaled logits to fp32: log-probabilities are off by 2^-23 |x| / tau together, and what they
+    leave of 1 with them (1.3e-4 at |x| / tau = 1112).  It is not held against a student that has no other token."""
+    rng = np.random.default_rng(11)
+    few = torch.as_tensor((3 * rng.standard_normal((1, 64, 200)) + offset).astype(np.float32))
+    wide = torch.full((1, 64, 5000), -float("inf"))
+    wide[..., 7:2007:10] = few  # the same tokens of a vocabulary of which the others are not allowed
+    for x in (few, wide):
+        t = dot_amd.top_logp(x.to(dev), 200, tau=tau)
+        rest = 1 - t.logp.double().exp().sum(-1)
+        assert rest.abs().max() < 2.0**-12 and (offset == 0 or rest.max() > 2.0**-20)
+        out, g = distill(dev, x, t.logp.cpu(), t.tokens.cpu().numpy(), tau=tau, reduction="none")
+        # the student's own: the divergence is what the lists are off by
+        assert torch.isfinite(out).all() and out.abs().max() < 2.0**-12 and g.abs().max() < 2.0**-12
+    # a rest that is none of rounding has no place
+    less = t.logp.cpu() - 2.0**-11
+    out = dot_amd.distill_loss(wide.to(dev), less.to(dev), t.tokens, tau=tau, reduction="none")
+    assert (out == float("inf")).all()
