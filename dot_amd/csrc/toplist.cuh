@@ -245,9 +245,14 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     }
     // Maxima and terms in one pass.  The terms are relative to the largest logit of the
     // wave's first packs: it is near the largest of all, or the sum is formed again below.
-    // x k - m k takes one rounding where m k has digits behind the point.
+    // x k - m k takes one rounding where m k has digits behind the point.  Behind packs of
+    // nothing but -inf the terms are relative to 1: as long as the largest is within 2^32
+    // of that, rounding x k costs 2^-24 of 22 at most, and no term that counts is below the
+    // smallest float (a row's largest logit at -69 and many 20 below it: 2e-5 of the sum were).
+    // Past that the sum is formed again too: 1024 x 131072 bf16 62 us, then 104.
     float pm[P];  // the largest logit of each pack
     float m = -__builtin_inff(), mk = 0.0f;
+    float reach = 100.0f;
     bool near = true;
     double s = 0.0;
 #pragma unroll
@@ -266,6 +271,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         if (u == 0) {
             const float first = wave_max(m);
             mk = first == -__builtin_inff() ? 0.0f : first * r.k;
+            if (first == -__builtin_inff()) reach = 32.0f;
             near = fabsf(mk) < 65536.0f;
             if (!near) mk = 0.0f;
         }
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
     m = wave_max(m);
     // what the wave's terms are relative to, as a binary logarithm
     double of = double(mk);
-    if (m > -__builtin_inff() && !(near && fabsf(m * r.k - mk) < 100.0f)) {
+    if (m > -__builtin_inff() && !(near && fabsf(m * r.k - mk) < reach)) {
         s = 0.0;
         of = double(m) * double(r.k);
         each([&](float f, int) { s += double(__builtin_amdgcn_exp2f((f - m) * r.k)); });

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import dot_amd
-from generation_cases import check_distill, logits_of, teacher_of
+from generation_cases import DTYPES, check_beam, check_distill, check_top, logits_of, teacher_of
 from oracle import generation as oracle
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -99,3 +99,29 @@ def test_rest_of_a_list_of_a_whole_vocabulary(dev, offset, tau):
     less = t.logp.cpu() - 2.0**-11
     out = dot_amd.distill_loss(wide.to(dev), less.to(dev), t.tokens, tau=tau, reduction="none")
     assert (out == float("inf")).all()
+
+
+# ---------------------------------------------------------------------------
+# Rows that begin with tokens that are not allowed
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [3000, 32768, 100003, 131072])
+@pytest.mark.parametrize("offset", [-69.0, -40.0, 30.0, 150.0])
+def test_banned_beginnings(dev, dtype, V, offset):
+    """Blocks of -inf as long as what a workgroup's threads take at once, and logits far from 0 behind them: the many
+    small terms of the sum count as where the logits lie around 0."""
+    print(f"[edges] banned {dev} {dtype} V={V} {offset}", flush=True)
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((1, 4, V)) + offset - 20
+    x[..., V // 2 + 5] = offset
+    at = np.arange(V)
+    long = 8 if dtype != "fp32" else 4
+    for row, every in enumerate((16 * 256 * long, 4 * 256 * long, 1024 * 8, 1 << 30)):
+        x[0, row, at % every < (256 * long if every < 1 << 30 else V // 3)] = -np.inf
+    logits = torch.as_tensor(x.astype(np.float32)).to(DTYPES[dtype])
+    for k in (1, 20, 100):
+        check_top(dot_amd.top_logp(logits.to(dev), k), logits, k)
+    scores = -np.arange(4.0)[None]
+    r = dot_amd.beam_step(logits.to(dev), torch.as_tensor(scores.astype(np.float32)).to(dev), k=8)
+    check_beam(r, logits, scores, 8)
