@@ -439,6 +439,7 @@ __global__ __launch_bounds__(kBlock) void finish_rows(Rows r, Teacher t, Out o, 
     Sum all{wave_max(mine.m), 0.0};
     if (mine.s != 0.0) mine.s *= short_exp((double(mine.m) - double(all.m)) * inverse_tau(r));
     all.s = wave_sum64(mine.s);
+    wave_lds_fence();
     if (__ballot(twice)) only_first(t.K, lists[wave], in);
     finish(r, t.K, o, at, in, all);
 }

@@ -138,12 +138,6 @@ __device__ __forceinline__ float across_groups(float x) {
     return x;
 }
 
-// Orders this wave's LDS writes before its later LDS reads.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 constexpr float kNegInf = -__builtin_inff();
 
 // A row as it lies in memory, in registers.

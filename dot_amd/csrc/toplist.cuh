@@ -374,6 +374,7 @@ __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut ou
         }
         held += __builtin_popcountll(all);
     }
+    wave_lds_fence();
     for (int j = lane; j - lane < min(held, HELD) * PN; j += kWave) {
         const bool in = j < held * PN;
         const int c = min(j / PN, min(held, HELD) - 1);

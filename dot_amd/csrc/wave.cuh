@@ -84,6 +84,12 @@ __device__ __forceinline__ double wave_sum64(double x) {
     return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
 }
 
+// Orders this wave's LDS writes before its later LDS reads.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Workgroup all-reduce of one value per wave through LDS, combined in wave order.
 // `scratch` needs kMaxWaves floats; contains a barrier on entry and exit.
 template <int NWAVES, class Op>
