@@ -114,7 +114,8 @@ def beam_reorder(
             keys and values (split a merged first dimension by ``cache.unflatten(0, (B, W))``).
             They may be views, the beams not innermost and of any strides, as long as the other
             dimensions are a run of neighbouring elements and at most one further dimension
-            besides that of the positions.  No two places may share memory.
+            besides that of the positions.  No two places may share memory; states may lie in
+            each other's gaps (keys and values of one tensor, of different widths or heads too).
         beams: int32 or int64 (B, W), such as ``beam_step(...).beams``; at most 128 beams.  A beam
             whose entry is outside [0, W) (an empty slot) stays as it is.
         lengths: Optional int32 or int64 (B,): the positions of each batch element that are in

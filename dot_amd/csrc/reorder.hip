@@ -40,16 +40,55 @@ int64_t reach_of(const dot_beam_state& s, int B, int W) {
 
 bool empty(const dot_beam_state& s) { return s.outer == 0 || s.positions == 0 || s.inner == 0; }
 
-// Whether two states have no byte in common: they lie apart, or interleave with the
-// same strides, as keys and values of one tensor do.
+// Whether sum_d k_d stride_d falls into [lo, hi] for some k_d of [least_d, most_d], the
+// strides descending; also where that is not settled in `steps` trials.
+struct Term {
+    int64_t stride, least, most;
+};
+using Wide = __int128;  // sums over two states, each up to 2^62
+bool meets(const Term* t, int n, Wide lo, Wide hi, int& steps) {
+    if (--steps < 0) return true;
+    Wide below = 0, above = 0;  // what the later terms can add
+    for (int i = 1; i < n; ++i) {
+        below += Wide(t[i].stride) * t[i].least;
+        above += Wide(t[i].stride) * t[i].most;
+    }
+    if (n == 0) return lo <= 0 && hi >= 0;
+    auto floor_of = [&](Wide x) { return x / t[0].stride - (x % t[0].stride < 0); };
+    const Wide first = std::max<Wide>(t[0].least, -floor_of(above - lo)), last = std::min<Wide>(t[0].most, floor_of(hi - below));
+    for (Wide k = first; k <= last; ++k)
+        if (meets(t + 1, n - 1, lo - k * t[0].stride, hi - k * t[0].stride, steps)) return true;
+    return false;
+}
+
+// Whether two states have no byte in common: they lie apart, or within each other's
+// gaps, as keys and values of one tensor do.
 bool disjoint(const dot_beam_state& x, const dot_beam_state& y, int B, int W) {
     const char *px = static_cast<const char*>(x.data), *py = static_cast<const char*>(y.data);
     if (px + reach_of(x, B, W) <= py || py + reach_of(y, B, W) <= px) return true;
-    if (x.stride_b != y.stride_b || x.stride_w != y.stride_w || x.stride_outer != y.stride_outer ||
-        x.stride_p != y.stride_p || x.outer != y.outer || x.positions != y.positions || x.inner != y.inner)
-        return false;
-    const std::array<Dim, 4> d = dims_of(x, B, W);
-    return apart(std::array<Dim, 5>{d[0], d[1], d[2], d[3], Dim{px < py ? py - px : px - py, 2}}, x.inner);
+    const std::array<Dim, 4> dx = dims_of(x, B, W), dy = dims_of(y, B, W);
+    if (x.stride_b == y.stride_b && x.stride_w == y.stride_w && x.stride_outer == y.stride_outer &&
+        x.stride_p == y.stride_p && x.outer == y.outer && x.positions == y.positions && x.inner == y.inner &&
+        apart(std::array<Dim, 5>{dx[0], dx[1], dx[2], dx[3], Dim{px < py ? py - px : px - py, 2}}, x.inner))
+        return true;
+    // px + sum i_d sx_d + a = py + sum j_d sy_d + b, equal strides in one term: at most three
+    // values of each k_d = i_d - j_d come into question, since what is left of either state
+    // is shorter than the stride
+    std::array<Term, 8> t;
+    int n = 0;
+    auto add = [&](const Dim& d, int64_t least, int64_t most) {
+        if (d.size <= 1 || d.stride == 0) return;
+        Term* same = std::find_if(t.data(), t.data() + n, [&](const Term& u) { return u.stride == d.stride; });
+        if (same == t.data() + n) t[size_t(n++)] = Term{d.stride, 0, 0};
+        same->least += least;
+        same->most += most;
+    };
+    for (const Dim& d : dx) add(d, 0, d.size - 1);
+    for (const Dim& d : dy) add(d, 1 - d.size, 0);
+    std::sort(t.data(), t.data() + n, [](const Term& u, const Term& v) { return u.stride > v.stride; });
+    int steps = 4096;
+    const Wide apart_by = py - px;
+    return !meets(t.data(), n, apart_by - (x.inner - 1), apart_by + (y.inner - 1), steps);
 }
 
 // Bytes of a unit: the largest power of two that divides every address.
@@ -107,15 +146,14 @@ static int checked(const dot_beam_reorder_args* a, std::vector<const dot_beam_st
             const char* end = static_cast<const char*>(moved[i]->data) + reach_of(*moved[i], a->B, a->W);
             if (static_cast<const char*>(moved[j]->data) >= end) break;  // and so are those behind it
             if (!disjoint(*moved[i], *moved[j], a->B, a->W))
-                return fail(DOT_ERR_INVALID_ARG, "states share memory");
+                return fail(DOT_ERR_INVALID_ARG,
+                            "states share memory, or interleave with too many strides to tell that they do not");
         }
     // the call reads these while it writes the states
     auto inside = [&](const void* p, int64_t bytes) {
-        for (const dot_beam_state* s : moved) {
-            const char* data = static_cast<const char*>(s->data);
-            if (static_cast<const char*>(p) < data + reach_of(*s, a->B, a->W) && data < static_cast<const char*>(p) + bytes)
-                return true;
-        }
+        const dot_beam_state one{const_cast<void*>(p), 0, 0, 0, 0, 1, 1, bytes};
+        for (const dot_beam_state* s : moved)
+            if (!disjoint(*s, one, a->B, a->W)) return true;
         return false;
     };
     if (inside(a->beams, int64_t(a->B) * a->W * (a->beams_are_int64 ? 8 : 4)) ||

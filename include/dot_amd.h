@@ -667,7 +667,7 @@ typedef struct {
 } dot_beam_reorder_args;
 
 /* The beams' states are exchanged in place, all from what they were before the
- * call.  No two states may share memory. */
+ * call.  No two states may share memory; they may lie in each other's gaps. */
 int dot_beam_reorder(const dot_beam_reorder_args* args, dot_stream_t stream);
 /* Its checks alone: a host function, data may be host memory. */
 int dot_beam_reorder_check(const dot_beam_reorder_args* args);

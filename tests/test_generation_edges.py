@@ -1,10 +1,14 @@
 """Top log-probabilities, distillation and beam search where their rules decide; tolerances in generation_cases.py."""
 
+import ctypes
+import os
+
 import numpy as np
 import pytest
 import torch
 
 import dot_amd
+from conftest import ROOT
 from generation_cases import DTYPES, check_beam, check_distill, check_top, logits_of, teacher_of
 from oracle import generation as oracle
 
@@ -125,3 +129,101 @@ def test_banned_beginnings(dev, dtype, V, offset):
     scores = -np.arange(4.0)[None]
     r = dot_amd.beam_step(logits.to(dev), torch.as_tensor(scores.astype(np.float32)).to(dev), k=8)
     check_beam(r, logits, scores, 8)
+
+
+# ---------------------------------------------------------------------------
+# States in each other's gaps
+# ---------------------------------------------------------------------------
+def neighbours():
+    """name -> (shape, views of it), with states of different sizes beside each other."""
+    return {
+        "widths": ((2, 4, 3, 8, 80), lambda t: [t[..., :64], t[..., 64:]]),
+        "heads": ((2, 4, 8, 6, 16), lambda t: [t[:, :, :, :4], t[:, :, :, 4:]]),
+        "lengths": ((2, 4, 3, 8, 16), lambda t: [t[:, :, :, :5], t[:, :, :, 5:]]),
+        "outer": ((2, 4, 5, 8, 16), lambda t: [t[:, :, :2], t[:, :, 2:3], t[:, :, 3:]]),
+        "tokens beside": ((2, 4, 3, 40), lambda t: [t[..., 8:], t[:, :, 0, 1], t[:, :, 1, :3]]),
+        "positions first": ((6, 2, 4, 3, 20), lambda t: [t[..., :16].permute(1, 2, 0, 3, 4), t[..., 16:].permute(1, 2, 0, 3, 4)]),
+        "layers": ((2, 4, 3, 2, 6, 24), lambda t: [v for i in range(3) for v in (t[:, :, i, 0, :, :16], t[:, :, i, 1])]),
+    }
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("name", list(neighbours()))
+def test_states_beside_each_other(dev, name):
+    print(f"[edges] beside {dev} {name}", flush=True)
+    shape, views = neighbours()[name]
+    t = torch.arange(np.prod(shape), dtype=torch.float32).view(shape)
+    beams = torch.as_tensor([[3, 0, 0, 7], [-1, 2, 1, 3]])
+    want = t.clone()
+    for v, old in zip(views(want), views(t)):
+        v.copy_(torch.as_tensor(oracle.beam_reorder(old.numpy(), beams.tolist())))
+    x = t.to(dev)
+    dot_amd.beam_reorder(views(x), beams.to(dev))
+    assert torch.equal(x.cpu(), want)
+
+
+def test_states_that_meet_are_refused():
+    beams = torch.as_tensor([[3, 0, 0, 7], [-1, 2, 1, 3]])
+    for shape, views in (((2, 4, 3, 8, 80), lambda t: [t[..., :65], t[..., 64:]]),
+                         ((2, 4, 8, 6, 16), lambda t: [t[:, :, :, :4], t[:, :, :, 3:]]),
+                         ((2, 4, 3, 40), lambda t: [t, t[:, :, 2, :1]])):
+        with pytest.raises(ValueError, match="share memory"):
+            dot_amd.beam_reorder(views(torch.zeros(shape)), beams)
+    # the beams themselves between the states' places, and in them
+    arena = torch.zeros(80, dtype=torch.int64)
+    state = arena.as_strided((2, 4, 4), (40, 6, 1))
+    for at, ok in ((22, True), (32, True), (15, False), (33, False)):
+        inside = arena[at : at + 8].view(2, 4)
+        inside.copy_(beams)
+        if ok:
+            dot_amd.beam_reorder(state, inside)
+        else:
+            with pytest.raises(ValueError, match="share memory"):
+                dot_amd.beam_reorder(state, inside)
+        inside.zero_()
+
+
+def test_meeting_states_by_their_bytes():
+    """The check of random states against the sets of their bytes."""
+    fields = [("data", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("sb", "sw", "so", "sp", "outer", "positions", "inner")]
+    State = type("State", (ctypes.Structure,), {"_fields_": fields})
+    P, I = ctypes.c_void_p, ctypes.c_int  # noqa: E741
+    Args = type("Args", (ctypes.Structure,), {"_fields_": [("states", P), ("count", I), ("B", I), ("W", I), ("beams", P),
+                                                           ("beams64", I), ("lengths", P), ("lengths64", I)]})
+    check = ctypes.CDLL(os.path.join(ROOT, "dot_amd", "libdot_amd.so")).dot_beam_reorder_check
+    rng = np.random.default_rng(0)
+
+    def state_of(sizes, strides, at, inner):
+        by = dict(zip(("sb", "sw", "so", "sp"), strides))
+        return State(data=at, outer=sizes[2], positions=sizes[3], inner=inner, **{k: int(v) for k, v in by.items()})
+
+    def bytes_of(sizes, strides, at, inner):
+        grid = np.zeros(1, np.int64) + at
+        for n, s in zip((*sizes, inner), (*strides, 1)):
+            grid = (grid[:, None] + s * np.arange(n)).ravel()
+        return set(grid.tolist())
+
+    def nested(sizes, inner):
+        """Strides in a random order, each past what the smaller ones reach."""
+        strides, reach = np.zeros(4, np.int64), inner
+        for d in rng.permutation(4):
+            strides[d] = reach + rng.integers(0, 9)
+            reach = strides[d] * (sizes[d] - 1) + reach
+        return strides
+
+    met = 0
+    for trial in range(3000):
+        sizes = rng.integers(1, 4, 4)
+        inner = int(rng.integers(1, 5))
+        strides = nested(sizes, inner + 3)
+        other, other_inner = sizes.copy(), int(rng.integers(1, 5))
+        other[2:] = rng.integers(1, 4, 2)
+        same = rng.random() < 0.6 and all(other <= sizes)
+        other_strides = strides if same else nested(other, other_inner)
+        x, y = (sizes, strides, 4096, inner), (other, other_strides, 4096 + int(rng.integers(-30, 60)), other_inner)
+        states = (State * 2)(state_of(*x), state_of(*y))
+        args = Args(states=ctypes.addressof(states), count=2, B=int(sizes[0]), W=int(sizes[1]), beams=1 << 40)
+        shared = bool(bytes_of(*x) & bytes_of(*y))
+        met += shared
+        assert check(ctypes.byref(args)) == (1 if shared else 0), (trial, x, y)
+    assert 300 < met < 2700
