@@ -70,8 +70,9 @@ __device__ __forceinline__ int named(const Rows& r, const Teacher& t, int64_t en
 }
 
 // s = sum 2^((x - m) k) of some logits, m one of them near the largest (-inf: of none but
-// -inf).  k is one float in the sums and everywhere else: a temperature that is off by
-// 3e-8 of itself moves a loss by that share of sum (Q - P) x / tau.
+// -inf).  k + klo of fp32 logits, for all other types (klo = 0) the same one float here
+// and everywhere else: a temperature that is off by up to 6e-8 of itself moves a loss by
+// that share of sum (Q - P) x / tau, and a gradient by less than it is rounded to.
 struct Sum {
     float m = -__builtin_inff();
     double s = 0.0;
@@ -84,7 +85,15 @@ struct Sum {
     }
 };
 // 1 / tau
-__device__ __forceinline__ double inverse_tau(const Rows& r) { return double(r.k) * 0.693147180559945309417; }
+__device__ __forceinline__ double inverse_tau(const Rows& r) {
+    return (double(r.k) + double(r.klo)) * 0.693147180559945309417;
+}
+// d log2(e) / tau of a difference
+template <class T>
+__device__ __forceinline__ float scaled(const Rows& r, float d) {
+    if constexpr (std::is_same_v<T, float>) return seqlogp::scaled(r, d);
+    else return d * r.k;
+}
 
 __device__ __forceinline__ void leave_out(const Out& o, int64_t at) {
     if (o.reduction == DOT_REDUCE_NONE) o.out[at] = 0.0f;
@@ -339,7 +348,11 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
     // x k - m k in one rounding where m k has digits behind the point
     const bool near = fabsf(mk) < 65536.0f;
     if (near) {
-        auto term = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, r.k, -mk)); };
+        auto term = [&](float x) {
+            float y = fmaf(x, r.k, -mk);
+            if constexpr (std::is_same_v<T, float>) y = fmaf(x, r.klo, y);
+            return __builtin_amdgcn_exp2f(y);
+        };
         a.s = double(term(before)) + double(term(behind));
         auto sum = [&](const float* f) {
             float y[PN];
@@ -350,7 +363,8 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
         if (stream) each(sum, std::true_type{});
         else each(sum, std::false_type{});
         a.s = wave_sum64(a.s);
-        a.s *= short_exp((double(mk) - double(m) * double(r.k)) * 0.693147180559945309417);  // what rounding m k left
+        // what rounding m k left
+        a.s *= short_exp((double(mk) - double(m) * (double(r.k) + double(r.klo))) * 0.693147180559945309417);
     }
     if (!near || a.s > 0x1p60) {
         // the largest logit of all, then the terms; from the caches
@@ -364,7 +378,7 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
         }, std::false_type{});
         m = a.m = wave_max(m);
         const float base = m == none ? 0.0f : m;
-        auto term = [&](float x) { return double(__builtin_amdgcn_exp2f((x - base) * r.k)); };
+        auto term = [&](float x) { return double(__builtin_amdgcn_exp2f(scaled<T>(r, x - base))); };
         a.s = term(before) + term(behind);
         if (groups) {
 #pragma unroll
@@ -518,7 +532,7 @@ __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     const float up = g.grad_out[g.grad_out_scalar ? 0 : g.reduction == DOT_REDUCE_NONE ? at : b];
     const float c = (g.reduction == DOT_REDUCE_MEAN ? up * g.weight[b] : up) * g.inv_tau;
     const float scale = c * st.y;
-    auto value = [&](float x) { return __builtin_amdgcn_exp2f((x - st.x) * r.k) * scale; };
+    auto value = [&](float x) { return __builtin_amdgcn_exp2f(scaled<T>(r, x - st.x)) * scale; };
     const bool together = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     auto pack_in = [&](int p, auto stream) {
         const T* at_p = row + sp.head + int64_t(p) * PN;

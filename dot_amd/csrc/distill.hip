@@ -56,7 +56,13 @@ seqlogp::Rows rows_of(const A* a, bool training, bool backward) {
     r.S = a->S;
     r.V = a->V;
     r.mask = a->mask;
-    r.k = float(1.4426950408889634074 / a->tau);
+    const double k = 1.4426950408889634074 / a->tau;
+    r.k = float(k);
+    r.klo = 0.0f;
+    if (a->dtype == DOT_F32) {  // klo > 0, as in the sequence log-probabilities
+        if (double(r.k) >= k) r.k = std::nextafter(r.k, 0.0f);
+        r.klo = float(k - double(r.k));
+    }
     r.splits = splits_of(a->B, a->S, a->V, a->dtype, backward);
     // past the caches but for the rows that the backward begins with, as for the
     // sequence log-probabilities
