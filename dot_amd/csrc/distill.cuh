@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Pa
             float y[PN];
 #pragma unroll
             for (int i = 0; i < PN; ++i) y[i] = term(f[i]);
-            a.s += double(seqlogp::pairwise<PN>(y));
+            a.s += double(pairwise<PN>(y));
         };
         if (stream) each(sum, std::true_type{});
         else each(sum, std::false_type{});

@@ -99,13 +99,6 @@ __device__ __forceinline__ const void* nothing_of(float) { return kNothing[DOT_F
 __device__ __forceinline__ const void* nothing_of(F16) { return kNothing[DOT_F16]; }
 __device__ __forceinline__ const void* nothing_of(BF16) { return kNothing[DOT_BF16]; }
 
-// Sum of N values, pairwise.
-template <int N>
-__device__ __forceinline__ float pairwise(const float* x) {
-    if constexpr (N == 1) return x[0];
-    else return pairwise<N / 2>(x) + pairwise<N - N / 2>(x + N / 2);
-}
-
 // Largest value and sum of 2^((x - m) k) so far; m = -inf: nothing but -inf.
 struct MaxSum {
     float m = -__builtin_inff();

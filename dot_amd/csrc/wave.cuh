@@ -84,6 +84,14 @@ __device__ __forceinline__ double wave_sum64(double x) {
     return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
 }
 
+// Sum of N values of a lane, pairwise: of the 4 or 8 terms of a pack, before they enter a
+// 64-bit sum, at most 3 roundings (2e-7 of their sum, of either sign).
+template <int N>
+__device__ __forceinline__ float pairwise(const float* x) {
+    if constexpr (N == 1) return x[0];
+    else return pairwise<N / 2>(x) + pairwise<N - N / 2>(x + N / 2);
+}
+
 // Orders this wave's LDS writes before its later LDS reads.
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
