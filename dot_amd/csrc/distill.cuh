@@ -228,8 +228,8 @@ __device__ __forceinline__ void only_first(int K, const int* list, Entries& in) 
 //
 // Bound by HBM in long rows (about 4500 of 131072 bf16: 218 us, 5.4 TB/s), in shorter ones by
 // what a workgroup does before and behind its logits as well (as
-// many of 32768, 64 entries: 72 us, 4.1 TB/s; half of 774 of 50021 fp32, 100 entries:
-// 23 us), and by latency in few (74 of 1000 fp32: 6.1 us).  seqlogp::kUnroll
+// many of 32768, 64 entries: 67 us, 4.4 TB/s; half of 774 of 50021 fp32, 100 entries:
+// 22 us), and by latency in few (74 of 1000 fp32: 6.2 us).  seqlogp::kUnroll
 // packs at once: 2 and 8 of them, or a bound on registers for more workgroups, were slower.
 template <class T>
 __global__ __launch_bounds__(kBlock) void row_stats(Rows r, Teacher t, Out o, Part* parts) {
@@ -509,7 +509,7 @@ struct GradArgs {
 };
 
 // dx of one span of a row.  Bound by HBM: 8192 rows of 131072 bf16, 55 % of them read,
-// 3.3 GB in 670 us, 4.9 TB/s; 8184 of 32768, 0.83 GB in 152 us, 5.5 TB/s.
+// 3.3 GB in 666 us, 5.0 TB/s; 8184 of 32768, 0.83 GB in 148 us, 5.6 TB/s.
 template <class T>
 __global__ __launch_bounds__(kBlock) void backward(Rows r, GradArgs g) {
     // last rows first: the forward has just read them

@@ -8,9 +8,9 @@
 // of several is read from memory once.
 //
 // Bound by HBM.  16 caches of 8 x 4 x 8 x 1024 x 128 bf16, three quarters of the
-// positions in use, 0.98 GB: 205 us; with loads and stores that stay in the caches 213,
-// and with each workgroup striding through one state of its own 215 (226): neighbouring
-// workgroups at neighbouring places meet open pages of the memory.
+// positions in use, 0.98 GB: 201 us; on inputs that take 205, loads and stores that stay in
+// the caches 213, and each workgroup striding through one state of its own 215 (226):
+// neighbouring workgroups at neighbouring places meet open pages of the memory.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -15,8 +15,8 @@
 // (ascending).  -inf and NaN are never selected.
 //
 // The logits are read once; everything else is small next to them (4096 x 131072 bf16
-// and 64 entries: 1.07 GB of logits, 4 MB of entries).  4096 x 131072 bf16 takes 219 us in
-// the scan, 4.9 TB/s, the rate of a large copy, and 23 us in the join.
+// and 64 entries: 1.07 GB of logits, 4 MB of entries).  4096 x 131072 bf16 takes 191 us in
+// the scan, 5.6 TB/s, and 20 us in the join.
 #pragma once
 
 #include <type_traits>
@@ -178,9 +178,10 @@ __device__ __forceinline__ float reached_by(const float (&v)[G], int r) {
 // largest entry is found by bisection over all of them instead.
 //
 // Bound by HBM where there are many spans; where they are few, by one workgroup's way
-// through its phases: 8 rows of 32768 bf16, 20 entries, 8.8 us, of which the loads are
-// half; 240 rows of 50021 fp32 in 4 spans, 96 entries, 17.7 us for 48 MB.  16 packs a
-// thread, not 8: half the lists for the join, and 4096 x 131072 bf16 took 297 us with 8.
+// through its phases: 8 rows of 32768 bf16, 20 entries, 8.6 us, of which the loads are
+// half; 240 rows of 50021 fp32 in 4 spans, 96 entries, 17.4 us for 48 MB.  16 packs a
+// thread, not 8: half the lists for the join, and 4096 x 131072 bf16 took 297 us with 8
+// where 16 took 219.
 template <class T, int P, bool DIRECT>
 __global__ __launch_bounds__(kBlock, 4) void scan(Rows r, Lists lists, TopOut out) {
     constexpr int PN = Pack<T>::N;
@@ -622,9 +623,9 @@ inline size_t join_shared(int R, int waves, int beams, int entries) {
 // EACH entries of a thread stay in registers; with 0 they are read again.
 //
 // One workgroup a list, so bound by its latency: the sums of the spans, a bound, what
-// reaches it, the ranks.  4 beams, 8 entries and 16 spans each 4.9 us; 8 beams, 16
-// entries and 4 spans 7; 48 beams, 96 entries and 4 spans 18.5; 4096 rows of 4 spans
-// and 64 entries 20 to 24, 999 of 128 entries 13.
+// reaches it, the ranks.  4 beams, 4 entries and 16 spans each 5.1 us; 8 beams, 16
+// entries and 4 spans 6.6; 48 beams, 96 entries and 4 spans 18.2; 4096 rows of 4 spans
+// and 64 entries 20, 999 of 128 entries 12.
 template <int R, bool BEAM, int EACH>
 __global__ __launch_bounds__(1024) void join(Rows r, Lists lists, JoinArgs a) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
