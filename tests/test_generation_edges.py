@@ -255,3 +255,45 @@ def test_gradients_of_far_tokens_have_no_common_error(dev, sign):
         up = (0.5 + np.random.default_rng(0).random((1, 2))).astype(np.float32)  # as check_distill draws it
         want = oracle.distill_grad(logits.shape, parts, up, tau)[..., 2:]
         assert np.abs((g.numpy()[..., 2:] / want - 1).mean(-1)).max() < 5e-7
+
+
+# ---------------------------------------------------------------------------
+# Small and uneven rows
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_a_vocabulary_of_one(dev, dtype):
+    rng = np.random.default_rng(6)
+    logits = torch.as_tensor(rng.standard_normal((2, 128, 1)).astype(np.float32)).to(DTYPES[dtype])
+    logits[1, 5] = -float("inf")
+    check_top(dot_amd.top_logp(logits.to(dev), 1), logits, 1)
+    scores = -np.sort(rng.random((2, 128)), 1)
+    r = dot_amd.beam_step(logits.to(dev), torch.as_tensor(scores.astype(np.float32)).to(dev))
+    check_beam(r, logits, scores, 128)
+    logits = logits[:, 6:]  # a position without an allowed token has no divergence to compare
+    logp, tokens = np.full((2, 122, 1), -0.25, np.float32), np.zeros((2, 122, 1), np.int64)
+    for direction, rest in (("forward", "none"), ("reverse", "bucket")):
+        distill(dev, logits, torch.as_tensor(logp), tokens, direction=direction, rest=rest)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("filler", ["-inf", "lowest", "low"])
+@pytest.mark.parametrize("V", [5000, 40000])
+def test_distillation_behind_a_filler(dev, dtype, V, filler):
+    """Rows that begin with tokens that are not allowed, as long as a workgroup's first packs and longer."""
+    print(f"[edges] filler {dev} {dtype} V={V} {filler}", flush=True)
+    rng = np.random.default_rng(V)
+    x = logits_of(rng, (1, 4, V), DTYPES[dtype])
+    value = {"-inf": -float("inf"), "lowest": torch.finfo(x.dtype).min, "low": -1e4}[filler]
+    logp, tokens = teacher_of(rng, x[..., V // 2 :], 30, tau=0.7)
+    tokens = tokens + V // 2
+    for row, n in enumerate((1, 4096, V // 2 - 1, V // 2)):
+        x[0, row, :n] = value
+    for direction, rest in (("forward", "bucket"), ("forward", "none"), ("reverse", "bucket")):
+        out, g = distill(dev, x, torch.as_tensor(logp), tokens, tau=0.7, direction=direction, rest=rest, reduction="none")
+        # where a named token is not allowed P log Q is -inf: 4096 tokens are more than half of 5000
+        named = torch.as_tensor(np.take_along_axis(x.float().numpy(), tokens, -1))
+        if filler == "-inf":
+            assert torch.equal(torch.isinf(out), torch.isinf(named).any(-1) & (direction == "forward"))
+        assert not torch.isnan(out).any() and torch.isfinite(g).all()
